@@ -129,6 +129,69 @@ int lcu_attention(void* out_dev, const void* q_dev, const void* k_cache_dev, con
  * llama_cu.cu:1196-1209: probs_dev (fp16 [n_vocab], may alias logits_dev), *token_host = argmax */
 int lcu_logits_head(void* probs_dev, const void* logits_dev, int n_vocab, float temperature, int* token_host, void* stream);
 
+/* ---- long contexts: a cache in 4 bits, eviction, beams ---------------------------------------- */
+/* No counterpart in the reference, whose caches are halves and whose client runs one sequence.  dtype of these operators: 0 half,
+ * 1 bfloat16, 2 binary32 (logits only).  Lengths and positions are read on the device (a captured step replays with new ones) and
+ * are the caller's to advance.  No call allocates, waits or keeps anything; workspaces belong to the caller, 16-byte aligned, with any
+ * contents, and calls that may overlap on the GPU need one each.  Arguments are checked before anything is launched.
+ *
+ * A 4-bit cache of one layer is four planes, 16-byte aligned: codes, u8 [n_seqs][n_kv_heads][ctx_len][head_dim / 2], and scales, half
+ * [n_seqs][n_kv_heads][ctx_len][head_dim / bs], for keys and for values.  head_dim 64 or 128; bs 32, 64 or 128, at most head_dim.
+ * With a the largest magnitude of a block of bs neighbouring dimensions the scale s is a / 7.5 rounded to 7 significant bits, at most
+ * 8704; x becomes floor(x / s + 8) within 0 .. 15 (8 where s is 0) and stands for (code - 7.5) * s, which a half holds exactly.  A block
+ * with an infinity or a NaN gets the scale NaN: rows that see it come out as NaN, others do not.  The codes of dimensions
+ * 32 g + 8 o .. + 7 are the nibbles, lowest first, of the row's little-endian 32-bit word o * (head_dim / 32) + g. */
+/* The counterpart of lcu_rope_scatter: m new rows for each of n_seqs sequences.  Row i of sequence s (row s * m + i of q, k_new and v_new,
+ * which lie ld_q / ld_kv elements apart, multiples of 8, 16-byte aligned) goes to row lengths[s] + i of its caches, at rotary position
+ * positions[s] + i (NULL: lengths[s] + i).  Neighbouring pairs are rotated by position * theta^(-2i / head_dim), angles in binary64;
+ * theta 0: no rotation.  Rotated queries go to q_out [n_seqs * m][n_heads * head_dim] (which may be q if ld_q is that; q NULL: none).
+ * Rows beyond ctx_len are not written, nor any of a sequence with a negative length (its queries are rotated all the same). */
+int lcu_cache4_append(void* k_codes_dev, void* k_scales_dev, void* v_codes_dev, void* v_scales_dev, void* q_out_dev, const void* q_dev, int ld_q,
+                      const void* k_new_dev, const void* v_new_dev, int ld_kv, const int32_t* lengths_dev, const int32_t* positions_dev, int n_seqs,
+                      int m, int n_heads, int n_kv_heads, int head_dim, int bs, int ctx_len, float theta, int dtype, void* stream);
+/* rows first[s] .. first[s] + count (first NULL: 0) of every sequence and head as values, [n_seqs][n_kv_heads][count][head_dim]; k_out or
+ * v_out may be NULL.  Rows outside 0 .. ctx_len read as zeros. */
+int lcu_cache4_read(void* k_out_dev, void* v_out_dev, const void* k_codes_dev, const void* k_scales_dev, const void* v_codes_dev,
+                    const void* v_scales_dev, const int32_t* first_dev, int n_seqs, int count, int n_kv_heads, int head_dim, int bs, int ctx_len,
+                    int dtype, void* stream);
+/* The counterpart of lcu_attention: m rows of q per sequence, rotated, over caches that hold their own rows already (lengths as given to
+ * lcu_cache4_append): row i of sequence s sees rows 0 .. lengths[s] + i.  n_heads is a multiple of n_kv_heads; head h reads key/value head
+ * h / (n_heads / n_kv_heads).  Scores are divided by sqrt(head_dim).  max_len: a bound on lengths[s] + m, at most ctx_len (rows beyond it are
+ * not seen).  A row that sees nothing (a negative length) gives zeros.
+ * weights (NULL: not wanted), binary32 [n_seqs][n_kv_heads][ctx_len]: = beta * weights + the probabilities that the cached row received from
+ * all m rows and the heads that read it, summed in a fixed order.  The call's own rows, from lengths[s] on, start from nothing, whatever
+ * their entries held; with beta 0 all do.  Entries of rows that none sees stay as they are.  The workspace is lcu_attention_cache4_workspace bytes (0 where none is needed). */
+uint64_t lcu_attention_cache4_workspace(int n_seqs, int m, int n_heads, int n_kv_heads, int head_dim, int max_len, int weights);
+int lcu_attention_cache4(void* out_dev, int ld_out, void* weights_dev, float beta, const void* q_dev, int ld_q, const void* k_codes_dev,
+                         const void* k_scales_dev, const void* v_codes_dev, const void* v_scales_dev, const int32_t* lengths_dev, int n_seqs, int m,
+                         int n_heads, int n_kv_heads, int head_dim, int bs, int ctx_len, int max_len, int dtype, void* workspace_dev,
+                         uint64_t workspace_bytes, void* stream);
+/* Rows that received little weight leave a cache of any format.  Of sequence s, head h the `recent` latest rows are kept and, of the others,
+ * the keep - recent with the largest weights ([n_seqs][n_kv_heads][ctx_len], binary32; ties: lowest row; a NaN is less than everything), in
+ * their order: kept [n_seqs][n_kv_heads][keep] lists them, -1 behind the last (sequences of up to keep rows keep all).  Row kept[i] of every
+ * plane moves to row i.  A plane is [n_seqs][n_kv_heads][ctx_len] rows of row_bytes[i] bytes (even, up to 65536; codes, scales, halves, the
+ * weights themselves); up to 8 of them (0: only the list is wanted); host arrays of device pointers.  Each destination,
+ * [n_seqs][n_kv_heads][dst_ctx_len], is its source (dst_ctx_len = ctx_len then) or does not overlap any source; its rows behind the last kept
+ * one stay as they are.  lengths_out (NULL: not wanted; may be lengths) = min(lengths, keep).  Keys stay rotated as they are: new rows go on
+ * at the position that the sequence had, which lcu_cache4_append takes beside the length.  All heads of a sequence keep as many rows. */
+int lcu_cache_evict(void* const* dst_planes, const void* const* src_planes, const int* row_bytes, int n_planes, const void* weights_dev,
+                    int32_t* kept_dev, int32_t* lengths_out_dev, const int32_t* lengths_dev, int n_seqs, int n_kv_heads, int ctx_len, int dst_ctx_len,
+                    int keep, int recent, void* stream);
+/* Beam search, one step of n_groups groups of `beams` beams (1 to 32).  Row g * beams + b of logits (ld elements apart) belongs to beam b of
+ * group g, whose score so far is scores[g][b].  The n_out (up to 64) best of scores[b] + log softmax(logits[b])[v] over beams and tokens,
+ * best first: parents (b), tokens (v) and scores_out, [n_groups][n_out].  Compared in binary64; ties go to the lowest beam, then the lowest
+ * token.  A NaN among logits counts as minus infinity; beams whose score is not finite, or whose logits have no finite maximum, offer all
+ * their tokens at minus infinity. */
+uint64_t lcu_beam_select_workspace(int n_groups, int beams, int n_vocab, int n_out);
+int lcu_beam_select(int32_t* parents_dev, int32_t* tokens_dev, float* scores_out_dev, const void* logits_dev, int ld, int dtype, const float* scores_dev,
+                    int n_groups, int beams, int n_vocab, int n_out, void* workspace_dev, uint64_t workspace_bytes, void* stream);
+/* The caches follow: rows 0 .. lengths[parent] of sequence g * beams + parents[g][b] go to sequence g * beams + b, in planes as above
+ * ([n_groups * beams][n_kv_heads][ctx_len] rows); other rows stay as they are.  lengths [n_groups * beams] are those before the step.  A plane whose
+ * destination is its source is permuted in place, any other destination must not overlap a source.  A parent outside 0 .. beams - 1
+ * leaves the destination's sequence as it is. */
+int lcu_cache_reorder(void* const* dst_planes, const void* const* src_planes, const int* row_bytes, int n_planes, const int32_t* parents_dev,
+                      const int32_t* lengths_dev, int n_groups, int beams, int n_kv_heads, int ctx_len, void* stream);
+
 /* ---- synthetic data ------------------------------------------------------------------------- */
 /* out[i] = fp16(scale * z(seed, name, first + i)), z approximately N(0,1), reproducible on any host */
 int lcu_synth_fill_f16(void* out_dev, uint64_t n, uint64_t seed, const char* name, float scale, uint64_t first, void* stream);

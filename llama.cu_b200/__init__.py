@@ -55,6 +55,14 @@ _SIG = {
     "lcu_rope_scatter_static": (C.c_int, [vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp]),
     "lcu_attention": (C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp]),
     "lcu_logits_head": (C.c_int, [vp, vp, C.c_int, C.c_float, C.POINTER(C.c_int), vp]),
+    "lcu_cache4_append": (C.c_int, [vp] * 6 + [C.c_int, vp, vp, C.c_int, vp, vp] + [C.c_int] * 7 + [C.c_float, C.c_int, vp]),
+    "lcu_cache4_read": (C.c_int, [vp] * 7 + [C.c_int] * 7 + [vp]),
+    "lcu_attention_cache4_workspace": (C.c_uint64, [C.c_int] * 7),
+    "lcu_attention_cache4": (C.c_int, [vp, C.c_int, vp, C.c_float, vp, C.c_int] + [vp] * 5 + [C.c_int] * 9 + [vp, C.c_uint64, vp]),
+    "lcu_cache_evict": (C.c_int, [vp, vp, vp, C.c_int, vp, vp, vp, vp] + [C.c_int] * 6 + [vp]),
+    "lcu_cache_reorder": (C.c_int, [vp, vp, vp, C.c_int, vp, vp] + [C.c_int] * 4 + [vp]),
+    "lcu_beam_select_workspace": (C.c_uint64, [C.c_int] * 4),
+    "lcu_beam_select": (C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, vp] + [C.c_int] * 4 + [vp, C.c_uint64, vp]),
     "lcu_selftest_bounded_wait": (C.c_int, [C.POINTER(C.c_int)]),
     "lcu_operator_error_word": (C.c_int, [C.POINTER(vp)]),
     "lcu_operator_status": (C.c_int, [C.POINTER(C.c_int)]),
@@ -312,6 +320,99 @@ def synth_f16(n, seed, name, scale, first=0):
     check(lib.lcu_synth_fill_f16(d.ptr, n, seed, name.encode(), scale, first, None))
     check(lib.lcu_synchronize())
     return d.to_host(np.uint16, (n,))
+
+
+OP_DTYPES = {"float16": 0, "bfloat16": 1, "float32": 2}  # number formats of the operators over 4-bit caches and of the beam selection
+
+
+def _pointers(buffers):
+    return (vp * len(buffers))(*[b.ptr for b in buffers])
+
+
+def beam_select(logits, scores, n_out, dtype="float32"):
+    """The n_out best continuations of every group of beams: logits [groups, beams, n_vocab] (binary32, or 16-bit patterns as uint16),
+    scores [groups, beams]; returns (parents, tokens, scores), each [groups, n_out], best first."""
+    logits = np.ascontiguousarray(logits)
+    groups, beams, n_vocab = logits.shape
+    dl, ds = DeviceBuffer.from_host(logits), DeviceBuffer.from_host(np.asarray(scores, np.float32))
+    out = [DeviceBuffer(groups * n_out * 4) for _ in range(3)]
+    ws = DeviceBuffer(max(16, lib.lcu_beam_select_workspace(groups, beams, n_vocab, n_out)))
+    check(lib.lcu_beam_select(out[0].ptr, out[1].ptr, out[2].ptr, dl.ptr, n_vocab, OP_DTYPES[dtype], ds.ptr, groups, beams, n_vocab, n_out, ws.ptr, ws.nbytes, None))
+    check(lib.lcu_synchronize())
+    return tuple(b.to_host(t, (groups, n_out)) for b, t in zip(out, (np.int32, np.int32, np.float32)))
+
+
+class Cache4:
+    """One layer's cache in 4 bits for several sequences, with the weight that every row has received.  Host arrays in and out (16-bit
+    patterns as uint16); `lengths` rows are held, the next row's position is `positions`."""
+
+    def __init__(self, n_seqs, n_kv_heads, head_dim, ctx_len, bs=32, dtype="float16"):
+        self.n_seqs, self.n_kv, self.hd, self.ctx, self.bs, self.dtype = n_seqs, n_kv_heads, head_dim, ctx_len, bs, OP_DTYPES[dtype]
+        rows = n_seqs * n_kv_heads * ctx_len
+        self.row_bytes = [head_dim // 2, 2 * head_dim // bs] * 2 + [4]
+        self.planes = [DeviceBuffer(rows * b) for b in self.row_bytes]  # codes and scales of the keys, of the values; weights
+        for p in self.planes:
+            check(lib.lcu_memset(p.ptr, 0, p.nbytes))
+        self.lengths, self.positions = np.zeros(n_seqs, np.int32), np.zeros(n_seqs, np.int32)
+
+    def _shape(self):
+        return self.n_kv, self.hd, self.bs, self.ctx
+
+    def append(self, q, k, v, theta=10000.0):
+        """Rows q [seqs, m, heads * hd], k, v [seqs, m, kv * hd] at the sequences' ends; returns the rotated queries.  `advance` counts them."""
+        q, k, v = (np.ascontiguousarray(a, np.uint16) for a in (q, k, v))
+        m, heads = q.shape[1], q.shape[2] // self.hd
+        dq, dk, dv, dl, dp = (DeviceBuffer.from_host(a) for a in (q, k, v, self.lengths, self.positions))
+        check(lib.lcu_cache4_append(*[p.ptr for p in self.planes[:4]], dq.ptr, dq.ptr, q.shape[2], dk.ptr, dv.ptr, k.shape[2], dl.ptr, dp.ptr,
+                                    self.n_seqs, m, heads, *self._shape(), theta, self.dtype, None))
+        check(lib.lcu_synchronize())
+        return dq.to_host(np.uint16, q.shape)
+
+    def attend(self, q, beta=1.0):
+        """Attention of rotated queries [seqs, m, heads * hd] whose own rows are in the cache but not yet counted; the rows' weights become
+        beta times the old ones plus what they receive now."""
+        q = np.ascontiguousarray(q, np.uint16)
+        m, heads, most = q.shape[1], q.shape[2] // self.hd, min(self.ctx, max(1, int(self.lengths.max()) + q.shape[1]))
+        dq, dl, do = DeviceBuffer.from_host(q), DeviceBuffer.from_host(self.lengths), DeviceBuffer(q.nbytes)
+        ws = DeviceBuffer(max(16, lib.lcu_attention_cache4_workspace(self.n_seqs, m, heads, self.n_kv, self.hd, most, 1)))
+        check(lib.lcu_attention_cache4(do.ptr, q.shape[2], self.planes[4].ptr, beta, dq.ptr, q.shape[2], *[p.ptr for p in self.planes[:4]], dl.ptr, self.n_seqs, m,
+                                       heads, *self._shape(), most, self.dtype, ws.ptr, ws.nbytes, None))
+        check(lib.lcu_synchronize())
+        return do.to_host(np.uint16, q.shape)
+
+    def advance(self, m):
+        """Counts m rows of every sequence in use."""
+        used = self.lengths >= 0
+        self.lengths[used] = np.minimum(self.lengths[used] + m, self.ctx)
+        self.positions[used] += m
+
+    def evict(self, keep, recent):
+        """Leaves `keep` rows of every sequence and head: the `recent` latest and the ones with most weight.  Returns their old places."""
+        dl, kept = DeviceBuffer.from_host(self.lengths), DeviceBuffer(self.n_seqs * self.n_kv * keep * 4)
+        planes = _pointers(self.planes)
+        check(lib.lcu_cache_evict(planes, planes, (C.c_int * 5)(*self.row_bytes), 5, self.planes[4].ptr, kept.ptr, dl.ptr, dl.ptr, self.n_seqs, self.n_kv, self.ctx,
+                                  self.ctx, keep, recent, None))
+        check(lib.lcu_synchronize())
+        self.lengths = dl.to_host(np.int32, (self.n_seqs,))
+        return kept.to_host(np.int32, (self.n_seqs, self.n_kv, keep))
+
+    def reorder(self, parents):
+        """Sequences as beams of groups, parents [groups, beams]: beam b goes on from beam parents[g, b]."""
+        parents = np.ascontiguousarray(parents, np.int32)
+        groups, beams = parents.shape
+        dp, dl, planes = DeviceBuffer.from_host(parents), DeviceBuffer.from_host(self.lengths), _pointers(self.planes)
+        check(lib.lcu_cache_reorder(planes, planes, (C.c_int * 5)(*self.row_bytes), 5, dp.ptr, dl.ptr, groups, beams, self.n_kv, self.ctx, None))
+        check(lib.lcu_synchronize())
+        at = (np.arange(groups)[:, None] * beams + parents).ravel()
+        self.lengths, self.positions = self.lengths[at].copy(), self.positions[at].copy()
+
+    def read(self, count, first=None):
+        """Keys and values of `count` rows from row first[s] on, as 16-bit patterns [seqs, kv, count, hd]."""
+        df = None if first is None else DeviceBuffer.from_host(np.asarray(first, np.int32))
+        out = [DeviceBuffer(self.n_seqs * self.n_kv * count * self.hd * 2) for _ in range(2)]
+        check(lib.lcu_cache4_read(out[0].ptr, out[1].ptr, *[p.ptr for p in self.planes[:4]], df.ptr if df else None, self.n_seqs, count, *self._shape(), self.dtype, None))
+        check(lib.lcu_synchronize())
+        return tuple(b.to_host(np.uint16, (self.n_seqs, self.n_kv, count, self.hd)) for b in out)
 
 
 class Model:

@@ -1,0 +1,233 @@
+// Selection over beams and vocabulary: the n best of scores[b] + log softmax(logits[b])[v] of every group of beams.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "cache4.cuh"
+#include "cache_rows.cuh"
+
+namespace lcu {
+namespace {
+
+constexpr int BEAM_THREADS = 256, BEAM_ITEMS = 16, BEAM_CHUNK = BEAM_THREADS * BEAM_ITEMS, BEAM_MAX_OUT = 64;
+constexpr size_t BEAM_MAX_SMEM = 160 * 1024;
+
+struct beam_args {
+  beam_params p;
+  int chunks;
+  float2* stats;        // [rows][chunks] maximum and sum of e^(x - maximum)
+  uint64_t* best;       // [rows][chunks][n_out] order of the logit above ~token; 0 = none
+};
+
+__device__ __forceinline__ float logit_at(const float* p, size_t i) { return p[i]; }
+__device__ __forceinline__ float logit_at(const __half* p, size_t i) { return __half2float(p[i]); }
+__device__ __forceinline__ float logit_at(const __nv_bfloat16* p, size_t i) { return __bfloat162float(p[i]); }
+
+// order of binary32 numbers as unsigned integers (-0 as 0), and back
+__device__ __forceinline__ uint32_t float_order(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float order_float(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ uint64_t double_order(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+  return b ^ ((b >> 63) ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ double order_double(uint64_t k) { return __longlong_as_double((long long)(k ^ ((k >> 63) ? 1ull << 63 : ~0ull))); }
+
+// One CTA per (row of logits, chunk of 4096): maximum, sum of exponentials, and the chunk's n best tokens.  A logit's order and its
+// token's complement make one 64-bit number that no other token has, so ties go to the lowest token by themselves.  Every thread keeps
+// the largest of its 16; the n-th largest of those 256 is below the n-th largest of all, and at most n threads hold numbers from it
+// on - 16 n candidates at most, about n as a rule - whose ranks are counted.
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args a) {
+  __shared__ uint64_t tops[BEAM_THREADS];
+  __shared__ uint64_t cand[BEAM_MAX_OUT * BEAM_ITEMS];
+  __shared__ float s_max[8];
+  __shared__ double s_sum[8];
+  __shared__ uint64_t s_threshold;
+  __shared__ int s_count;
+  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n_out = a.p.n_out, v0 = chunk * BEAM_CHUNK;
+  const T* x = reinterpret_cast<const T*>(a.p.logits) + (size_t)row * a.p.ld;
+  if (tid == 0) {
+    s_count = 0;
+    s_threshold = 0;
+  }
+  uint64_t top = 0;
+  float mx = -INFINITY, val[BEAM_ITEMS];
+#pragma unroll
+  for (int i = 0; i < BEAM_ITEMS; ++i) {
+    const int v = v0 + i * BEAM_THREADS + tid;
+    float f = v < a.p.n_vocab ? logit_at(x, v) : -INFINITY;
+    if (f != f) f = -INFINITY;  // no number: never chosen before one
+    val[i] = f;
+    mx = fmaxf(mx, f);
+    if (v < a.p.n_vocab) top = max(top, (uint64_t)float_order(f) << 32 | (uint32_t)~v);
+  }
+  tops[tid] = top;
+  mx = warp_max(mx);
+  if (lane == 0) s_max[warp] = mx;
+  __syncthreads();
+  mx = s_max[0];
+#pragma unroll
+  for (int w = 1; w < 8; ++w) mx = fmaxf(mx, s_max[w]);
+  double sum = 0.0;
+  if (mx > -INFINITY) {
+    float part = 0.f;
+#pragma unroll
+    for (int i = 0; i < BEAM_ITEMS; ++i) part += expf(val[i] - mx);
+    sum = part;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) s_sum[warp] = sum;
+  int rank = 0;
+#pragma unroll 8
+  for (int t = 0; t < BEAM_THREADS; ++t) rank += tops[t] > top;
+  if (top && rank == n_out - 1) s_threshold = top;
+  __syncthreads();
+  if (tid == 0) {
+    double s = 0.0;
+    for (int w = 0; w < 8; ++w) s += s_sum[w];
+    a.stats[(size_t)row * a.chunks + chunk] = make_float2(mx, (float)s);
+  }
+  const uint64_t threshold = s_threshold;
+#pragma unroll
+  for (int i = 0; i < BEAM_ITEMS; ++i) {
+    const int v = v0 + i * BEAM_THREADS + tid;
+    const uint64_t k = (uint64_t)float_order(val[i]) << 32 | (uint32_t)~v;
+    if (v < a.p.n_vocab && k >= threshold) cand[atomicAdd(&s_count, 1)] = k;
+  }
+  __syncthreads();
+  const int count = s_count;
+  uint64_t* best = a.best + ((size_t)row * a.chunks + chunk) * n_out;
+  for (int c = tid; c < count; c += BEAM_THREADS) {
+    const uint64_t k = cand[c];
+    int r = 0;
+    for (int t = 0; t < count; ++t) r += cand[t] > k;
+    if (r < n_out) best[r] = k;
+  }
+  for (int r = count + tid; r < n_out; r += BEAM_THREADS) best[r] = 0;
+}
+
+struct scored {
+  uint64_t order;   // of the score in 64 bits; 0: nothing
+  uint64_t place;   // beam * n_vocab + token
+};
+__device__ __forceinline__ bool better(const scored& a, const scored& b) { return a.order > b.order || (a.order == b.order && a.place < b.place); }
+
+// One CTA per group: log-sum-exp of every beam in 64 bits, then the n best of the chunks' candidates, in the way of the first kernel.
+__global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_args a) {
+  __shared__ double lse[MAX_BEAMS], base[MAX_BEAMS];
+  __shared__ scored tops[BEAM_THREADS];
+  __shared__ scored s_threshold;
+  __shared__ int s_count;
+  extern __shared__ scored cand[];
+  const int group = blockIdx.x, tid = threadIdx.x, n_out = a.p.n_out, per_beam = a.chunks * n_out;
+  if (tid == 0) {
+    s_count = 0;
+    s_threshold = scored{0, ~0ull};
+  }
+  for (int b = tid >> 5; b < a.p.beams; b += BEAM_THREADS / 32) {
+    const float2* st = a.stats + ((size_t)group * a.p.beams + b) * a.chunks;
+    float mx = -INFINITY;
+    for (int c = tid & 31; c < a.chunks; c += 32) mx = fmaxf(mx, st[c].x);
+    mx = warp_max(mx);
+    double sum = 0.0;
+    if (mx > -INFINITY && mx < INFINITY)
+      for (int c = tid & 31; c < a.chunks; c += 32) sum += (double)st[c].y * exp((double)st[c].x - (double)mx);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((tid & 31) == 0) {
+      const float s = a.p.scores[(size_t)group * a.p.beams + b];
+      // a beam without a finite score, or whose logits have no finite maximum, offers its first tokens at minus infinity
+      const bool fine = mx > -INFINITY && mx < INFINITY && s > -INFINITY && s < INFINITY;
+      lse[b] = (double)mx + log(sum);
+      base[b] = fine ? (double)s : -INFINITY;
+    }
+  }
+  __syncthreads();
+  const int total = a.p.beams * per_beam;
+  auto at = [&](int t) {
+    const int b = t / per_beam, e = t - b * per_beam;
+    if (base[b] == -INFINITY) return e < min(n_out, a.p.n_vocab) ? scored{double_order(-INFINITY), (uint64_t)b * a.p.n_vocab + e} : scored{0, ~0ull};
+    const uint64_t k = a.best[((size_t)group * a.p.beams + b) * per_beam + e];
+    if (!k) return scored{0, ~0ull};
+    return scored{double_order((double)order_float((uint32_t)(k >> 32)) - lse[b] + base[b]), (uint64_t)b * a.p.n_vocab + (uint32_t)~(uint32_t)k};
+  };
+  scored top{0, ~0ull};
+  for (int t = tid; t < total; t += BEAM_THREADS) {
+    const scored s = at(t);
+    if (better(s, top)) top = s;
+  }
+  tops[tid] = top;
+  __syncthreads();
+  int rank = 0;
+  for (int t = 0; t < BEAM_THREADS; ++t) rank += better(tops[t], top);
+  if (top.order && rank == n_out - 1) s_threshold = top;
+  __syncthreads();
+  const scored threshold = s_threshold;
+  for (int t = tid; t < total; t += BEAM_THREADS) {
+    const scored s = at(t);
+    if (s.order && !better(threshold, s)) cand[atomicAdd(&s_count, 1)] = s;
+  }
+  __syncthreads();
+  const int count = s_count;
+  for (int c = tid; c < count; c += BEAM_THREADS) {
+    const scored s = cand[c];
+    int r = 0;
+    for (int t = 0; t < count; ++t) r += better(cand[t], s);
+    if (r < n_out) {
+      const size_t o = (size_t)group * n_out + r;
+      a.p.parents[o] = (int)(s.place / a.p.n_vocab);
+      a.p.tokens[o] = (int)(s.place % a.p.n_vocab);
+      a.p.scores_out[o] = (float)order_double(s.order);
+    }
+  }
+}
+
+int beam_chunks(int n_vocab) { return (int)ceil_div((size_t)n_vocab, BEAM_CHUNK); }
+
+}  // namespace
+
+size_t beam_select_workspace(int n_groups, int beams, int n_vocab, int n_out) {
+  return (size_t)n_groups * beams * beam_chunks(n_vocab) * (sizeof(float2) + (size_t)n_out * sizeof(uint64_t));
+}
+
+int launch_beam_select(const beam_params& p, int dtype, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  LCU_REQUIRE(p.parents && p.tokens && p.scores_out && p.logits && p.scores, "beam_select: a null pointer");
+  LCU_REQUIRE(dtype == OP_F16 || dtype == OP_BF16 || dtype == OP_F32, "beam_select: number format %d is not 0 (half), 1 (bfloat16) or 2 (binary32)", dtype);
+  LCU_REQUIRE(p.n_groups >= 1 && p.beams >= 1 && p.beams <= MAX_BEAMS, "beam_select: %d groups of %d beams (1 to %d)", p.n_groups, p.beams, MAX_BEAMS);
+  LCU_REQUIRE(p.n_vocab >= 1 && p.n_vocab <= (1 << 24) && p.ld >= p.n_vocab, "beam_select: a vocabulary of %d in rows of %d", p.n_vocab, p.ld);
+  LCU_REQUIRE(p.n_out >= 1 && p.n_out <= BEAM_MAX_OUT && p.n_out <= (long long)p.beams * p.n_vocab, "beam_select: %d continuations (1 to %d, and no more than there are)", p.n_out,
+              BEAM_MAX_OUT);
+  LCU_REQUIRE(((uintptr_t)p.logits & (dtype == OP_F32 ? 3 : 1)) == 0, "beam_select: logits must be aligned to their type");
+  const int chunks = beam_chunks(p.n_vocab);
+  const size_t rows = (size_t)p.n_groups * p.beams, need = beam_select_workspace(p.n_groups, p.beams, p.n_vocab, p.n_out);
+  LCU_REQUIRE(rows * chunks < (1ull << 31), "beam_select: too many rows of logits");
+  LCU_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, "beam_select: %zu bytes of 16-byte aligned workspace are needed, %zu are there", need,
+              workspace ? workspace_bytes : (size_t)0);
+  // at most n_out threads hold candidates, each of them its share of all
+  const size_t total = (size_t)p.beams * chunks * p.n_out, most = std::min(total, (size_t)p.n_out * ceil_div(total, BEAM_THREADS));
+  const size_t smem = most * sizeof(scored);
+  LCU_REQUIRE(smem <= BEAM_MAX_SMEM, "beam_select: %d of %d beams over a vocabulary of %d are too many", p.n_out, p.beams, p.n_vocab);
+  if (int rc_dev = need_device()) return rc_dev;
+  static bool attr_done[16] = {};
+  int dev = 0;
+  LCU_CUDA(cudaGetDevice(&dev));
+  if (dev >= 16 || !attr_done[dev]) {
+    LCU_CUDA(cudaFuncSetAttribute(beam_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BEAM_MAX_SMEM));
+    if (dev < 16) attr_done[dev] = true;
+  }
+  beam_args a{p, chunks, (float2*)workspace, (uint64_t*)((float2*)workspace + rows * chunks)};
+  const unsigned ctas = (unsigned)(rows * chunks);
+  if (dtype == OP_F16) beam_rows_kernel<__half><<<ctas, BEAM_THREADS, 0, stream>>>(a);
+  else if (dtype == OP_BF16) beam_rows_kernel<__nv_bfloat16><<<ctas, BEAM_THREADS, 0, stream>>>(a);
+  else beam_rows_kernel<float><<<ctas, BEAM_THREADS, 0, stream>>>(a);
+  beam_group_kernel<<<p.n_groups, BEAM_THREADS, smem, stream>>>(a);
+  LCU_CUDA(cudaGetLastError());
+  return LCU_OK;
+}
+
+}  // namespace lcu

@@ -11,6 +11,8 @@
 #include "attention.cuh"
 #include "block_model.cuh"
 #include "block_ops.cuh"
+#include "cache4.cuh"
+#include "cache_rows.cuh"
 #include "gemm_tc.cuh"
 #include "gemv.cuh"
 #include "ops.cuh"
@@ -351,6 +353,76 @@ int lcu_logits_head(void* probs_dev, const void* logits_dev, int n_vocab, float 
   LCU_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
   LCU_CUDA(cudaMemcpy(token_host, d_tok + 8, 4, cudaMemcpyDeviceToHost));
   return LCU_OK;
+}
+
+// ---- long contexts: the 4-bit cache, eviction, beams
+static cache4_view cache4_planes(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int n_seqs, int n_kv_heads,
+                                 int head_dim, int bs, int ctx_len) {
+  return cache4_view{(uint8_t*)const_cast<void*>(k_codes), (__half*)const_cast<void*>(k_scales), (uint8_t*)const_cast<void*>(v_codes),
+                     (__half*)const_cast<void*>(v_scales), n_seqs, n_kv_heads, head_dim, bs, ctx_len};
+}
+int lcu_cache4_append(void* k_codes_dev, void* k_scales_dev, void* v_codes_dev, void* v_scales_dev, void* q_out_dev, const void* q_dev, int ld_q,
+                      const void* k_new_dev, const void* v_new_dev, int ld_kv, const int32_t* lengths_dev, const int32_t* positions_dev, int n_seqs,
+                      int m, int n_heads, int n_kv_heads, int head_dim, int bs, int ctx_len, float theta, int dtype, void* stream) {
+  cache4_append_params p{};
+  p.c = cache4_planes(k_codes_dev, k_scales_dev, v_codes_dev, v_scales_dev, n_seqs, n_kv_heads, head_dim, bs, ctx_len);
+  p.q_out = q_out_dev;
+  p.q = q_dev;
+  p.ld_q = ld_q;
+  p.k_new = k_new_dev;
+  p.v_new = v_new_dev;
+  p.ld_kv = ld_kv;
+  p.lengths = lengths_dev;
+  p.positions = positions_dev;
+  p.m = m;
+  p.n_heads = n_heads;
+  p.theta = theta;
+  return launch_cache4_append(p, dtype, (cudaStream_t)stream);
+}
+int lcu_cache4_read(void* k_out_dev, void* v_out_dev, const void* k_codes_dev, const void* k_scales_dev, const void* v_codes_dev,
+                    const void* v_scales_dev, const int32_t* first_dev, int n_seqs, int count, int n_kv_heads, int head_dim, int bs, int ctx_len,
+                    int dtype, void* stream) {
+  return launch_cache4_read(k_out_dev, v_out_dev, cache4_planes(k_codes_dev, k_scales_dev, v_codes_dev, v_scales_dev, n_seqs, n_kv_heads, head_dim, bs, ctx_len),
+                            first_dev, count, dtype, (cudaStream_t)stream);
+}
+uint64_t lcu_attention_cache4_workspace(int n_seqs, int m, int n_heads, int n_kv_heads, int head_dim, int max_len, int weights) {
+  return cache4_attention_workspace(n_seqs, m, n_heads, n_kv_heads, head_dim, max_len, weights != 0);
+}
+int lcu_attention_cache4(void* out_dev, int ld_out, void* weights_dev, float beta, const void* q_dev, int ld_q, const void* k_codes_dev,
+                         const void* k_scales_dev, const void* v_codes_dev, const void* v_scales_dev, const int32_t* lengths_dev, int n_seqs, int m,
+                         int n_heads, int n_kv_heads, int head_dim, int bs, int ctx_len, int max_len, int dtype, void* workspace_dev,
+                         uint64_t workspace_bytes, void* stream) {
+  cache4_attention_params p{};
+  p.c = cache4_planes(k_codes_dev, k_scales_dev, v_codes_dev, v_scales_dev, n_seqs, n_kv_heads, head_dim, bs, ctx_len);
+  p.out = out_dev;
+  p.ld_out = ld_out;
+  p.weights = (float*)weights_dev;
+  p.beta = beta;
+  p.q = q_dev;
+  p.ld_q = ld_q;
+  p.lengths = lengths_dev;
+  p.m = m;
+  p.n_heads = n_heads;
+  p.max_len = max_len;
+  return launch_attention_cache4(p, dtype, workspace_dev, workspace_bytes, (cudaStream_t)stream);
+}
+int lcu_cache_evict(void* const* dst_planes, const void* const* src_planes, const int* row_bytes, int n_planes, const void* weights_dev,
+                    int32_t* kept_dev, int32_t* lengths_out_dev, const int32_t* lengths_dev, int n_seqs, int n_kv_heads, int ctx_len, int dst_ctx_len,
+                    int keep, int recent, void* stream) {
+  return launch_cache_evict(evict_params{dst_planes, src_planes, row_bytes, n_planes, (const float*)weights_dev, kept_dev, lengths_out_dev, lengths_dev,
+                                         n_seqs, n_kv_heads, ctx_len, dst_ctx_len, keep, recent},
+                            (cudaStream_t)stream);
+}
+int lcu_cache_reorder(void* const* dst_planes, const void* const* src_planes, const int* row_bytes, int n_planes, const int32_t* parents_dev,
+                      const int32_t* lengths_dev, int n_groups, int beams, int n_kv_heads, int ctx_len, void* stream) {
+  return launch_cache_reorder(reorder_params{dst_planes, src_planes, row_bytes, n_planes, parents_dev, lengths_dev, n_groups, beams, n_kv_heads, ctx_len},
+                              (cudaStream_t)stream);
+}
+uint64_t lcu_beam_select_workspace(int n_groups, int beams, int n_vocab, int n_out) { return beam_select_workspace(n_groups, beams, n_vocab, n_out); }
+int lcu_beam_select(int32_t* parents_dev, int32_t* tokens_dev, float* scores_out_dev, const void* logits_dev, int ld, int dtype, const float* scores_dev,
+                    int n_groups, int beams, int n_vocab, int n_out, void* workspace_dev, uint64_t workspace_bytes, void* stream) {
+  return launch_beam_select(beam_params{parents_dev, tokens_dev, scores_out_dev, logits_dev, ld, scores_dev, n_groups, beams, n_vocab, n_out}, dtype, workspace_dev,
+                            workspace_bytes, (cudaStream_t)stream);
 }
 
 int lcu_synth_fill_f16(void* out_dev, uint64_t n, uint64_t seed, const char* name, float scale, uint64_t first, void* stream) {

@@ -41,6 +41,15 @@ const char* last_error();
     }                                     \
   } while (0)
 
+// for entry points that check their arguments before they look for a device
+inline int need_device() {
+  int n = 0;
+  if (cudaGetDeviceCount(&n) == cudaSuccess && n > 0) return LCU_OK;
+  cudaGetLastError();
+  set_last_error("no CUDA device is visible: this library has no CPU path");
+  return LCU_ERR_CUDA;
+}
+
 inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
 inline size_t round_up(size_t a, size_t b) { return ceil_div(a, b) * b; }
 

@@ -1,0 +1,149 @@
+"""Operators over 4-bit caches, eviction and beams: every refusal of an argument comes before a device is needed; format of the cache."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import plain_cache4 as P
+from conftest import load_package
+
+lcu = load_package()
+A = 1 << 20  # an address that nothing reads: the calls below are refused
+
+
+def refused(rc, words):
+    assert rc == 2 and words.encode() in lcu.lib.lcu_last_error(), (rc, lcu.lib.lcu_last_error())
+
+
+def append(**k):
+    a = dict(kc=A, ks=A, vc=A, vs=A, qo=A, q=A, ldq=512, k=A, v=A, ldkv=256, lengths=A, positions=None, seqs=1, m=1, heads=4, kv=2, hd=128, bs=32, ctx=64,
+             theta=10000.0, dtype=0, stream=None)
+    return lcu.lib.lcu_cache4_append(*{**a, **k}.values())
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(kc=None), "null pointer"), (dict(vs=None), "null pointer"), (dict(k=None), "null pointer"), (dict(lengths=None), "null pointer"), (dict(qo=None), "null pointer"),
+    (dict(hd=96), "head_dim 96"), (dict(hd=64, bs=128), "block size 128"), (dict(bs=16), "block size 16"), (dict(bs=0), "block size 0"), (dict(seqs=0), "no sequences"),
+    (dict(kv=0), "no sequences"), (dict(ctx=0), "no sequences"), (dict(kc=A + 8), "16-byte aligned"), (dict(ks=A + 2), "16-byte aligned"), (dict(dtype=2), "number format 2"),
+    (dict(m=0), "no rows"), (dict(heads=0), "no rows"), (dict(ldkv=248), "row strides"), (dict(ldq=516), "row strides"), (dict(k=A + 4), "16-byte aligned"),
+    (dict(ldq=520, qo=A), "must be dense"), (dict(theta=-1.0), "theta"), (dict(theta=float("nan")), "theta"), (dict(seqs=1 << 16, m=1 << 16), "too many")])
+def test_append_refuses(change, words):
+    refused(append(**change), words)
+
+
+def attend(**k):
+    a = dict(out=A, ldo=512, w=None, beta=0.0, q=A, ldq=512, kc=A, ks=A, vc=A, vs=A, lengths=A, seqs=1, m=1, heads=4, kv=2, hd=128, bs=32, ctx=64, most=64, dtype=0,
+             ws=A, bytes=1 << 40, stream=None)
+    return lcu.lib.lcu_attention_cache4(*{**a, **k}.values())
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(out=None), "null pointer"), (dict(q=None), "null pointer"), (dict(lengths=None), "null pointer"), (dict(kc=None), "null pointer"), (dict(heads=3), "3 heads over 2"),
+    (dict(m=0), "0 rows"), (dict(most=65), "exceed the cache"), (dict(most=0), "exceed the cache"), (dict(ldo=504), "row strides"), (dict(ldq=500), "row strides"),
+    (dict(q=A + 8), "16-byte aligned"), (dict(out=A + 2), "16-byte aligned"), (dict(dtype=2), "number format 2"), (dict(hd=80), "head_dim 80"),
+    (dict(w=A, ws=None), "workspace"), (dict(w=A, bytes=0), "workspace"), (dict(w=A, ws=A + 4), "workspace"), (dict(seqs=40000), "too many")])
+def test_attention_refuses(change, words):
+    refused(attend(**change), words)
+
+
+def test_read_refuses():
+    def read(**k):
+        a = dict(ko=A, vo=A, kc=A, ks=A, vc=A, vs=A, first=None, seqs=1, count=1, kv=2, hd=128, bs=32, ctx=64, dtype=0, stream=None)
+        return lcu.lib.lcu_cache4_read(*{**a, **k}.values())
+
+    refused(read(ko=None, vo=None), "nothing to read")
+    refused(read(count=0), "nothing to read")
+    refused(read(ko=A + 4), "16-byte aligned")
+    refused(read(dtype=5), "number format 5")
+    refused(read(bs=24), "block size 24")
+
+
+def planes(*addresses):
+    return (C.c_void_p * len(addresses))(*addresses)
+
+
+def test_evict_refuses():
+    def evict(**k):
+        a = dict(dst=planes(A), src=planes(A), rb=(C.c_int * 1)(64), n=1, w=A, kept=A, lo=None, lengths=A, seqs=1, kv=2, ctx=64, dctx=64, keep=10, recent=2, stream=None)
+        return lcu.lib.lcu_cache_evict(*{**a, **k}.values())
+
+    refused(evict(n=9), "9 planes")
+    refused(evict(n=-1), "-1 planes")
+    refused(evict(src=planes(None)), "plane 0 is a null pointer")
+    refused(evict(rb=(C.c_int * 1)(3)), "rows of 3 bytes")
+    refused(evict(rb=(C.c_int * 1)(0)), "rows of 0 bytes")
+    refused(evict(dst=planes(A + 1)), "odd address")
+    refused(evict(w=None), "null pointer")
+    refused(evict(kept=None), "null pointer")
+    refused(evict(keep=0), "keep 0 rows")
+    refused(evict(keep=65), "keep 65 rows")
+    refused(evict(recent=11), "keep 10 rows")
+    refused(evict(recent=-1), "keep 10 rows")
+    refused(evict(dst=planes(1 << 24), dctx=9), "into 9")
+    refused(evict(dctx=32), "in place")
+    refused(evict(seqs=0), "0 sequences")
+
+
+def test_reorder_refuses():
+    def reorder(**k):
+        a = dict(dst=planes(A), src=planes(A), rb=(C.c_int * 1)(64), n=1, parents=A, lengths=A, groups=1, beams=4, kv=2, ctx=64, stream=None)
+        return lcu.lib.lcu_cache_reorder(*{**a, **k}.values())
+
+    refused(reorder(n=0), "0 planes")
+    refused(reorder(parents=None), "null pointer")
+    refused(reorder(beams=0), "0 beams")
+    refused(reorder(beams=33), "33 beams")
+    refused(reorder(groups=0), "0 groups")
+    refused(reorder(ctx=0), "0 rows")
+
+
+def test_beam_select_refuses():
+    def select(**k):
+        a = dict(parents=A, tokens=A, out=A, logits=A, ld=100, dtype=0, scores=A, groups=1, beams=4, vocab=100, n=4, ws=A, bytes=1 << 40, stream=None)
+        return lcu.lib.lcu_beam_select(*{**a, **k}.values())
+
+    refused(select(logits=None), "null pointer")
+    refused(select(scores=None), "null pointer")
+    refused(select(dtype=3), "number format 3")
+    refused(select(beams=33), "33 beams")
+    refused(select(ld=99), "vocabulary of 100 in rows of 99")
+    refused(select(vocab=0), "vocabulary of 0")
+    refused(select(n=0), "0 continuations")
+    refused(select(n=65), "65 continuations")
+    refused(select(beams=1, vocab=3, ld=3, n=4), "4 continuations")
+    refused(select(logits=A + 1), "aligned to their type")
+    refused(select(dtype=2, logits=A + 2), "aligned to their type")
+    refused(select(bytes=16), "workspace")
+    refused(select(ws=None), "workspace")
+
+
+def test_valid_calls_need_a_device():
+    if lcu.lib.lcu_device_count() > 0:
+        pytest.skip("a GPU is present")
+    for call in (append, attend):
+        assert call() == 1 and b"no CUDA device" in lcu.lib.lcu_last_error()
+    with pytest.raises(lcu.LcuError, match="no CUDA device"):
+        lcu.beam_select(np.zeros((1, 2, 10), np.float32), np.zeros((1, 2), np.float32), 2)
+
+
+@pytest.mark.parametrize("hd,bs", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+def test_values_of_the_cache_are_exact_halves(hd, bs):
+    """Seven-bit scales: every value (code - 7.5) * scale is a half; rows come back within half a step (the largest magnitude of a block may
+    lie up to 2^-7 of itself, 0.06 steps, above 7.5 scales: still nearest to the last code)."""
+    rng = np.random.default_rng(hd + bs)
+    x = (rng.standard_normal((400, hd)) * 10.0 ** rng.uniform(-2, 3, (400, 1))).astype(np.float32)
+    s = P.scales_of(x, bs)
+    c = P.codes_of(x, s, bs)
+    v = P.values_of(c, s, bs)
+    assert (P.unpack(P.pack(c)) == c).all()
+    assert (v.astype(np.float16).astype(np.float64) == v).all()
+    assert (np.abs(v - x) <= 0.5 * np.repeat(s.astype(np.float64), bs, -1) * (1 + 2.0 ** -7) + 2.0 ** -7 * np.abs(x)).all()
+
+
+def test_plain_eviction_and_beams():
+    w = np.array([5, 1, np.nan, 1, 9, 0, 2], np.float32)
+    assert P.evict(w, 7, 4, 2) == [0, 4, 5, 6]
+    assert P.evict(w, 6, 4, 0) == [0, 1, 3, 4] and P.evict(w, 6, 5, 0) == [0, 1, 3, 4, 5]
+    assert P.evict(w, 3, 4, 1) == [0, 1, 2] and P.evict(w, -1, 4, 1) == []
+    p, t, s = P.beam_select(np.array([[0.0, 1.0], [0.0, 1.0]]), np.array([-1.0, -1.0]), 4)
+    assert p.tolist() == [0, 1, 0, 1] and t.tolist() == [1, 1, 0, 0]
