@@ -1,6 +1,6 @@
 // Attention over the 4-bit cache (cache4.cuh): o_i = sum_j p_ij v_j, p_i = softmax_j(q_i . k_j / sqrt(head_dim)) over the rows j that row i
 // sees, and on request the weight that every cached row received from the rows and heads of this call.
-#include "cache4.cuh"
+#include "cache4_attention.cuh"
 
 namespace lcu {
 namespace {
@@ -118,7 +118,11 @@ int launch_rows(const rows_args& a, cudaStream_t stream) {
 
 }  // namespace
 
-size_t cache4_attention_workspace(int n_seqs, int m, int n_heads, int, int, int, bool weights) {
+// rows that go to the kernel of few rows
+static bool few_rows(int m, int group) { return m * group <= 16 || m == 1; }
+
+size_t cache4_attention_workspace(int n_seqs, int m, int n_heads, int n_kv, int, int max_len, bool weights) {
+  if (few_rows(m, n_heads / n_kv)) return attention_cache4_step_workspace(n_seqs, m, n_heads, max_len, weights);
   return weights ? (size_t)n_seqs * m * n_heads * sizeof(float2) : 0;
 }
 
@@ -138,6 +142,7 @@ int launch_attention_cache4(const cache4_attention_params& p, int dtype, void* w
   LCU_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
               "attention_cache4: %zu bytes of 16-byte aligned workspace are needed, %zu are there", need, workspace ? workspace_bytes : (size_t)0);
   if (int rc_dev = need_device()) return rc_dev;
+  if (few_rows(p.m, p.n_heads / p.c.n_kv)) return launch_attention_cache4_step(p, dtype, workspace, stream);
   rows_args a{p, p.weights ? (float2*)workspace : nullptr};
   if (dtype == OP_F16) return p.c.hd == 128 ? launch_rows<__half, 128>(a, stream) : launch_rows<__half, 64>(a, stream);
   return p.c.hd == 128 ? launch_rows<__nv_bfloat16, 128>(a, stream) : launch_rows<__nv_bfloat16, 64>(a, stream);
