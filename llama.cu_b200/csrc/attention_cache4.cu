@@ -119,10 +119,10 @@ int launch_rows(const rows_args& a, cudaStream_t stream) {
 }  // namespace
 
 // rows that go to the kernel of few rows
-static bool few_rows(int m, int group) { return m * group <= 16 || m == 1; }
+static bool few_rows(int m, int group) { return (long long)m * group <= 16 || m == 1; }
 
-size_t cache4_attention_workspace(int n_seqs, int m, int n_heads, int n_kv, int, int max_len, bool weights) {
-  if (few_rows(m, n_heads / n_kv)) return attention_cache4_step_workspace(n_seqs, m, n_heads, max_len, weights);
+size_t cache4_attention_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
+  if (few_rows(m, n_heads / n_kv)) return attention_cache4_step_workspace(n_seqs, m, n_heads, n_kv, hd, max_len, weights);
   return weights ? (size_t)n_seqs * m * n_heads * sizeof(float2) : 0;
 }
 
@@ -132,6 +132,7 @@ int launch_attention_cache4(const cache4_attention_params& p, int dtype, void* w
   LCU_REQUIRE(dtype == OP_F16 || dtype == OP_BF16, "attention_cache4: number format %d is not 0 (half) or 1 (bfloat16)", dtype);
   LCU_REQUIRE(p.out && p.q && p.lengths, "attention_cache4: a null pointer");
   LCU_REQUIRE(p.m >= 1 && p.n_heads >= 1 && p.n_heads % p.c.n_kv == 0, "attention_cache4: %d rows, %d heads over %d key/value heads", p.m, p.n_heads, p.c.n_kv);
+  LCU_REQUIRE(p.m < (1 << 26) && p.c.ctx < (1 << 26), "attention_cache4: %d rows, %d in the cache", p.m, p.c.ctx);
   LCU_REQUIRE(p.max_len >= 1 && p.max_len <= p.c.ctx, "attention_cache4: %d rows exceed the cache's %d", p.max_len, p.c.ctx);
   LCU_REQUIRE((long long)p.n_heads * p.c.hd < (1 << 24) && (long long)p.c.n_seqs * p.m * p.n_heads < (1ll << 31) && (long long)p.c.n_seqs * p.c.n_kv < 65536,
               "attention_cache4: %d sequences of %d rows of %d heads are too many", p.c.n_seqs, p.m, p.n_heads);

@@ -1,15 +1,22 @@
 // Attention of few rows over the 4-bit cache (cache4.cuh): single tokens, and a handful of rows (a draft that is checked).
 //
 //   s_jc = q_c . k_j / sqrt(head_dim),  o_c = sum_j e^(s_jc - max) v_j / sum_j e^(s_jc - max),   columns c = (row, head of the key/value head)
-// One cluster of CTAs per (sequence, key/value head) walks the cached rows once, whatever the number of columns up to 16; CTAs share the
-// rows in runs, warps interleave tiles of 16.  What bounds it is the cache's bytes (at most 0.57 a value) and, close behind, the
-// instructions that turn nibbles into halves: 41 values a cycle and SM arrive, a value costs about one lane's instruction and a half.
-// So nothing else happens to a value: codes become code - 7.5 as halves in three bit operations per four values and one subtraction per
-// two, and go straight into the registers of m16n8k16 products, with the cached rows as the wide side (16 keys x 8 columns for the
-// scores, 16 dimensions x 8 columns for the outputs).  The order of the codes in a row (cache4.cuh) is such that a lane's words of 32
-// dimensions belong to one block of scales: scores are scaled in binary32 per block after the product, exactly; values take their scale
-// as halves, exactly too (7-bit scales).  Scores, sums and outputs are binary32; probabilities are rounded to half (2^-11) as operands.
-// The running maximum of a column is raised only when a score passes it by 8 (powers of two): e^(s - max) up to 256 fits a half.
+// What bounds it is the cache's bytes (at most 0.57 a value) and, close behind, the instructions that turn nibbles into halves: 41 values
+// a cycle and SM arrive, and bit operations issue for 64 lanes a cycle.  So as little as possible happens to a value.  The cached rows are
+// the wide side of m16n8k16 products (16 keys x 8 columns for the scores, 16 dimensions x 8 columns for the outputs), whose operands are
+// made in registers:
+//   keys: a masked nibble is a half already, the subnormal code * 2^-24 (or * 2^-20, four bits further up; those dimensions' queries
+//     are a sixteenth).  The 7.5 is a product with the column's sum of queries, where the accumulator starts.
+//   values: bits or'ed below an exponent are 1024 + code (or 64 + code); less the constant, times the scale, less 7.5 scales: exact.
+// The order of the codes in a row (cache4.cuh) is such that a lane's words of 32 dimensions belong to one block of scales: scores are
+// scaled in binary32 per block after the product, exactly; values take their scale as halves, exactly too (7-bit scales).
+// Scores, sums and outputs are binary32; probabilities are rounded to half (2^-11) as operands.  The running maximum of a column is raised
+// only when a score passes it by 8 (powers of two): e^(s - max) up to 256 fits a half.
+//
+// Work is dealt in chunks of 32 cached rows: those of all (sequence, key/value head, up to 16 columns) in a row, an equal run of them per
+// CTA, whatever the lengths (which only the device knows).  A warp's chunks come through a ring of its own in shared memory, one
+// on its way while the other is worked on.  Where a run ends inside a unit, sums go to the workspace and a second kernel joins them (and
+// forms the weights, once the sums are known).
 //
 // A block of values whose scale is no number counts as zeros in the product, and the first such row is remembered per block: columns
 // that see it get NaN there, columns of earlier rows of the same tile do not.
@@ -21,32 +28,70 @@
 namespace lcu {
 namespace {
 
-constexpr int ST_WARPS = 8, ST_THREADS = 32 * ST_WARPS, ST_TILE = 16;
+constexpr int ST_WARPS = 8, ST_THREADS = 32 * ST_WARPS, ST_TILE = 16, ST_CHUNK = 32, ST_STAGES = 3, ST_CTAS = 2 * 148;
 
 struct step_args {
   cache4_attention_params p;
-  float* scores;     // [n_seqs * m][n_heads][max_len], powers of two (weights only)
+  int ctas, col_blocks;  // of the first kernel; units per (sequence, key/value head)
+  float* parts;          // [ctas][2][cols][hd] sums of runs that begin, or end, inside a unit
+  float2* part_ml;       // [ctas][2][cols] their maxima (powers of two) and sums
+  int* part_bad;         // [ctas][2][4] first row whose values of a block are no numbers
+  float2* unit_ml;       // [units][cols] maximum and sum of units that one CTA did (weights only)
+  float* scores;         // [n_seqs * m][n_heads][max_len], powers of two (weights only)
 };
+
+// what both kernels know of the work: chunks of a sequence, places of units in the row of all chunks
+// (fewer than 2^31 chunks: the host sees to it)
+struct step_plan {
+  unsigned total, ctas;  // chunks of all units; CTAs that have any of them: one at least each
+  unsigned share, more;  // of a CTA; CTAs that have one more
+  __device__ __forceinline__ step_plan(unsigned chunks, unsigned launched) : total(chunks), ctas(min(launched, chunks)) {
+    share = ctas ? total / ctas : 0u;
+    more = total - share * ctas;
+  }
+  __device__ __forceinline__ static int chunks(const cache4_attention_params& p, int held) {
+    const int room = min(p.c.ctx, p.max_len);
+    return held < 0 ? 0 : ((held >= room ? room : min(held + p.m, room)) + ST_CHUNK - 1) / ST_CHUNK;  // (m is below 2^26, rooms too)
+  }
+  __device__ __forceinline__ unsigned first_of(unsigned cta) const { return cta * share + min(cta, more); }
+  __device__ __forceinline__ unsigned cta_of(unsigned chunk) const {
+    const unsigned long_ones = more * (share + 1);
+    return chunk < long_ones ? chunk / (share + 1) : more + (chunk - long_ones) / share;
+  }
+};
+// chunks of the sequences before `seq` (per unit of a sequence), and of all; by a whole warp
+__device__ __forceinline__ void count_chunks(const cache4_attention_params& p, int seq, unsigned& before, unsigned& all) {
+  unsigned b = 0, n = 0;
+  for (int s = threadIdx.x & 31; s < p.c.n_seqs; s += 32) {
+    const unsigned c = step_plan::chunks(p, p.lengths[s]);
+    n += c;
+    b += s < seq ? c : 0;
+  }
+  all = __reduce_add_sync(0xffffffffu, n);
+  before = __reduce_add_sync(0xffffffffu, b);
+}
 
 __device__ __forceinline__ float ex2(float y) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
   return r;
 }
-// code - 7.5 for the nibbles i of both 16-bit halves of a word, i = 0 .. 3: bits 4 .. 7 of a half with exponent 6 are sixteenths of 64 + code
-__device__ __forceinline__ void centred(uint32_t w, uint32_t (&h)[4]) {
-  constexpr uint32_t MASK = 0x00f000f0u, BASE = 0x54005400u;
-  const __half2 mid = __halves2half2(__ushort_as_half(0x5478), __ushort_as_half(0x5478));  // 71.5
-  const uint32_t b[4] = {((w << 4) & MASK) | BASE, (w & MASK) | BASE, ((w >> 4) & MASK) | BASE, ((w >> 8) & MASK) | BASE};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&b[i]), mid);
-    h[i] = *reinterpret_cast<const uint32_t*>(&v);
-  }
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t as_word(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// (w & mask) | bits as one instruction (left to itself the compiler makes two, and moves, of many: 114 for 64 of a tile)
+__device__ __forceinline__ uint32_t masked_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
 }
-__device__ __forceinline__ uint32_t scaled(uint32_t h, __half2 s) {
-  const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&h), s);
-  return *reinterpret_cast<const uint32_t*>(&v);
+// (code - 7.5) * s for the nibbles i of both 16-bit halves of a word, i = 0 .. 3; c = -7.5 s
+__device__ __forceinline__ void scaled_values(uint32_t w, __half2 s, __half2 c, uint32_t (&h)[4]) {
+  const __half2 low = as_half2(0xe400e400u), high = as_half2(0xd400d400u);  // -1024, -64
+  const uint32_t v = w >> 8;
+  h[0] = as_word(__hfma2(__hadd2(as_half2(masked_or(w, 0x000f000fu, 0x64006400u)), low), s, c));
+  h[1] = as_word(__hfma2(__hadd2(as_half2(masked_or(w, 0x00f000f0u, 0x54005400u)), high), s, c));
+  h[2] = as_word(__hfma2(__hadd2(as_half2(masked_or(v, 0x000f000fu, 0x64006400u)), low), s, c));
+  h[3] = as_word(__hfma2(__hadd2(as_half2(masked_or(v, 0x00f000f0u, 0x54005400u)), high), s, c));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {  // an 8 x 8 tile of halves, two neighbours of a row per lane
   uint32_t r;
@@ -55,84 +100,132 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {  // an 8 x 8 tile o
 }
 __device__ __forceinline__ __half half_of(uint32_t v, int hi) { return __ushort_as_half((unsigned short)(hi ? v >> 16 : v & 0xffff)); }
 
-// what a lane holds of a tile: octet t of every 32 dimensions of two keys; VW words of four values' rows; their scales
-template <int HD, int NB>
-struct tile_words {
-  static constexpr int G = HD / 32, VW = HD / 64;
-  uint32_t k[2][G], v[4][VW], ks[2][NB == 4 ? 2 : 1], vs[4];
-};
-
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&r)[N], const uint8_t* p) {
-  if constexpr (N == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
-  } else if constexpr (N == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    r[0] = v.x; r[1] = v.y;
-  } else {
-    r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
+__device__ __forceinline__ void mma_16816_onto(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
+template <int N>
+__device__ __forceinline__ void shared_words(uint32_t (&r)[N], uint32_t at) {
+  if constexpr (N == 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+  else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at));
+  else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[0]) : "r"(at));
+}
+template <int BYTES>
+__device__ __forceinline__ void cp_async_part(uint32_t dst, const void* src, int there) {  // (the rest is zeros)
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there) : "memory");
+}
+__device__ __forceinline__ uint32_t shared_half(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+  return v;
+}
+// keys' codes, values' codes and both kinds of scales of a chunk (scales with 16 bytes to spare: see send)
+template <int HD, int NB>
+struct step_ring {
+  static constexpr uint32_t ROW = HD / 2, PLANE = ST_CHUNK * ROW, SCALES = ST_CHUNK * 2 * NB + 16, STAGE = 2 * PLANE + 2 * SCALES;
+};
 
 template <typename T, int HD, int NB, int NT, bool WEIGHTS>
 __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_kernel(const step_args a) {
-  using words = tile_words<HD, NB>;
-  constexpr int G = words::G, VW = words::VW, BG = G / NB;  // BG groups of 32 dimensions per block
+  constexpr int G = HD / 32, VW = HD / 64, BG = G / NB;  // groups of 32 dimensions, of a block; words of a value's row in a lane
   constexpr bool TWO = HD == 128 && NB == 4;                // a lane's two value words lie in two blocks
-  constexpr int COLS = 8 * NT;
-  extern __shared__ float s_o[];                            // [ST_WARPS][COLS][HD]; then the CTA's sums in the first [COLS][HD]
-  __shared__ float2 s_ml[ST_WARPS][COLS], s_cta[COLS], s_fin[COLS];
+  constexpr int COLS = 8 * NT, ROW = HD / 2, CPR = ROW / 16;
+  using ring_t = step_ring<HD, NB>;
+  constexpr uint32_t PLANE = ring_t::PLANE, SCALES = ring_t::SCALES, STAGE = ring_t::STAGE;
+  extern __shared__ __align__(128) uint8_t s_raw[];         // rings of the warps; then sums [ST_WARPS][COLS][HD]
+  float* s_o = reinterpret_cast<float*>(s_raw);
+  __shared__ float2 s_ml[ST_WARPS][COLS];
   __shared__ int s_bad[4];
   const cache4_attention_params& p = a.p;
-  const int rank = (int)cluster_ctarank(), cs = (int)cluster_nctarank();
-  const int unit = blockIdx.x / cs, seq = unit / p.c.n_kv, kvh = unit - seq * p.c.n_kv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int group = p.n_heads / p.c.n_kv, n_cols = p.m * group, held = p.lengths[seq];
+  const int group = p.n_heads / p.c.n_kv, n_cols = p.m * group, per_seq = p.c.n_kv * a.col_blocks;
+  pdl_launch_dependents();
   const int bound = min(p.c.ctx, p.max_len);
-  auto limit_of = [&](int c) { return c < n_cols ? (int)min((long long)held + c / group + 1, (long long)bound) : 0; };
-  auto row_of = [&](int c) { return (size_t)seq * p.m + c / group; };
-  auto head_of = [&](int c) { return kvh * group + c % group; };
-  if (held < 0) {  // (the whole cluster)
-    for (int e = rank * ST_THREADS + tid; e < n_cols * HD / 2; e += cs * ST_THREADS)
-      reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + row_of(e / (HD / 2)) * p.ld_out + head_of(e / (HD / 2)) * HD)[e % (HD / 2)] = 0u;
-    return;
-  }
-  const int T_all = limit_of(n_cols - 1), T_first = limit_of(0);
-  const int tiles = (T_all + ST_TILE - 1) / ST_TILE;
-  const int tile_lo = (int)((long long)tiles * rank / cs), tile_hi = (int)((long long)tiles * (rank + 1) / cs);
-  const size_t unit_rows = (size_t)unit * p.c.ctx;
-  const uint8_t* k_codes = p.c.k_codes + unit_rows * (HD / 2) + t * (4 * G);
-  const uint8_t* v_codes = p.c.v_codes + unit_rows * (HD / 2) + g * (4 * VW);
-  const uint8_t* k_scales = reinterpret_cast<const uint8_t*>(p.c.k_scales + unit_rows * NB);
-  const int v_block = (g * VW % G) / BG;  // the (first) block of this lane's values
-  const uint8_t* v_scales = reinterpret_cast<const uint8_t*>(p.c.v_scales + unit_rows * NB + v_block);
+  unsigned before, sum_chunks;
+  count_chunks(p, 0, before, sum_chunks);
+  const step_plan plan(sum_chunks * per_seq, a.ctas);
+  if (blockIdx.x >= plan.ctas) return;
+  unsigned at = plan.first_of(blockIdx.x);
+  const unsigned end = plan.first_of(blockIdx.x + 1);
   // tile row r stands for key perm(r): rows 2t, 2t+1, 2t+8, 2t+9, whose probabilities a lane multiplies with values, are keys 4t .. 4t+3
   const int key_a = 4 * (g >> 1) + (g & 1);  // rows g and g + 8: keys key_a and key_a + 2
-  auto fetch = [&](words& w, int tile) {
-    const int j0 = tile * ST_TILE, last = T_all - 1;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const size_t j = min(j0 + key_a + 2 * r, last);
-      load_words<G>(w.k[r], k_codes + j * (HD / 2));
-      if constexpr (NB == 4) load_words<2>(w.ks[r], k_scales + j * 8);
-      else if constexpr (NB == 2) load_words<1>(w.ks[r], k_scales + j * 4);
-      else w.ks[r][0] = __ldg(reinterpret_cast<const unsigned short*>(k_scales + j * 2));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const size_t j = min(j0 + 4 * t + i, last);
-      load_words<VW>(w.v[i], v_codes + j * (HD / 2));
-      if constexpr (TWO) w.vs[i] = __ldg(reinterpret_cast<const uint32_t*>(v_scales + j * (2 * NB)));
-      else w.vs[i] = __ldg(reinterpret_cast<const unsigned short*>(v_scales + j * (2 * NB)));
-    }
-  };
+  const uint32_t ring = smem_u32(s_raw) + warp * (ST_STAGES * STAGE);
+  const int v_block = (g * VW % G) / BG;     // the (first) block of this lane's values
+  // places in the ring: of this lane's pieces of a chunk's values (exchanged within 128 bytes, so that the lanes of one load, in rows four
+  // apart, meet different banks), of its words
+  const uint32_t to_v0 = (uint32_t)(lane ^ (((lane / (4 * CPR)) & 3) << 1)) * 16, to_v1 = (uint32_t)(lane ^ (((32 / (4 * CPR) + lane / (4 * CPR)) & 3) << 1)) * 16;
+  auto word_at = [&](int i) { return (uint32_t)((((4 * t + i) * CPR + g * (4 * VW) / 16) ^ (t << 1)) * 16 + g * (4 * VW) % 16); };
+  const uint32_t from_v0 = word_at(0), from_v1 = word_at(1), from_v2 = word_at(2), from_v3 = word_at(3);
+  const uint32_t from_k = (uint32_t)(key_a * ROW + t * (4 * G));
+  int seq = 0;
+  unsigned seq_at = 0;                       // the sequence's first chunk
 
-  for (int c0 = 0; c0 < n_cols; c0 += COLS) {  // (once, unless there are more than 16 columns)
-    // ---- queries as the narrow operand: column g of each n-tile, octet t of every 32 dimensions, in the codes' order of pairs
+  while (at < end) {
+    // ---- the unit that chunk `at` belongs to
+    int held = p.lengths[seq], chunks = step_plan::chunks(p, held);
+    while (at >= seq_at + chunks * per_seq) {
+      seq_at += chunks * per_seq;
+      held = p.lengths[++seq];
+      chunks = step_plan::chunks(p, held);
+    }
+    const int unit_in_seq = (int)((at - seq_at) / (unsigned)chunks);
+    const int kvh = (unsigned)unit_in_seq / (unsigned)a.col_blocks, c0 = (unit_in_seq - kvh * a.col_blocks) * COLS;
+    const unsigned unit_at = seq_at + (unsigned)(unit_in_seq * chunks);
+    const int lo = (int)(at - unit_at), hi = min(chunks, (int)(end - unit_at));
+    auto limit_of = [&](int c) { return c < n_cols ? (held >= bound ? bound : min(held + c / group + 1, bound)) : 0; };
+    auto row_of = [&](int c) { return (size_t)seq * p.m + c / group; };
+    auto head_of = [&](int c) { return kvh * group + c % group; };
+    const int T_all = limit_of(n_cols - 1), T_first = limit_of(0);
+    const size_t head_rows = ((size_t)seq * p.c.n_kv + kvh) * p.c.ctx;
+    const uint8_t* k_codes = p.c.k_codes + head_rows * ROW;
+    const uint8_t* v_codes = p.c.v_codes + head_rows * ROW;
+    const uint8_t* k_scales = reinterpret_cast<const uint8_t*>(p.c.k_scales + head_rows * NB);
+    const uint8_t* v_scales = reinterpret_cast<const uint8_t*>(p.c.v_scales + head_rows * NB);
+    // (with one block a head's scales may start between two words: they are copied from the word they start in)
+    const uint32_t skew = NB == 1 ? (uint32_t)(head_rows & 1) * 2 : 0u;
+    const long long s_left = (long long)((size_t)p.c.n_seqs * p.c.n_kv * p.c.ctx - head_rows) * 2;  // (one block) bytes to the planes' end
+
+    // a chunk's codes and scales to the ring; rows behind the last one are the last one again
+    auto send = [&](int chunk, uint32_t to) {
+      const size_t first = (size_t)(chunk * ST_CHUNK) * ROW + lane * 16;
+      const uint8_t *k_at = k_codes + first, *v_at = v_codes + first;
+      if (chunk * ST_CHUNK + ST_CHUNK <= T_all) {
+#pragma unroll
+        for (int i = 0; i < CPR; ++i) {
+          cp_async16(to + lane * 16 + i * 512, k_at + i * 512);
+          cp_async16(to + PLANE + (i & 1 ? to_v1 : to_v0) + i * 512, v_at + i * 512);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < CPR; ++i) {
+          const int back = max(0, chunk * ST_CHUNK + (i * 32 + lane) / CPR - (T_all - 1)) * ROW;
+          cp_async16(to + lane * 16 + i * 512, k_at + i * 512 - back);
+          cp_async16(to + PLANE + (i & 1 ? to_v1 : to_v0) + i * 512, v_at + i * 512 - back);
+        }
+      }
+      // scales in words: a row's, or (one block) those that hold a row that is seen; none is read past the end of its plane
+      constexpr int UNIT = NB == 4 ? 8 : 4, UNITS = ST_CHUNK * 2 * NB / UNIT + (NB == 1);
+      const int byte = chunk * (ST_CHUNK * 2 * NB) + lane * UNIT - (int)skew;
+      if (lane < UNITS && byte < T_all * (2 * NB)) {
+        const int there = NB == 1 ? (int)min((long long)UNIT, s_left - byte) : UNIT;
+        cp_async_part<UNIT>(to + 2 * PLANE + lane * UNIT, k_scales + byte, there);
+        cp_async_part<UNIT>(to + 2 * PLANE + SCALES + lane * UNIT, v_scales + byte, there);
+      }
+      cp_async_commit();
+    };
+    int chunk = lo + warp;
+    uint32_t stage = ring;
+    if (chunk < hi) {
+      send(chunk, stage);
+      if (chunk + ST_WARPS < hi) send(chunk + ST_WARPS, stage + STAGE);
+      else cp_async_commit();
+    }
+
+  // ---- queries as the narrow operand: column g of each n-tile, octet t of every 32 dimensions, in the codes' order of pairs
     uint32_t qf[NT][G][4];
-    float f[NT][2];
-    int lim[NT][2];
+    float f[NT][2], start[NT][NB][2];
+    float* at_score[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int c = c0 + n * 8 + g;
@@ -145,29 +238,51 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
 #pragma unroll
         for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[gd][e]));
       }
-      // bfloat16 queries: a power of two takes the column's largest magnitude into [1, 2); halves are exact from 2^-14 of it on
+      // a power of two takes the column's largest magnitude into [2^14, 2^15): halves, and their sixteenths, are exact from 2^-24 of it on
       float up = 1.f, down = 1.f;
-      if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const uint32_t ex = __float_as_uint(most) >> 23;
-        if (ex >= 1 && ex <= 253) {
-          up = __uint_as_float((254u - ex) << 23);
-          down = __uint_as_float(ex << 23);
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int ex = (int)(__float_as_uint(most) >> 23);
+      if (ex >= 20 && ex <= 250) {  // (what is smaller than 2^-107 gives scores of nothing as it is)
+        up = __uint_as_float((uint32_t)(127 + 14 + 127 - ex) << 23);
+        down = __uint_as_float((uint32_t)(ex - 14) << 23);
+      }
+      float corr[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) corr[b] = 0.f;
+#pragma unroll
+      for (int gd = 0; gd < G; ++gd) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) corr[gd / BG] += x[gd][e] * up;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float m = i & 1 ? up * 0.0625f : up;
+          qf[n][gd][i] = pack2<__half>(x[gd][i] * m, x[gd][i + 4] * m);
         }
       }
-#pragma unroll
-      for (int gd = 0; gd < G; ++gd)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qf[n][gd][i] = pack2<__half>(x[gd][i] * up, x[gd][i + 4] * up);
-      const float factor = down * (1.4426950408889634f * rsqrtf((float)HD));
+      const float factor = down * (16777216.f * 1.4426950408889634f * rsqrtf((float)HD));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         f[n][e] = __shfl_sync(0xffffffffu, factor, (2 * t + e) * 4);
-        lim[n][e] = limit_of(c0 + n * 8 + 2 * t + e);
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        corr[b] += __shfl_xor_sync(0xffffffffu, corr[b], 1);
+        corr[b] += __shfl_xor_sync(0xffffffffu, corr[b], 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) start[n][b][e] = __shfl_sync(0xffffffffu, corr[b], (2 * t + e) * 4) * (-7.5f / 16777216.f);
+      }
+      if constexpr (WEIGHTS) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int cc = min(c0 + n * 8 + 2 * t + e, n_cols - 1);
+          at_score[n][e] = a.scores + (row_of(cc) * p.n_heads + head_of(cc)) * p.max_len;
+        }
       }
     }
-    float o[NT][VW * 4][4], mx[NT][2], sum[NT][2];
+
+    // less: minus the maximum (0 while there is none); high: 8 above it, as the products give scores (minus infinity while there is none)
+    float o[NT][VW * 4][4], less[NT][2], high[NT][2], sum[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -176,149 +291,179 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
         for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        mx[n][e] = -INFINITY;
+        less[n][e] = 0.f;
+        high[n][e] = -INFINITY;
         sum[n][e] = 0.f;
       }
     }
     int bad0 = 0x7fffffff, bad1 = 0x7fffffff;
     if (tid < 4) s_bad[tid] = 0x7fffffff;
 
-    words w;
-    int tile = tile_lo + warp;
-    if (tile < tile_hi) fetch(w, tile);
-    for (; tile < tile_hi; tile += ST_WARPS) {
-      const words now = w;
-      if (tile + ST_WARPS < tile_hi) fetch(w, tile + ST_WARPS);
-      const int j0 = tile * ST_TILE;
-      // ---- scores
-      float s[NT][4];
+    for (; chunk < hi; chunk += ST_WARPS) {
+      if (chunk + 2 * ST_WARPS < hi) send(chunk + 2 * ST_WARPS, stage == ring ? ring + 2 * STAGE : stage - STAGE);  // (its readers have passed the __syncwarp below)
+      else cp_async_commit();
+      cp_async_wait<2>();
+      __syncwarp();
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        float acc[NT][4];
+      for (int u = 0; u < 2; ++u) {
+        const int j0 = chunk * ST_CHUNK + u * ST_TILE;
+        uint32_t ks[2][NB == 4 ? 2 : 1], vs[4];
+        uint32_t k0[G], k1[G], vw0[VW], vw1[VW], vw2[VW], vw3[VW];
+        {
+          const uint32_t tile_at = stage + u * ST_TILE * ROW;
+          shared_words<G>(k0, tile_at + from_k);
+          shared_words<G>(k1, tile_at + from_k + 2 * ROW);
+          shared_words<VW>(vw0, tile_at + PLANE + from_v0);
+          shared_words<VW>(vw1, tile_at + PLANE + from_v1);
+          shared_words<VW>(vw2, tile_at + PLANE + from_v2);
+          shared_words<VW>(vw3, tile_at + PLANE + from_v3);
+          const uint32_t ks_at = stage + 2 * PLANE + (u * ST_TILE + key_a) * (2 * NB) + skew;
+          const uint32_t vs_at = stage + 2 * PLANE + SCALES + (u * ST_TILE + 4 * t) * (2 * NB) + v_block * 2 + skew;
 #pragma unroll
-        for (int gb = 0; gb < BG; ++gb) {
-          const int gd = b * BG + gb;
-          uint32_t ka[4], kb[4];
-          centred(now.k[0][gd], ka);
-          centred(now.k[1][gd], kb);
+          for (int r = 0; r < 2; ++r) {
+            if constexpr (NB == 1) ks[r][0] = shared_half(ks_at + 2 * r * (2 * NB));
+            else shared_words<NB / 2>(ks[r], ks_at + 2 * r * (2 * NB));
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (TWO) {
+              uint32_t w[1];
+              shared_words<1>(w, vs_at + i * (2 * NB));
+              vs[i] = w[0];
+            } else {
+              vs[i] = shared_half(vs_at + i * (2 * NB));
+            }
+          }
+        }
+        // ---- scores
+        float s[NT][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          float acc[NT][4];
+#pragma unroll
+          for (int gb = 0; gb < BG; ++gb) {
+            const int gd = b * BG + gb;
+            const uint32_t ka = k0[gd], kb = k1[gd], ka8 = ka >> 8, kb8 = kb >> 8;
+            constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              if (gb == 0) mma_16816_onto(acc[n], ka & LOW, kb & LOW, ka & HIGH, kb & HIGH, qf[n][gd][0], qf[n][gd][1], start[n][b][0], start[n][b][1]);
+              else mma_16816(acc[n], ka & LOW, kb & LOW, ka & HIGH, kb & HIGH, qf[n][gd][0], qf[n][gd][1]);
+              mma_16816(acc[n], ka8 & LOW, kb8 & LOW, ka8 & HIGH, kb8 & HIGH, qf[n][gd][2], qf[n][gd][3]);
+            }
+          }
+          const float sa = __half2float(half_of(ks[0][b >> 1], b & 1)), sb = __half2float(half_of(ks[1][b >> 1], b & 1));
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            if (gb == 0) mma_16816_from(acc[n], ka[0], kb[0], ka[1], kb[1], qf[n][gd][0], qf[n][gd][1], 0.f);
-            else mma_16816(acc[n], ka[0], kb[0], ka[1], kb[1], qf[n][gd][0], qf[n][gd][1]);
-            mma_16816(acc[n], ka[2], kb[2], ka[3], kb[3], qf[n][gd][2], qf[n][gd][3]);
+            s[n][0] = b ? fmaf(sa, acc[n][0], s[n][0]) : sa * acc[n][0];
+            s[n][1] = b ? fmaf(sa, acc[n][1], s[n][1]) : sa * acc[n][1];
+            s[n][2] = b ? fmaf(sb, acc[n][2], s[n][2]) : sb * acc[n][2];
+            s[n][3] = b ? fmaf(sb, acc[n][3], s[n][3]) : sb * acc[n][3];
           }
         }
-        const float sa = __half2float(half_of(now.ks[0][b >> 1], b & 1)), sb = __half2float(half_of(now.ks[1][b >> 1], b & 1));
+        bool raise = false;
+        const bool ragged = j0 + ST_TILE > T_first;  // of the last rows some columns see fewer, and the tile may hang over the end
+        if (ragged) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          s[n][0] = b ? fmaf(sa, acc[n][0], s[n][0]) : sa * acc[n][0];
-          s[n][1] = b ? fmaf(sa, acc[n][1], s[n][1]) : sa * acc[n][1];
-          s[n][2] = b ? fmaf(sb, acc[n][2], s[n][2]) : sb * acc[n][2];
-          s[n][3] = b ? fmaf(sb, acc[n][3], s[n][3]) : sb * acc[n][3];
-        }
-      }
-      const bool ragged = j0 + ST_TILE > T_first;  // (of the last rows some columns see fewer, and the tile may hang over the end)
-      bool raise = false;
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] *= f[n][e & 1];
-          if (ragged && j0 + key_a + (e & 2) >= lim[n][e & 1]) s[n][e] = -INFINITY;
-        }
-        if constexpr (WEIGHTS) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = c0 + n * 8 + 2 * t + (e & 1), j = j0 + key_a + (e & 2);
-            if (c < n_cols && j < T_all) a.scores[(row_of(c) * p.n_heads + head_of(c)) * p.max_len + j] = s[n][e];
-          }
-        }
-        raise |= fmaxf(s[n][0], s[n][2]) > mx[n][0] + 8.f || fmaxf(s[n][1], s[n][3]) > mx[n][1] + 8.f;
-      }
-      if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float k[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(s[n][e], s[n][e + 2]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            top = fmaxf(top, mx[n][e]);
-            k[e] = mx[n][e] == -INFINITY ? 0.f : ex2(mx[n][e] - top);
-            mx[n][e] = top;
-            sum[n][e] *= k[e];
-          }
-#pragma unroll
-          for (int i = 0; i < VW * 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][i][e] *= k[e & 1];
-        }
-      }
-      // ---- probabilities, with columns as rows
-      uint32_t pf[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float b0 = mx[n][0] == -INFINITY ? 0.f : mx[n][0], b1 = mx[n][1] == -INFINITY ? 0.f : mx[n][1];
-        const float e0 = ex2(s[n][0] - b0), e1 = ex2(s[n][1] - b1), e2 = ex2(s[n][2] - b0), e3 = ex2(s[n][3] - b1);
-        sum[n][0] += e0 + e2;
-        sum[n][1] += e1 + e3;
-        pf[n][0] = transposed(pack2<__half>(e0, e1));
-        pf[n][1] = transposed(pack2<__half>(e2, e3));
-      }
-      // ---- values
-      uint32_t vs[4] = {now.vs[0], now.vs[1], now.vs[2], now.vs[3]};
-      if (j0 + ST_TILE > T_all) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (j0 + 4 * t + i >= T_all) vs[i] = 0u;
-      }
-      {
-        const __half2 x0 = *reinterpret_cast<const __half2*>(&vs[0]), x1 = *reinterpret_cast<const __half2*>(&vs[1]);
-        const __half2 x2 = *reinterpret_cast<const __half2*>(&vs[2]), x3 = *reinterpret_cast<const __half2*>(&vs[3]);
-        const __half2 z = __hadd2(__hadd2(x0, x1), __hadd2(x2, x3));  // (up to 4 x 8704: finite)
-        const __half zz = __hadd(__low2half(z), __high2half(z));
-        if (__hisnan(zz)) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (__hisnan(half_of(vs[i], 0))) {
-              bad0 = min(bad0, j0 + 4 * t + i);
-              vs[i] &= 0xffff0000u;
+            for (int e = 0; e < 2; ++e) {
+              const int limit = limit_of(c0 + n * 8 + 2 * t + e);
+              if (j0 + key_a >= limit) s[n][e] = -INFINITY;
+              if (j0 + key_a + 2 >= limit) s[n][e + 2] = -INFINITY;
             }
-            if (__hisnan(half_of(vs[i], 1))) {
-              bad1 = min(bad1, j0 + 4 * t + i);
-              vs[i] &= 0x0000ffffu;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (j0 + 4 * t + i >= T_all) vs[i] = 0u;
+        }
+        if constexpr (WEIGHTS) {  // (a column's rows that it does not see: minus infinity, read by nobody)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = j0 + key_a + (e & 2);
+              if (c0 + n * 8 + 2 * t + (e & 1) < n_cols && (!ragged || j < T_all)) at_score[n][e & 1][j] = s[n][e] * f[n][e & 1];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) raise |= fmaxf(s[n][0], s[n][2]) > high[n][0] || fmaxf(s[n][1], s[n][3]) > high[n][1];
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float k[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(s[n][e], s[n][e + 2]) * f[n][e];
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              const bool none = high[n][e] == -INFINITY;
+              if (!none) top = fmaxf(top, -less[n][e]);
+              k[e] = none ? 0.f : ex2(-less[n][e] - top);
+              less[n][e] = top == -INFINITY ? 0.f : -top;
+              high[n][e] = (top + 8.f) / f[n][e];
+              sum[n][e] *= k[e];
+            }
+#pragma unroll
+            for (int i = 0; i < VW * 4; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[n][i][e] *= k[e & 1];
+          }
+        }
+        // ---- probabilities, with columns as rows
+        uint32_t pf[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float e0 = ex2(fmaf(s[n][0], f[n][0], less[n][0])), e1 = ex2(fmaf(s[n][1], f[n][1], less[n][1]));
+          const float e2 = ex2(fmaf(s[n][2], f[n][0], less[n][0])), e3 = ex2(fmaf(s[n][3], f[n][1], less[n][1]));
+          sum[n][0] += e0 + e2;
+          sum[n][1] += e1 + e3;
+          pf[n][0] = transposed(pack2<__half>(e0, e1));
+          pf[n][1] = transposed(pack2<__half>(e2, e3));
+        }
+        // ---- values
+        {
+          const __half2 z = __hadd2(__hadd2(as_half2(vs[0]), as_half2(vs[1])), __hadd2(as_half2(vs[2]), as_half2(vs[3])));  // (up to 4 x 8704: finite)
+          if (__hisnan(__hadd(__low2half(z), __high2half(z)))) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (__hisnan(half_of(vs[i], 0))) {
+                bad0 = min(bad0, j0 + 4 * t + i);
+                vs[i] &= 0xffff0000u;
+              }
+              if (__hisnan(half_of(vs[i], 1))) {
+                bad1 = min(bad1, j0 + 4 * t + i);
+                vs[i] &= 0x0000ffffu;
+              }
             }
           }
         }
-      }
 #pragma unroll
-      for (int vw = 0; vw < VW; ++vw) {
-        const uint32_t pick = TWO && vw ? 0x7632u : 0x5410u;
-        const uint32_t s01w = __byte_perm(vs[0], vs[1], pick), s23w = __byte_perm(vs[2], vs[3], pick);
-        const __half2 s01 = *reinterpret_cast<const __half2*>(&s01w), s23 = *reinterpret_cast<const __half2*>(&s23w);
+        for (int vw = 0; vw < VW; ++vw) {
+          const uint32_t pick = TWO && vw ? 0x7632u : 0x5410u;
+          const __half2 s01 = as_half2(__byte_perm(vs[0], vs[1], pick)), s23 = as_half2(__byte_perm(vs[2], vs[3], pick));
+          const __half2 minus = as_half2(0xc780c780u);  // -7.5
+          const __half2 c01 = __hmul2(s01, minus), c23 = __hmul2(s23, minus);
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          uint32_t h01[4], h23[4];
-          centred(__byte_perm(now.v[0][vw], now.v[1][vw], hh ? 0x7632 : 0x5410), h01);
-          centred(__byte_perm(now.v[2][vw], now.v[3][vw], hh ? 0x7632 : 0x5410), h23);
+          for (int hh = 0; hh < 2; ++hh) {
+            uint32_t h01[4], h23[4];
+            scaled_values(__byte_perm(vw0[vw], vw1[vw], hh ? 0x7632 : 0x5410), s01, c01, h01);
+            scaled_values(__byte_perm(vw2[vw], vw3[vw], hh ? 0x7632 : 0x5410), s23, c23, h23);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            h01[i] = scaled(h01[i], s01);
-            h23[i] = scaled(h23[i], s23);
+            for (int mm = 0; mm < 2; ++mm)
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                mma_16816(o[n][vw * 4 + hh * 2 + mm], h01[2 * mm], h01[2 * mm + 1], h23[2 * mm], h23[2 * mm + 1], pf[n][0], pf[n][1]);
           }
-#pragma unroll
-          for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              mma_16816(o[n][vw * 4 + hh * 2 + mm], h01[2 * mm], h01[2 * mm + 1], h23[2 * mm], h23[2 * mm + 1], pf[n][0], pf[n][1]);
         }
       }
+      __syncwarp();
+      stage = stage == ring + 2 * STAGE ? ring : stage + STAGE;
     }
 
     // ---- the warps meet
     const int here = min(COLS, n_cols - c0);
+    __syncthreads();  // (the rings are read; s_bad is set)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -328,7 +473,7 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int c = n * 8 + 2 * t + e;
-        if (g == 0) s_ml[warp][c] = make_float2(mx[n][e], l);
+        if (g == 0) s_ml[warp][c] = make_float2(high[n][e] == -INFINITY ? -INFINITY : -less[n][e], l);
         if (c < here) {
 #pragma unroll
           for (int i = 0; i < VW * 4; ++i) {
@@ -338,97 +483,157 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
         }
       }
     }
-    __syncthreads();  // (s_bad is set)
-    bad0 = min(bad0, __shfl_xor_sync(0xffffffffu, bad0, 1));
-    bad0 = min(bad0, __shfl_xor_sync(0xffffffffu, bad0, 2));
-    if (t == 0 && bad0 != 0x7fffffff) atomicMin(&s_bad[v_block], bad0);
-    if constexpr (TWO) {
-      bad1 = min(bad1, __shfl_xor_sync(0xffffffffu, bad1, 1));
-      bad1 = min(bad1, __shfl_xor_sync(0xffffffffu, bad1, 2));
-      if (t == 0 && bad1 != 0x7fffffff) atomicMin(&s_bad[v_block + 1], bad1);
-    }
-    if (tid < here) {
-      float top = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int w8 = 0; w8 < ST_WARPS; ++w8) top = fmaxf(top, s_ml[w8][tid].x);
-#pragma unroll
-      for (int w8 = 0; w8 < ST_WARPS; ++w8) {
-        const float k = top == -INFINITY || s_ml[w8][tid].x == -INFINITY ? 1.f : ex2(s_ml[w8][tid].x - top);  // (a maximum of nothing: a sum of 0, or of NaN)
-        l += s_ml[w8][tid].y * k;
-      }
-      s_cta[tid] = make_float2(top, l);
-    }
+    if (bad0 != 0x7fffffff) atomicMin(&s_bad[v_block], bad0);
+    if (bad1 != 0x7fffffff) atomicMin(&s_bad[v_block + 1], bad1);
     __syncthreads();
-    for (int e = tid; e < here * HD; e += ST_THREADS) {
-      const int c = e / HD;
-      const float top = s_cta[c].x;
-      float v = 0.f;
-#pragma unroll
-      for (int w8 = 0; w8 < ST_WARPS; ++w8) {
-        const float k = top == -INFINITY || s_ml[w8][c].x == -INFINITY ? 1.f : ex2(s_ml[w8][c].x - top);
-        v += s_o[w8 * COLS * HD + e] * k;
-      }
-      s_o[e] = v;  // (this thread alone reads and writes place e of the first warp's part)
-    }
-    // ---- the CTAs meet
-    cluster_sync();
-    if (tid < here) {
-      float top = -INFINITY, l = 0.f;
-      const uint32_t mine = smem_u32(&s_cta[tid]);
-      for (int r = 0; r < cs; ++r) top = fmaxf(top, ld_dsmem_f32(mapa(mine, r)));
-      for (int r = 0; r < cs; ++r) {
-        const float m1 = ld_dsmem_f32(mapa(mine, r)), l1 = ld_dsmem_f32(mapa(mine + 4, r));
-        l += l1 * (top == -INFINITY || m1 == -INFINITY ? 1.f : ex2(m1 - top));
-      }
-      s_fin[tid] = make_float2(top, 1.f / l);
-    }
-    __syncthreads();
-    for (int e = rank * ST_THREADS + tid; e < here * HD / 2; e += cs * ST_THREADS) {
+    const bool whole = lo == 0 && hi == chunks;
+    const size_t slot = (size_t)blockIdx.x * 2 + (lo == 0);
+    for (int e = tid; e < here * (HD / 2); e += ST_THREADS) {
       const int c = e / (HD / 2), d = 2 * (e % (HD / 2));
-      const float top = s_fin[c].x;
-      float x = 0.f, y = 0.f;
-      int bad = 0x7fffffff;
-      for (int r = 0; r < cs; ++r) {
-        const float m1 = ld_dsmem_f32(mapa(smem_u32(&s_cta[c]), r));
-        const float k = top == -INFINITY || m1 == -INFINITY ? 1.f : ex2(m1 - top);
-        x += ld_dsmem_f32(mapa(smem_u32(&s_o[c * HD + d]), r)) * k;
-        y += ld_dsmem_f32(mapa(smem_u32(&s_o[c * HD + d + 1]), r)) * k;
-        bad = min(bad, __float_as_int(ld_dsmem_f32(mapa(smem_u32(&s_bad[d * NB / HD]), r))));
+      float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < ST_WARPS; ++w) top = fmaxf(top, s_ml[w][c].x);
+#pragma unroll
+      for (int w = 0; w < ST_WARPS; ++w) {
+        const float2 ml = s_ml[w][c];
+        const float k = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // (a maximum of nothing: sums of 0, or of NaN)
+        const float2 v = *reinterpret_cast<const float2*>(&s_o[(w * COLS + c) * HD + d]);
+        l += ml.y * k;
+        x += v.x * k;
+        y += v.y * k;
       }
-      const float rl = bad < limit_of(c0 + c) ? __int_as_float(0x7fffffff) : s_fin[c].y;
-      reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + row_of(c0 + c) * p.ld_out + head_of(c0 + c) * HD)[d / 2] = pack2<T>(x * rl, y * rl);
-    }
-    // ---- weights of this CTA's rows: every lane reads the scores that it wrote
-    if constexpr (WEIGHTS) {
-      for (int u = tile_lo + warp; u < tile_hi; u += ST_WARPS) {
-        float add[2] = {0.f, 0.f};
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int lc = n * 8 + 2 * t + (e & 1), c = c0 + lc, j = u * ST_TILE + key_a + (e & 2);
-            if (c < n_cols && j < lim[n][e & 1]) add[e >> 1] += ex2(a.scores[(row_of(c) * p.n_heads + head_of(c)) * p.max_len + j] - s_fin[lc].x) * s_fin[lc].y;
-          }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          add[r] += __shfl_xor_sync(0xffffffffu, add[r], 1);
-          add[r] += __shfl_xor_sync(0xffffffffu, add[r], 2);
-          const int j = u * ST_TILE + key_a + 2 * r;
-          if (t == 0 && j < T_all) {
-            float* at = p.weights + unit_rows + j;
-            if (c0) *at += add[r];
-            else *at = p.beta == 0.f || j >= held ? add[r] : fmaf(p.beta, *at, add[r]);
-          }
-        }
+      if (whole) {
+        const float rl = s_bad[d * NB / HD] < limit_of(c0 + c) ? __int_as_float(0x7fffffff) : 1.f / l;
+        reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + row_of(c0 + c) * p.ld_out + head_of(c0 + c) * HD)[d / 2] = pack2<T>(x * rl, y * rl);
+        if (WEIGHTS && d == 0) a.unit_ml[((size_t)seq * per_seq + unit_in_seq) * COLS + c] = make_float2(top, l);
+      } else {
+        *reinterpret_cast<float2*>(&a.parts[(slot * COLS + c) * HD + d]) = make_float2(x, y);
+        if (d == 0) a.part_ml[slot * COLS + c] = make_float2(top, l);
       }
     }
-    cluster_sync();  // (no CTA leaves, or starts on other columns, while another reads its shared memory)
+    if (!whole && tid < 4) a.part_bad[slot * 4 + tid] = s_bad[tid];
+    __syncthreads();  // (the rings are free)
+    at = unit_at + hi;
   }
 }
 
+// Joins the sums of units that several CTAs did (and gives zeros for sequences not in use): a CTA per unit; and behind those, with weights, a
+// CTA per (sequence, key/value head, 512 rows), which finds maxima and sums of all columns and adds the probabilities in their order.
+constexpr int JOIN_THREADS = 128, JOIN_KEYS = 4 * JOIN_THREADS;
+template <typename T, int HD, int NB, int NT>
+__global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step_args a) {
+  constexpr int COLS = 8 * NT;
+  const cache4_attention_params& p = a.p;
+  const int tid = threadIdx.x, group = p.n_heads / p.c.n_kv, n_cols = p.m * group, per_seq = p.c.n_kv * a.col_blocks;
+  const int units = p.c.n_seqs * per_seq;
+  const int key_blocks = (p.max_len + JOIN_KEYS - 1) / JOIN_KEYS;
+  const bool joins = (int)blockIdx.x < units;
+  const int sh = joins ? 0 : ((int)blockIdx.x - units) / key_blocks;
+  const int seq = joins ? (int)blockIdx.x / per_seq : sh / p.c.n_kv;
+  const int held = p.lengths[seq], chunks = step_plan::chunks(p, held);
+  if (!joins && held < 0) return;
+  unsigned before, sum_chunks;
+  count_chunks(p, seq, before, sum_chunks);
+  const step_plan plan(sum_chunks * per_seq, a.ctas);
+  pdl_wait();
+  auto row_of = [&](int c) { return (size_t)seq * p.m + c / group; };
+  // maximum and sum of column c of a unit, whoever did it
+  auto find = [&](int unit_in_seq, int c, int& first, int& last) {
+    const unsigned unit_at = before * per_seq + (unsigned)(unit_in_seq * chunks);
+    first = (int)plan.cta_of(unit_at);
+    last = (int)plan.cta_of(unit_at + chunks - 1);
+    if (first == last) return a.unit_ml ? a.unit_ml[((size_t)seq * per_seq + unit_in_seq) * COLS + c] : make_float2(0.f, 1.f);
+    float2 all = make_float2(-INFINITY, 0.f);
+    for (int b = first; b <= last; ++b) all.x = fmaxf(all.x, a.part_ml[((size_t)b * 2 + (b == first)) * COLS + c].x);
+    for (int b = first; b <= last; ++b) {
+      const float2 ml = a.part_ml[((size_t)b * 2 + (b == first)) * COLS + c];
+      all.y += ml.y * (ml.x == -INFINITY ? 1.f : ex2(ml.x - all.x));
+    }
+    return all;
+  };
+  if (joins) {
+    const int unit_in_seq = (int)blockIdx.x % per_seq, kvh = unit_in_seq / a.col_blocks, c0 = unit_in_seq % a.col_blocks * COLS, here = min(COLS, n_cols - c0);
+    auto place = [&](int c, int d) {
+      return reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + row_of(c0 + c) * p.ld_out + (kvh * group + (c0 + c) % group) * HD) + d / 2;
+    };
+    if (held < 0) {
+      for (int e = tid; e < here * (HD / 2); e += JOIN_THREADS) *place(e / (HD / 2), 2 * (e % (HD / 2))) = 0u;
+      return;
+    }
+    for (int e = tid; e < here * (HD / 2); e += JOIN_THREADS) {
+      const int c = e / (HD / 2), d = 2 * (e % (HD / 2));
+      int first, last, bad = 0x7fffffff;
+      const float2 ml = find(unit_in_seq, c, first, last);
+      if (first == last) return;
+      float x = 0.f, y = 0.f;
+      for (int b = first; b <= last; ++b) {
+        const size_t slot = (size_t)b * 2 + (b == first);
+        const float m1 = a.part_ml[slot * COLS + c].x, k = m1 == -INFINITY ? 1.f : ex2(m1 - ml.x);
+        const float2 v = *reinterpret_cast<const float2*>(&a.parts[(slot * COLS + c) * HD + d]);
+        x += v.x * k;
+        y += v.y * k;
+        bad = min(bad, a.part_bad[slot * 4 + d * NB / HD]);
+      }
+      const int limit = (int)min((long long)held + (c0 + c) / group + 1, (long long)min(p.c.ctx, p.max_len));
+      const float rl = bad < limit ? __int_as_float(0x7fffffff) : 1.f / ml.y;
+      *place(c, d) = pack2<T>(x * rl, y * rl);
+    }
+    return;
+  }
+  // ---- weights
+  __shared__ float2 s_fin[64];
+  const int kvh = sh % p.c.n_kv, j0 = (((int)blockIdx.x - units) % key_blocks) * JOIN_KEYS, bound = min(p.c.ctx, p.max_len);
+  const int T_all = (int)min((long long)held + p.m, (long long)bound);
+  if (j0 >= T_all) return;
+  float w[JOIN_KEYS / JOIN_THREADS] = {};
+  for (int c64 = 0; c64 < n_cols; c64 += 64) {
+    __syncthreads();
+    if (tid < 64 && c64 + tid < n_cols) {
+      const int c = c64 + tid;
+      int first, last;
+      const float2 ml = find(kvh * a.col_blocks + c / COLS, c % COLS, first, last);
+      s_fin[tid] = make_float2(ml.x, 1.f / ml.y);
+    }
+    __syncthreads();
+    for (int c = c64; c < min(n_cols, c64 + 64); ++c) {
+      const float* scores = a.scores + (row_of(c) * p.n_heads + kvh * group + c % group) * p.max_len;
+      const int limit = (int)min((long long)held + c / group + 1, (long long)bound);
+      const float2 fin = s_fin[c - c64];
+#pragma unroll
+      for (int i = 0; i < JOIN_KEYS / JOIN_THREADS; ++i) {
+        const int j = j0 + i * JOIN_THREADS + tid;
+        if (j < limit) w[i] += ex2(scores[j] - fin.x) * fin.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < JOIN_KEYS / JOIN_THREADS; ++i) {
+    const int j = j0 + i * JOIN_THREADS + tid;
+    if (j < T_all) {
+      float* to = p.weights + (size_t)sh * p.c.ctx + j;
+      *to = p.beta == 0.f || j >= held ? w[i] : fmaf(p.beta, *to, w[i]);
+    }
+  }
+}
+
+// the work as the host knows it: units, and CTAs that find a chunk for each of their warps if sequences are as long as they may be
+struct step_shape {
+  int cols, col_blocks, ctas;
+  long long units;
+  step_shape(int n_seqs, int m, int n_heads, int n_kv, int max_len) {
+    const int n_cols = m * (n_heads / n_kv);
+    cols = n_cols <= 8 ? 8 : 16;
+    col_blocks = (n_cols + cols - 1) / cols;
+    units = (long long)n_seqs * n_kv * col_blocks;
+    const long long chunks = units * ((max_len + ST_CHUNK - 1) / ST_CHUNK);
+    ctas = (int)std::max(1ll, std::min((long long)ST_CTAS / (cols / 8), (chunks + ST_WARPS - 1) / ST_WARPS));
+  }
+};
+
 template <typename T, int HD, int NB, int NT, bool WEIGHTS>
-int launch_step(const step_args& a, int cs, cudaStream_t stream) {
-  constexpr size_t SMEM = (size_t)ST_WARPS * 8 * NT * HD * sizeof(float);
+int launch_step(const step_args& a, cudaStream_t stream) {
+  constexpr size_t RING = (size_t)ST_WARPS * ST_STAGES * step_ring<HD, NB>::STAGE, SUMS = (size_t)ST_WARPS * 8 * NT * HD * sizeof(float);
+  constexpr size_t SMEM = RING > SUMS ? RING : SUMS;
   auto* kernel = attention_step_kernel<T, HD, NB, NT, WEIGHTS>;
   static bool attr_done[16] = {};
   int dev = 0;
@@ -437,59 +642,68 @@ int launch_step(const step_args& a, int cs, cudaStream_t stream) {
     LCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
     if (dev < 16) attr_done[dev] = true;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)cs * a.p.c.n_seqs * a.p.c.n_kv);
-  cfg.blockDim = dim3(ST_THREADS);
-  cfg.dynamicSmemBytes = SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cs;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  LCU_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+  kernel<<<a.ctas, ST_THREADS, SMEM, stream>>>(a);
+  const long long units = (long long)a.p.c.n_seqs * a.p.c.n_kv * a.col_blocks;
+  const long long blocks = units + (WEIGHTS ? (long long)a.p.c.n_seqs * a.p.c.n_kv * ((a.p.max_len + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
+  LCU_CUDA(launch_after(attention_join_kernel<T, HD, NB, NT>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, stream, a));
   return LCU_OK;
 }
 
 template <typename T, int HD, int NB>
-int launch_cols(const step_args& a, int cs, cudaStream_t stream) {
-  const bool one = a.p.m * (a.p.n_heads / a.p.c.n_kv) <= 8;
-  if (a.p.weights) return one ? launch_step<T, HD, NB, 1, true>(a, cs, stream) : launch_step<T, HD, NB, 2, true>(a, cs, stream);
-  return one ? launch_step<T, HD, NB, 1, false>(a, cs, stream) : launch_step<T, HD, NB, 2, false>(a, cs, stream);
+int launch_cols(const step_args& a, int cols, cudaStream_t stream) {
+  if (a.p.weights) return cols == 8 ? launch_step<T, HD, NB, 1, true>(a, stream) : launch_step<T, HD, NB, 2, true>(a, stream);
+  return cols == 8 ? launch_step<T, HD, NB, 1, false>(a, stream) : launch_step<T, HD, NB, 2, false>(a, stream);
 }
 
 template <typename T>
-int launch_shape(const step_args& a, int cs, cudaStream_t stream) {
+int launch_shape(const step_args& a, int cols, cudaStream_t stream) {
   const int nb = a.p.c.hd / a.p.c.bs;
   if (a.p.c.hd == 128) {
-    if (nb == 4) return launch_cols<T, 128, 4>(a, cs, stream);
-    if (nb == 2) return launch_cols<T, 128, 2>(a, cs, stream);
-    return launch_cols<T, 128, 1>(a, cs, stream);
+    if (nb == 4) return launch_cols<T, 128, 4>(a, cols, stream);
+    if (nb == 2) return launch_cols<T, 128, 2>(a, cols, stream);
+    return launch_cols<T, 128, 1>(a, cols, stream);
   }
-  if (nb == 2) return launch_cols<T, 64, 2>(a, cs, stream);
-  return launch_cols<T, 64, 1>(a, cs, stream);
+  if (nb == 2) return launch_cols<T, 64, 2>(a, cols, stream);
+  return launch_cols<T, 64, 1>(a, cols, stream);
+}
+
+// the workspace's parts, each 16-byte aligned
+size_t step_layout(step_args* a, void* workspace, const step_shape& w, int n_seqs, int m, int n_heads, int hd, int max_len, bool weights) {
+  size_t used = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = used;
+    used += round_up(bytes, 16);
+    return (uint8_t*)workspace + at;
+  };
+  const size_t slots = (size_t)w.ctas * 2;
+  uint8_t* parts = take(slots * w.cols * hd * sizeof(float));
+  uint8_t* part_ml = take(slots * w.cols * sizeof(float2));
+  uint8_t* part_bad = take(slots * 4 * sizeof(int));
+  uint8_t* unit_ml = weights ? take((size_t)w.units * w.cols * sizeof(float2)) : nullptr;
+  uint8_t* scores = weights ? take((size_t)n_seqs * m * n_heads * max_len * sizeof(float)) : nullptr;
+  if (a) {
+    a->parts = (float*)parts;
+    a->part_ml = (float2*)part_ml;
+    a->part_bad = (int*)part_bad;
+    a->unit_ml = (float2*)unit_ml;
+    a->scores = (float*)scores;
+  }
+  return used;
 }
 
 }  // namespace
 
-size_t attention_cache4_step_workspace(int n_seqs, int m, int n_heads, int max_len, bool weights) {
-  return weights ? (size_t)n_seqs * m * n_heads * max_len * sizeof(float) : 0;
-}
-
-// CTAs that share a (sequence, key/value head): enough for two per SM over all of them, none with less than a tile for each warp
-static int step_cluster(const cache4_attention_params& p) {
-  const long long units = (long long)p.c.n_seqs * p.c.n_kv, per_warp = (p.max_len + ST_TILE - 1) / ST_TILE / ST_WARPS;
-  int cs = 1;
-  while (cs < 8 && units * cs < 2 * 148 && 2 * cs <= per_warp) cs *= 2;
-  return cs;
+size_t attention_cache4_step_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
+  return step_layout(nullptr, nullptr, step_shape(n_seqs, m, n_heads, n_kv, max_len), n_seqs, m, n_heads, hd, max_len, weights);
 }
 
 int launch_attention_cache4_step(const cache4_attention_params& p, int dtype, void* workspace, cudaStream_t stream) {
-  step_args a{p, (float*)workspace};
-  const int cs = step_cluster(p);
-  return dtype == OP_F16 ? launch_shape<__half>(a, cs, stream) : launch_shape<__nv_bfloat16>(a, cs, stream);
+  const long long chunks = (long long)p.c.n_seqs * p.c.n_kv * ((p.m * (p.n_heads / p.c.n_kv) + 7) / 8) * ((p.max_len + ST_CHUNK - 1) / ST_CHUNK);
+  LCU_REQUIRE(chunks < (1ll << 31), "attention_cache4: %d sequences of %d heads over %d rows are too many", p.c.n_seqs, p.n_heads, p.max_len);
+  const step_shape w(p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.max_len);
+  step_args a{p, w.ctas, w.col_blocks};
+  step_layout(&a, workspace, w, p.c.n_seqs, p.m, p.n_heads, p.c.hd, p.max_len, p.weights != nullptr);
+  return dtype == OP_F16 ? launch_shape<__half>(a, w.cols, stream) : launch_shape<__nv_bfloat16>(a, w.cols, stream);
 }
 
 }  // namespace lcu

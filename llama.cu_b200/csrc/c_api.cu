@@ -386,6 +386,7 @@ int lcu_cache4_read(void* k_out_dev, void* v_out_dev, const void* k_codes_dev, c
                             first_dev, count, dtype, (cudaStream_t)stream);
 }
 uint64_t lcu_attention_cache4_workspace(int n_seqs, int m, int n_heads, int n_kv_heads, int head_dim, int max_len, int weights) {
+  if (n_seqs < 1 || m < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || head_dim < 1 || max_len < 1) return 0;  // (a call of such sizes is refused)
   return cache4_attention_workspace(n_seqs, m, n_heads, n_kv_heads, head_dim, max_len, weights != 0);
 }
 int lcu_attention_cache4(void* out_dev, int ld_out, void* weights_dev, float beta, const void* q_dev, int ld_q, const void* k_codes_dev,
@@ -418,7 +419,10 @@ int lcu_cache_reorder(void* const* dst_planes, const void* const* src_planes, co
   return launch_cache_reorder(reorder_params{dst_planes, src_planes, row_bytes, n_planes, parents_dev, lengths_dev, n_groups, beams, n_kv_heads, ctx_len},
                               (cudaStream_t)stream);
 }
-uint64_t lcu_beam_select_workspace(int n_groups, int beams, int n_vocab, int n_out) { return beam_select_workspace(n_groups, beams, n_vocab, n_out); }
+uint64_t lcu_beam_select_workspace(int n_groups, int beams, int n_vocab, int n_out) {
+  if (n_groups < 1 || beams < 1 || n_vocab < 1 || n_out < 1) return 0;
+  return beam_select_workspace(n_groups, beams, n_vocab, n_out);
+}
 int lcu_beam_select(int32_t* parents_dev, int32_t* tokens_dev, float* scores_out_dev, const void* logits_dev, int ld, int dtype, const float* scores_dev,
                     int n_groups, int beams, int n_vocab, int n_out, void* workspace_dev, uint64_t workspace_bytes, void* stream) {
   return launch_beam_select(beam_params{parents_dev, tokens_dev, scores_out_dev, logits_dev, ld, scores_dev, n_groups, beams, n_vocab, n_out}, dtype, workspace_dev,
