@@ -1,0 +1,638 @@
+// Attention of prompt rows over the 4-bit cache (cache4.cuh) on tcgen05.
+//
+//   s_rj = q_r . k_j / sqrt(head_dim),  o_r = sum_j e^(s_rj - max) v_j / sum_j e^(s_rj - max),   rows r = (row of the call, head of the key/value head)
+// A prompt meets every cached row once per 128 rows, so the codes are expanded to halves once, exactly (7-bit scales), into the workspace
+// of the call - 4 bytes moved per value and product, against codes expanded again for each 128 x 128 tile at a cost close to the tile's own
+// exponentials.  bfloat16 queries become halves too, each row by a power of two, so that both types share everything behind.
+//
+// One CTA per (sequence, key/value head, 128 rows), two CTAs per SM: while one's scores are exponentiated, the other's products run.
+// Scores lie in tensor memory; a thread owns a row, reads 32 keys at a time and keeps the running maximum and the sum; probabilities
+// go back to tensor memory, over the scores, as halves: the A operand of the product with the values, whose accumulator stays in tensor
+// memory.  A maximum is raised only when a score passes it by 8 (powers of two), so that the exponentials of a tile are formed with
+// the old one while its own maximum is looked for; only where a row fails that test is its warp's tile done again and the output rescaled.
+//
+// Weights: once maxima and sums are known, a second kernel forms the scores the other way round - a thread owns a cached row - and adds
+// e^(s - max) / sum over all rows in their order.
+//
+// Values whose scale is no number are expanded to zeros and the first such row of every 128 and block is listed: rows that see it
+// get NaN in that block's dimensions, earlier ones do not.
+#include <algorithm>
+#include <type_traits>
+
+#include "cache4_attention.cuh"
+#include "runtime.cuh"
+#include "tc_common.cuh"
+
+namespace lcu {
+namespace {
+
+constexpr int PR_ROWS = 128, PR_KEYS = 128, PR_SOFT_WARPS = 4, PR_THREADS = 32 * (PR_SOFT_WARPS + 2);
+
+struct prompt_args {
+  cache4_attention_params p;
+  __half* k_half;     // [units][t_pad][hd]
+  __half* v_half;
+  __half* q_half;     // [units][r_pad][hd]
+  float2* row_stats;  // [units][r_pad] factor of a row's scores (powers of two); logarithm of its sum (weights; infinity: no such row)
+  int* bad;           // [units][t_pad / 128][4] first row of each 128 whose values of a block are no numbers
+  int t_pad, r_pad;
+  int* err;
+};
+
+__device__ __forceinline__ int rows_of(const cache4_attention_params& p, int held) {  // cached rows that the last row of the call sees
+  const int room = min(p.c.ctx, p.max_len);
+  return held < 0 ? 0 : held >= room ? room : min(held + p.m, room);
+}
+__device__ __forceinline__ int limit_of(const cache4_attention_params& p, int held, int i) {
+  const int room = min(p.c.ctx, p.max_len);
+  return held < 0 ? 0 : held >= room ? room : min(held + i + 1, room);
+}
+
+// ------------------------------------------------------------------ expansion
+// One CTA per 128 rows of a unit's keys and values, or of its queries.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) prompt_expand_kernel(const prompt_args a, int key_blocks, int row_blocks) {
+  const cache4_attention_params& p = a.p;
+  __shared__ int s_bad[4];
+  constexpr int WORDS = HD / 8, G = HD / 32;
+  const int unit = blockIdx.x / (key_blocks + row_blocks), b = blockIdx.x % (key_blocks + row_blocks), seq = unit / p.c.n_kv, kvh = unit % p.c.n_kv;
+  const int held = p.lengths[seq], seen = rows_of(p, held);
+  pdl_launch_dependents();
+  if (b < key_blocks) {
+    if (b * PR_KEYS >= seen) return;
+    if (threadIdx.x < 4) s_bad[threadIdx.x] = 0x7fffffff;
+    __syncthreads();
+    const int nb = HD / p.c.bs;
+    for (int w = threadIdx.x; w < PR_KEYS * WORDS; w += 256) {
+      const int r = w / WORDS, word = w % WORDS, j = b * PR_KEYS + r, d = (word % G) * 32 + (word / G) * 8;
+      uint4 k = make_uint4(0, 0, 0, 0), v = k;
+      if (j < seen) {
+        const size_t at = (size_t)unit * p.c.ctx + j;
+        const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_codes + at * (HD / 2)) + word), vw = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_codes + at * (HD / 2)) + word);
+        const float ks = __half2float(p.c.k_scales[at * nb + d / p.c.bs]);
+        float vs = __half2float(p.c.v_scales[at * nb + d / p.c.bs]);
+        if (vs != vs) {
+          atomicMin(&s_bad[d / p.c.bs], j);
+          vs = 0.f;
+        }
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = cache4_value(kw, e, ks);
+        k = pack8<__half>(x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = cache4_value(vw, e, vs);
+        v = pack8<__half>(x);
+      }
+      const size_t to = ((size_t)unit * a.t_pad + j) * HD + d;
+      *reinterpret_cast<uint4*>(a.k_half + to) = k;
+      *reinterpret_cast<uint4*>(a.v_half + to) = v;
+    }
+    __syncthreads();
+    if (threadIdx.x < 4) a.bad[((size_t)unit * key_blocks + b) * 4 + threadIdx.x] = s_bad[threadIdx.x];
+    return;
+  }
+  // queries: HD / 8 lanes per row
+  const int group = p.n_heads / p.c.n_kv, rows = p.m * group;
+  for (int w = threadIdx.x; w < PR_ROWS * WORDS; w += 256) {
+    const int r = (b - key_blocks) * PR_ROWS + w / WORDS, word = w % WORDS;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    float down = 1.f;
+    if (r < rows) v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + ((size_t)seq * p.m + r / group) * p.ld_q + (kvh * group + r % group) * HD + word * 8);
+    if (sizeof(T) == 2 && !std::is_same<T, __half>::value) {  // a power of two takes the row's largest magnitude into [1, 2)
+      float x[8], most = 0.f;
+      unpack8<T>(v, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+#pragma unroll
+      for (int o = 1; o < WORDS; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      const int ex = (int)(__float_as_uint(most) >> 23);
+      float up = 1.f;
+      if (ex >= 20 && ex <= 230) {
+        up = __uint_as_float((uint32_t)(254 - ex) << 23);
+        down = __uint_as_float((uint32_t)ex << 23);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= up;
+      v = pack8<__half>(x);
+    }
+    *reinterpret_cast<uint4*>(a.q_half + ((size_t)unit * a.r_pad + r) * HD + word * 8) = v;
+    if (word == 0) a.row_stats[(size_t)unit * a.r_pad + r] = make_float2(down * (1.4426950408889634f * rsqrtf((float)HD)), INFINITY);
+  }
+}
+
+// ------------------------------------------------------------------ shared pieces
+__device__ __forceinline__ float ex2(float y) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+  return r;
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void st_32x32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols) : "memory");
+}
+
+template <int HD>
+struct prompt_shape {
+  static constexpr int NKB = HD / 64;                        // 64-wide blocks of the head dimension
+  static constexpr uint32_t BLOCK = 128 * 64 * 2;            // 128 rows x 64 dimensions
+  static constexpr uint32_t OPERAND = NKB * BLOCK;           // queries, keys or values (2 x NKB atoms of 64 keys x 64 dimensions)
+  static constexpr int RING = HD == 128 ? 2 : 4;             // two CTAs per SM
+  static constexpr uint32_t SMEM = (1 + RING) * OPERAND + 1024 /* alignment slack */ + 256 /* barriers, tensor-memory slot */;
+  static constexpr uint32_t IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);  // values: contiguous along the dimension
+};
+
+// barriers
+constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + 4, B_S = B_EMPTY + 4, B_P = B_S + 1, B_O = B_P + 1, B_COUNT = B_O + 1;
+
+// ------------------------------------------------------------------ outputs
+template <typename T, int HD>
+__global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                         const __grid_constant__ CUtensorMap map_v, const prompt_args a, int row_blocks, int units) {
+  using sh = prompt_shape<HD>;
+  constexpr int NKB = sh::NKB, RING = sh::RING;
+  constexpr uint32_t OPERAND = sh::OPERAND, V_ATOM = 64 * 64 * 2, TMEM_COLS = 256, O_COL = 128;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t q_addr = base, ring_addr = base + OPERAND;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (1 + RING) * OPERAND);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ int s_bad[4];
+  const cache4_attention_params& p = a.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the last rows, which see most, first; all units' side by side
+  const int block = row_blocks - 1 - (int)blockIdx.x / units, unit = (int)blockIdx.x % units, seq = unit / p.c.n_kv, kvh = unit % p.c.n_kv;
+  const int group = p.n_heads / p.c.n_kv, rows = p.m * group, r0 = block * PR_ROWS;
+
+  if (tid == 0) {
+    mbar_init(smem_u32(&bars[B_Q]), 1);
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(smem_u32(&bars[B_FULL + i]), 1);
+      mbar_init(smem_u32(&bars[B_EMPTY + i]), 1);
+    }
+    mbar_init(smem_u32(&bars[B_S]), 1);
+    mbar_init(smem_u32(&bars[B_P]), PR_SOFT_WARPS);
+    mbar_init(smem_u32(&bars[B_O]), 1);
+    *failed = 0;
+    fence_mbar_init();
+  }
+  if (tid < 4) s_bad[tid] = 0x7fffffff;
+  if (warp == PR_SOFT_WARPS + 1) tmem_alloc(tmem_slot, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr bool HEED = false;  // (an earlier launch's error says nothing about this one)
+  const int held = p.lengths[seq];
+  const int n_tiles = (limit_of(p, held, min(r0 + PR_ROWS, rows) / group - (min(r0 + PR_ROWS, rows) % group == 0)) + PR_KEYS - 1) / PR_KEYS;
+
+  if (warp == PR_SOFT_WARPS) {
+    if (n_tiles && tc_elect()) {  // ---- loads: queries; K_0, V_0, K_1, V_1, ..
+      mbar_arrive_expect_tx(smem_u32(&bars[B_Q]), OPERAND);
+      for (int kb = 0; kb < NKB; ++kb) tma_load_3d(q_addr + kb * sh::BLOCK, &map_q, kb * 64, r0, unit, smem_u32(&bars[B_Q]));
+      tc_ring r;
+      for (int it = 0; it < 2 * n_tiles; ++it, r.step(RING)) {
+        if (!mbar_wait(smem_u32(&bars[B_EMPTY + r.slot]), r.phase ^ 1u, a.err, DEV_ERR_EMPTY_WAIT, HEED)) break;
+        const uint32_t full = smem_u32(&bars[B_FULL + r.slot]), dst = ring_addr + (uint32_t)r.slot * OPERAND;
+        const int j0 = (it >> 1) * PR_KEYS;
+        mbar_arrive_expect_tx(full, OPERAND);
+        if (!(it & 1)) {
+          for (int kb = 0; kb < NKB; ++kb) tma_load_3d(dst + kb * sh::BLOCK, &map_k, kb * 64, j0, unit, full);
+        } else {
+          for (int kb2 = 0; kb2 < 2; ++kb2)
+            for (int c = 0; c < NKB; ++c) tma_load_3d(dst + (kb2 * NKB + c) * V_ATOM, &map_v, c * 64, j0 + kb2 * 64, unit, full);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == PR_SOFT_WARPS + 1) {
+    // ---- products, in this order: S_0, O += P_0 V_0, S_1, ..: scores only replace probabilities that have been read
+    bool ok = n_tiles > 0 && mbar_wait_warp(smem_u32(&bars[B_Q]), 0, a.err, DEV_ERR_FULL_WAIT, HEED);
+    tc_ring r;
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      ok = mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
+      if (!ok) break;
+      tc_fence_after();
+      if (tc_elect()) {
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+          const uint64_t a_desc = smem_desc_sw128(q_addr + kb * sh::BLOCK), b_desc = smem_desc_sw128(ring_addr + (uint32_t)r.slot * OPERAND + kb * sh::BLOCK);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, a_desc + 2 * k, b_desc + 2 * k, sh::IDESC_S, (kb | k) != 0);
+        }
+        tc_commit(smem_u32(&bars[B_EMPTY + r.slot]));
+        tc_commit(smem_u32(&bars[B_S]));
+      }
+      __syncwarp();
+      r.step(RING);
+      ok = mbar_wait_warp(smem_u32(&bars[B_P]), (uint32_t)j & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
+      ok = ok && mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
+      if (!ok) break;
+      tc_fence_after();
+      if (tc_elect()) {
+#pragma unroll
+        for (int kb2 = 0; kb2 < 2; ++kb2) {
+          const uint64_t b_desc = smem_desc_sw128_mn(ring_addr + (uint32_t)r.slot * OPERAND + kb2 * NKB * V_ATOM, V_ATOM);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_ts(tmem + O_COL, tmem + kb2 * 32 + k * 8, b_desc + (uint64_t)(k * 2048 >> 4), sh::IDESC_PV, (j | kb2 | k) != 0);
+        }
+        tc_commit(smem_u32(&bars[B_EMPTY + r.slot]));
+        if (j + 1 == n_tiles) tc_commit(smem_u32(&bars[B_O]));
+      }
+      __syncwarp();
+      r.step(RING);
+    }
+    if (!ok && n_tiles) {  // (lets the softmax warps leave, without results)
+      if (tc_elect()) {
+        *failed = 1;
+        __threadfence_block();
+        tc_commit(smem_u32(&bars[B_S]));
+        tc_commit(smem_u32(&bars[B_O]));
+      }
+      __syncwarp();
+    }
+  } else {
+    // ---- softmax: a thread owns row r0 + tid
+    const int r = r0 + tid, i = r / group, limit = r < rows ? limit_of(p, held, i) : 0;
+    const int warp_limit = __shfl_sync(0xffffffffu, limit, 0);  // (what the warp's first row sees; a row that is none: 0, see below)
+    const bool all_there = __all_sync(0xffffffffu, r < rows);
+    const uint32_t s_at = tmem + ((uint32_t)(warp * 32) << 16), o_at = s_at + O_COL;
+    const float f = a.row_stats[(size_t)unit * a.r_pad + r].x;
+    // the first tile that holds a row of no numbers among those this CTA sees
+    if (n_tiles) {
+      const int nb = HD / p.c.bs;
+      const int* list = a.bad + (size_t)unit * (a.t_pad / PR_KEYS) * 4;
+      for (int e = tid; e < n_tiles * nb; e += 32 * PR_SOFT_WARPS) {
+        const int v = list[(e / nb) * 4 + e % nb];
+        if (v != 0x7fffffff) atomicMin(&s_bad[e % nb], v);
+      }
+    }
+    float less = 0.f, high = -INFINITY, sum = 0.f;  // minus the maximum (0 while there is none); 8 above it, as the products give scores
+    bool go = true;
+    for (int j = 0; j < n_tiles; ++j) {
+      const bool ok = mbar_wait(smem_u32(&bars[B_S]), (uint32_t)j & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
+      tc_fence_after();
+      go = __all_sync(0xffffffffu, ok && *failed == 0);
+      if (!go) break;
+      const int left = limit - j * PR_KEYS;  // keys of the tile that the row sees
+      const bool ragged = !all_there || warp_limit < (j + 1) * PR_KEYS;
+      uint32_t pw[64];
+      float top, part;
+      auto tile = [&]() {
+        top = -INFINITY;
+        part = 0.f;
+        uint32_t x[2][32];
+        tc_ld_32x32(s_at, x[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tc_wait_ld();
+          if (c < 3) tc_ld_32x32(s_at + (uint32_t)((c + 1) * 32), x[(c + 1) & 1]);
+          uint32_t(&s)[32] = x[c & 1];
+          if (ragged) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= left) s[e] = 0xff800000u;
+          }
+          float t0 = -INFINITY, t1 = -INFINITY, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float s0 = __uint_as_float(s[e]), s1 = __uint_as_float(s[e + 1]);
+            t0 = fmaxf(t0, s0);
+            t1 = fmaxf(t1, s1);
+            const float e0 = ex2(fmaf(s0, f, less)), e1 = ex2(fmaf(s1, f, less));
+            a0 += e0;
+            a1 += e1;
+            pw[c * 16 + e / 2] = pack2<__half>(e0, e1);
+          }
+          top = fmaxf(top, fmaxf(t0, t1));
+          part += a0 + a1;
+        }
+      };
+      tile();
+      if (__any_sync(0xffffffffu, top > high)) {
+        const bool none = high == -INFINITY;
+        float now = top * f;
+        if (!none) now = fmaxf(now, -less);
+        const float k = none ? 0.f : ex2(-less - now);
+        less = now == -INFINITY ? 0.f : -now;
+        high = (now + 8.f) / f;
+        sum *= k;
+        if (j) {
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t x[32];
+            tc_ld_32x32(o_at + (uint32_t)(c * 32), x);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * k);
+            st_32x32(o_at + (uint32_t)(c * 32), x);
+          }
+        }
+        tile();
+      }
+      sum += part;
+      st_32x32(s_at, pw);
+      st_32x32(s_at + 32, pw + 32);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bars[B_P]));
+    }
+    bar_sync(1, 32 * PR_SOFT_WARPS);  // (s_bad)
+    if (n_tiles) {
+      const bool ok = mbar_wait(smem_u32(&bars[B_O]), 0, a.err, DEV_ERR_TMEM_WAIT, HEED);
+      tc_fence_after();
+      go = __all_sync(0xffffffffu, go && ok && *failed == 0);
+    }
+    if (go) {
+      const float rl = limit ? 1.f / sum : 0.f;
+      T* out = reinterpret_cast<T*>(p.out) + ((size_t)seq * p.m + i) * p.ld_out + (kvh * group + r % group) * HD;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t x[32];
+        if (n_tiles) {
+          tc_ld_32x32(o_at + (uint32_t)(c * 32), x);
+          tc_wait_ld();
+        }
+        if (r < rows) {
+          const bool none = limit && s_bad[c * 32 / p.c.bs] < limit;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = none ? __int_as_float(0x7fffffff) : limit ? __uint_as_float(x[q * 8 + e]) * rl : 0.f;
+            reinterpret_cast<uint4*>(out)[c * 4 + q] = pack8<T>(y);
+          }
+        }
+      }
+      if (p.weights && r < rows) a.row_stats[(size_t)unit * a.r_pad + r].y = limit ? log2f(sum) - less : INFINITY;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == PR_SOFT_WARPS + 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_free(tmem, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ weights
+// One CTA per (sequence, key/value head, 128 cached rows), two per SM; rows of the call in tiles of 128 through a ring.  Two score
+// accumulators: one tile's exponentials run under the next one's product.
+constexpr int W_KEYS = 0, W_FULL = 1, W_EMPTY = W_FULL + 2, W_S = W_EMPTY + 2, W_FREE = W_S + 2, W_COUNT = W_FREE + 2;
+template <int HD>
+__global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const prompt_args a,
+                                                                       int key_blocks, int units) {
+  using sh = prompt_shape<HD>;
+  constexpr int NKB = sh::NKB;
+  constexpr uint32_t OPERAND = sh::OPERAND, TMEM_COLS = 256, STATS = 128 * sizeof(float2), STAGE = OPERAND + STATS;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t k_addr = base, ring_addr = base + OPERAND, stats_addr = ring_addr + 2 * OPERAND;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 3 * OPERAND + 2 * STATS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + W_COUNT);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const cache4_attention_params& p = a.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int block = (int)blockIdx.x / units, unit = (int)blockIdx.x % units, seq = unit / p.c.n_kv;
+  const int group = p.n_heads / p.c.n_kv, rows = p.m * group, j0 = block * PR_KEYS;
+  if (tid == 0) {
+    mbar_init(smem_u32(&bars[W_KEYS]), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars[W_FULL + i]), 1);
+      mbar_init(smem_u32(&bars[W_EMPTY + i]), 1 + PR_SOFT_WARPS);
+      mbar_init(smem_u32(&bars[W_S + i]), 1);
+      mbar_init(smem_u32(&bars[W_FREE + i]), PR_SOFT_WARPS);
+    }
+    *failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == PR_SOFT_WARPS + 1) tmem_alloc(tmem_slot, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  constexpr bool HEED = false;
+  const int held = p.lengths[seq], seen = rows_of(p, held);
+  // rows from the first that sees the first key on
+  const int first = max(0, j0 - held) * group / PR_ROWS, n_tiles = j0 < seen ? (rows + PR_ROWS - 1) / PR_ROWS - first : 0;
+
+  if (warp == PR_SOFT_WARPS) {
+    if (n_tiles > 0 && tc_elect()) {
+      mbar_arrive_expect_tx(smem_u32(&bars[W_KEYS]), OPERAND);
+      for (int kb = 0; kb < NKB; ++kb) tma_load_3d(k_addr + kb * sh::BLOCK, &map_k, kb * 64, j0, unit, smem_u32(&bars[W_KEYS]));
+      tc_ring r;
+      for (int it = 0; it < n_tiles; ++it, r.step(2)) {
+        if (!mbar_wait(smem_u32(&bars[W_EMPTY + r.slot]), r.phase ^ 1u, a.err, DEV_ERR_EMPTY_WAIT, HEED)) break;
+        const uint32_t full = smem_u32(&bars[W_FULL + r.slot]);
+        mbar_arrive_expect_tx(full, STAGE);
+        for (int kb = 0; kb < NKB; ++kb) tma_load_3d(ring_addr + (uint32_t)r.slot * OPERAND + kb * sh::BLOCK, &map_q, kb * 64, (first + it) * PR_ROWS, unit, full);
+        bulk_g2s(stats_addr + (uint32_t)r.slot * STATS, a.row_stats + (size_t)unit * a.r_pad + (first + it) * PR_ROWS, STATS, full);
+      }
+    }
+    __syncwarp();
+  } else if (warp == PR_SOFT_WARPS + 1) {
+    bool ok = n_tiles > 0 && mbar_wait_warp(smem_u32(&bars[W_KEYS]), 0, a.err, DEV_ERR_FULL_WAIT, HEED);
+    tc_ring r;
+    for (int it = 0; it < n_tiles && ok; ++it, r.step(2)) {
+      ok = mbar_wait_warp(smem_u32(&bars[W_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
+      ok = ok && mbar_wait_warp(smem_u32(&bars[W_FREE + r.slot]), r.phase ^ 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
+      if (!ok) break;
+      tc_fence_after();
+      if (tc_elect()) {
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+          const uint64_t a_desc = smem_desc_sw128(k_addr + kb * sh::BLOCK), b_desc = smem_desc_sw128(ring_addr + (uint32_t)r.slot * OPERAND + kb * sh::BLOCK);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_f16(tmem + (uint32_t)(r.slot * 128), a_desc + 2 * k, b_desc + 2 * k, sh::IDESC_S, (kb | k) != 0);
+        }
+        tc_commit(smem_u32(&bars[W_EMPTY + r.slot]));
+        tc_commit(smem_u32(&bars[W_S + r.slot]));
+      }
+      __syncwarp();
+    }
+    if (!ok && n_tiles > 0) {
+      if (tc_elect()) {
+        *failed = 1;
+        __threadfence_block();
+        tc_commit(smem_u32(&bars[W_S]));
+        tc_commit(smem_u32(&bars[W_S + 1]));
+      }
+      __syncwarp();
+    }
+  } else if (n_tiles > 0) {
+    const int j = j0 + tid;
+    // the first row that sees the key (none sees one behind the last)
+    const int from = j >= seen ? 0x7fffffff : max(0, j - held) * group;
+    float total = 0.f;
+    bool go = true;
+    tc_ring r;
+    for (int it = 0; it < n_tiles; ++it, r.step(2)) {
+      const bool ok = mbar_wait(smem_u32(&bars[W_S + r.slot]), r.phase, a.err, DEV_ERR_TMEM_WAIT, HEED);
+      tc_fence_after();
+      go = __all_sync(0xffffffffu, ok && *failed == 0);
+      if (!go) break;
+      const int q0 = (first + it) * PR_ROWS;
+      const bool ragged = !__all_sync(0xffffffffu, from <= q0) || q0 + PR_ROWS > rows;
+      const uint32_t s_at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(r.slot * 128);
+      const float4* st = reinterpret_cast<const float4*>(smem + 3 * OPERAND + (size_t)r.slot * STATS);
+      float part = 0.f;
+      uint32_t x[2][32];
+      tc_ld_32x32(s_at, x[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tc_wait_ld();
+        if (c < 3) tc_ld_32x32(s_at + (uint32_t)((c + 1) * 32), x[(c + 1) & 1]);
+        const uint32_t(&s)[32] = x[c & 1];
+        float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float4 fl = st[c * 16 + e / 2];
+          float e0 = ex2(fmaf(__uint_as_float(s[e]), fl.x, -fl.y)), e1 = ex2(fmaf(__uint_as_float(s[e + 1]), fl.z, -fl.w));
+          if (ragged) {
+            const int row = q0 + c * 32 + e;
+            if (row < from || row >= rows) e0 = 0.f;
+            if (row + 1 < from || row + 1 >= rows) e1 = 0.f;
+          }
+          a0 += e0;
+          a1 += e1;
+        }
+        part += a0 + a1;
+      }
+      total += part;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&bars[W_FREE + r.slot]));
+        mbar_arrive(smem_u32(&bars[W_EMPTY + r.slot]));
+      }
+    }
+    if (go && j < seen) {
+      float* to = p.weights + (size_t)unit * p.c.ctx + j;
+      *to = p.beta == 0.f || j >= held ? total : fmaf(p.beta, *to, total);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == PR_SOFT_WARPS + 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_free(tmem, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ host
+size_t prompt_layout(prompt_args* a, void* workspace, int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len) {
+  size_t used = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = used;
+    used += round_up(bytes, 128);
+    return (uint8_t*)workspace + at;
+  };
+  const size_t units = (size_t)n_seqs * n_kv, t_pad = round_up(max_len, PR_KEYS), r_pad = round_up((size_t)m * (n_heads / n_kv), PR_ROWS);
+  uint8_t* k = take(units * t_pad * hd * 2);
+  uint8_t* v = take(units * t_pad * hd * 2);
+  uint8_t* q = take(units * r_pad * hd * 2);
+  uint8_t* stats = take(units * r_pad * sizeof(float2));
+  uint8_t* bad = take(units * (t_pad / PR_KEYS) * 4 * sizeof(int));
+  if (a) {
+    a->k_half = (__half*)k;
+    a->v_half = (__half*)v;
+    a->q_half = (__half*)q;
+    a->row_stats = (float2*)stats;
+    a->bad = (int*)bad;
+    a->t_pad = (int)t_pad;
+    a->r_pad = (int)r_pad;
+  }
+  return used;
+}
+
+template <typename K>
+int allow_smem(K* kernel, uint32_t bytes, bool (&done)[16]) {
+  int dev = 0;
+  LCU_CUDA(cudaGetDevice(&dev));
+  if (dev >= 16 || !done[dev]) {
+    LCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 16) done[dev] = true;
+  }
+  return LCU_OK;
+}
+
+template <typename T, int HD>
+int launch_prompt(const prompt_args& a, cudaStream_t stream) {
+  using sh = prompt_shape<HD>;
+  const cache4_attention_params& p = a.p;
+  const int units = p.c.n_seqs * p.c.n_kv, key_blocks = a.t_pad / PR_KEYS, row_blocks = a.r_pad / PR_ROWS;
+  CUtensorMap map_q, map_k, map_v;
+  {
+    const uint64_t rows_q[3] = {(uint64_t)HD, (uint64_t)a.r_pad, (uint64_t)units}, step_q[2] = {(uint64_t)HD * 2, (uint64_t)a.r_pad * HD * 2};
+    const uint64_t rows_k[3] = {(uint64_t)HD, (uint64_t)a.t_pad, (uint64_t)units}, step_k[2] = {(uint64_t)HD * 2, (uint64_t)a.t_pad * HD * 2};
+    const uint32_t box[3] = {64, 128, 1}, box_v[3] = {64, 64, 1};
+    int rc = tc_encode_map(&map_q, a.q_half, 3, rows_q, step_q, box);
+    if (!rc) rc = tc_encode_map(&map_k, a.k_half, 3, rows_k, step_k, box);
+    if (!rc) rc = tc_encode_map(&map_v, a.v_half, 3, rows_k, step_k, box_v);
+    if (rc) return rc;
+  }
+  prompt_expand_kernel<T, HD><<<(unsigned)units * (key_blocks + row_blocks), 256, 0, stream>>>(a, key_blocks, row_blocks);
+  static bool done[16] = {}, done_w[16] = {};
+  int rc = allow_smem(prompt_attention_kernel<T, HD>, sh::SMEM, done);
+  if (rc) return rc;
+  LCU_CUDA(launch_after(prompt_attention_kernel<T, HD>, dim3((unsigned)units * row_blocks), dim3(PR_THREADS), sh::SMEM, stream, map_q, map_k, map_v, a, row_blocks, units));
+  if (p.weights) {
+    constexpr uint32_t SMEM_W = 3 * sh::OPERAND + 2 * 128 * sizeof(float2) + 1024 + 256;
+    rc = allow_smem(prompt_weights_kernel<HD>, SMEM_W, done_w);
+    if (rc) return rc;
+    LCU_CUDA(launch_after(prompt_weights_kernel<HD>, dim3((unsigned)units * key_blocks), dim3(PR_THREADS), SMEM_W, stream, map_q, map_k, a, key_blocks, units));
+  }
+  return LCU_OK;
+}
+
+}  // namespace
+
+size_t attention_cache4_prompt_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len) {
+  return prompt_layout(nullptr, nullptr, n_seqs, m, n_heads, n_kv, hd, max_len);
+}
+
+int launch_attention_cache4_prompt(const cache4_attention_params& p, int dtype, void* workspace, cudaStream_t stream) {
+  const long long units = (long long)p.c.n_seqs * p.c.n_kv, rows = (long long)p.m * (p.n_heads / p.c.n_kv);
+  LCU_REQUIRE(rows < (1ll << 30) && units * ((p.max_len + rows) / 128 + 2) < (1ll << 31), "attention_cache4: %d sequences of %d rows of %d heads over %d rows are too many", p.c.n_seqs,
+              p.m, p.n_heads, p.max_len);
+  prompt_args a{};
+  a.p = p;
+  a.err = device_scratch_words();
+  LCU_REQUIRE(a.err != nullptr, "attention_cache4: no error word");
+  prompt_layout(&a, workspace, p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.c.hd, p.max_len);
+  if (dtype == OP_F16) return p.c.hd == 128 ? launch_prompt<__half, 128>(a, stream) : launch_prompt<__half, 64>(a, stream);
+  return p.c.hd == 128 ? launch_prompt<__nv_bfloat16, 128>(a, stream) : launch_prompt<__nv_bfloat16, 64>(a, stream);
+}
+
+}  // namespace lcu
