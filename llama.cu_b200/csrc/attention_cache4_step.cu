@@ -6,7 +6,8 @@
 // the wide side of m16n8k16 products (16 keys x 8 columns for the scores, 16 dimensions x 8 columns for the outputs), whose operands are
 // made in registers:
 //   keys: a masked nibble is a half already, the subnormal code * 2^-24 (or * 2^-20, four bits further up; those dimensions' queries
-//     are a sixteenth).  The 7.5 is a product with the column's sum of queries, where the accumulator starts.
+//     are a sixteenth).  The 7.5 is a product with the column's sum of queries, where the accumulator starts.  Where weights are wanted,
+//     code - 7.5 is formed instead: the products' sums then cancel less, and weights are 1.4e-7 off (2-norm) instead of 8e-7, for 1 us of 58.
 //   values: bits or'ed below an exponent are 1024 + code (or 64 + code); less the constant, times the scale, less 7.5 scales: exact.
 // The order of the codes in a row (cache4.cuh) is such that a lane's words of 32 dimensions belong to one block of scales: scores are
 // scaled in binary32 per block after the product, exactly; values take their scale as halves, exactly too (7-bit scales).
@@ -92,6 +93,22 @@ __device__ __forceinline__ void scaled_values(uint32_t w, __half2 s, __half2 c, 
   h[1] = as_word(__hfma2(__hadd2(as_half2(masked_or(w, 0x00f000f0u, 0x54005400u)), high), s, c));
   h[2] = as_word(__hfma2(__hadd2(as_half2(masked_or(v, 0x000f000fu, 0x64006400u)), low), s, c));
   h[3] = as_word(__hfma2(__hadd2(as_half2(masked_or(v, 0x00f000f0u, 0x54005400u)), high), s, c));
+}
+// code - 7.5 for the same nibbles
+__device__ __forceinline__ void centred(uint32_t w, uint32_t (&h)[4]) {
+  const __half2 low = as_half2(0xe400e400u), middle = as_half2(0xc780c780u), high = as_half2(0xd478d478u);  // -1024, -7.5, -71.5
+  const uint32_t v = w >> 8;
+  h[0] = as_word(__hadd2(__hadd2(as_half2(masked_or(w, 0x000f000fu, 0x64006400u)), low), middle));
+  h[1] = as_word(__hadd2(as_half2(masked_or(w, 0x00f000f0u, 0x54005400u)), high));
+  h[2] = as_word(__hadd2(__hadd2(as_half2(masked_or(v, 0x000f000fu, 0x64006400u)), low), middle));
+  h[3] = as_word(__hadd2(as_half2(masked_or(v, 0x00f000f0u, 0x54005400u)), high));
+}
+// code * 2^-24 and code * 2^-20 in turn: the masked bits as they are
+__device__ __forceinline__ void bare(uint32_t w, uint32_t (&h)[4]) {
+  h[0] = w & 0x000f000fu;
+  h[1] = w & 0x00f000f0u;
+  h[2] = (w >> 8) & 0x000f000fu;
+  h[3] = (w >> 8) & 0x00f000f0u;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {  // an 8 x 8 tile of halves, two neighbours of a row per lane
   uint32_t r;
@@ -256,11 +273,11 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
         for (int e = 0; e < 8; ++e) corr[gd / BG] += x[gd][e] * up;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float m = i & 1 ? up * 0.0625f : up;
+          const float m = i & 1 && !WEIGHTS ? up * 0.0625f : up;
           qf[n][gd][i] = pack2<__half>(x[gd][i] * m, x[gd][i + 4] * m);
         }
       }
-      const float factor = down * (16777216.f * 1.4426950408889634f * rsqrtf((float)HD));
+      const float factor = down * ((WEIGHTS ? 1.f : 16777216.f) * 1.4426950408889634f * rsqrtf((float)HD));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         f[n][e] = __shfl_sync(0xffffffffu, factor, (2 * t + e) * 4);
@@ -270,7 +287,10 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
         corr[b] += __shfl_xor_sync(0xffffffffu, corr[b], 1);
         corr[b] += __shfl_xor_sync(0xffffffffu, corr[b], 2);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) start[n][b][e] = __shfl_sync(0xffffffffu, corr[b], (2 * t + e) * 4) * (-7.5f / 16777216.f);
+        for (int e = 0; e < 2; ++e) {
+          const float of_column = __shfl_sync(0xffffffffu, corr[b], (2 * t + e) * 4) * (-7.5f / 16777216.f);
+          start[n][b][e] = WEIGHTS ? 0.f : of_column;
+        }
       }
       if constexpr (WEIGHTS) {
 #pragma unroll
@@ -343,13 +363,19 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
 #pragma unroll
           for (int gb = 0; gb < BG; ++gb) {
             const int gd = b * BG + gb;
-            const uint32_t ka = k0[gd], kb = k1[gd], ka8 = ka >> 8, kb8 = kb >> 8;
-            constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
+            uint32_t ka[4], kb[4];  // pairs of dimensions in the queries' order
+            if constexpr (WEIGHTS) {
+              centred(k0[gd], ka);
+              centred(k1[gd], kb);
+            } else {
+              bare(k0[gd], ka);
+              bare(k1[gd], kb);
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              if (gb == 0) mma_16816_onto(acc[n], ka & LOW, kb & LOW, ka & HIGH, kb & HIGH, qf[n][gd][0], qf[n][gd][1], start[n][b][0], start[n][b][1]);
-              else mma_16816(acc[n], ka & LOW, kb & LOW, ka & HIGH, kb & HIGH, qf[n][gd][0], qf[n][gd][1]);
-              mma_16816(acc[n], ka8 & LOW, kb8 & LOW, ka8 & HIGH, kb8 & HIGH, qf[n][gd][2], qf[n][gd][3]);
+              if (gb == 0) mma_16816_onto(acc[n], ka[0], kb[0], ka[1], kb[1], qf[n][gd][0], qf[n][gd][1], start[n][b][0], start[n][b][1]);
+              else mma_16816(acc[n], ka[0], kb[0], ka[1], kb[1], qf[n][gd][0], qf[n][gd][1]);
+              mma_16816(acc[n], ka[2], kb[2], ka[3], kb[3], qf[n][gd][2], qf[n][gd][3]);
             }
           }
           const float sa = __half2float(half_of(ks[0][b >> 1], b & 1)), sb = __half2float(half_of(ks[1][b >> 1], b & 1));
