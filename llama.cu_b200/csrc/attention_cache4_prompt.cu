@@ -506,28 +506,32 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
       const uint32_t s_at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(r.slot * 128);
       const float4* st = reinterpret_cast<const float4*>(smem + 3 * OPERAND + (size_t)r.slot * STATS);
       float part = 0.f;
-      uint32_t x[2][32];
-      tc_ld_32x32(s_at, x[0]);
+      auto tile = [&](auto checked) {  // (checked: some of the keys, or of the rows, are none that count)
+        uint32_t x[2][32];
+        tc_ld_32x32(s_at, x[0]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tc_wait_ld();
-        if (c < 3) tc_ld_32x32(s_at + (uint32_t)((c + 1) * 32), x[(c + 1) & 1]);
-        const uint32_t(&s)[32] = x[c & 1];
-        float a0 = 0.f, a1 = 0.f;
+        for (int c = 0; c < 4; ++c) {
+          tc_wait_ld();
+          if (c < 3) tc_ld_32x32(s_at + (uint32_t)((c + 1) * 32), x[(c + 1) & 1]);
+          const uint32_t(&s)[32] = x[c & 1];
+          float a0 = 0.f, a1 = 0.f;
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float4 fl = st[c * 16 + e / 2];
-          float e0 = ex2(fmaf(__uint_as_float(s[e]), fl.x, -fl.y)), e1 = ex2(fmaf(__uint_as_float(s[e + 1]), fl.z, -fl.w));
-          if (ragged) {
-            const int row = q0 + c * 32 + e;
-            if (row < from || row >= rows) e0 = 0.f;
-            if (row + 1 < from || row + 1 >= rows) e1 = 0.f;
+          for (int e = 0; e < 32; e += 2) {
+            const float4 fl = st[c * 16 + e / 2];
+            float e0 = ex2(fmaf(__uint_as_float(s[e]), fl.x, -fl.y)), e1 = ex2(fmaf(__uint_as_float(s[e + 1]), fl.z, -fl.w));
+            if constexpr (decltype(checked)::value) {
+              const int row = q0 + c * 32 + e;
+              if (row < from || row >= rows) e0 = 0.f;
+              if (row + 1 < from || row + 1 >= rows) e1 = 0.f;
+            }
+            a0 += e0;
+            a1 += e1;
           }
-          a0 += e0;
-          a1 += e1;
+          part += a0 + a1;
         }
-        part += a0 + a1;
-      }
+      };
+      if (ragged) tile(std::true_type{});
+      else tile(std::false_type{});
       total += part;
       tc_fence_before();
       __syncwarp();

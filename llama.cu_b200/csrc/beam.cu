@@ -9,8 +9,8 @@
 namespace lcu {
 namespace {
 
-constexpr int BEAM_THREADS = 256, BEAM_ITEMS = 16, BEAM_CHUNK = BEAM_THREADS * BEAM_ITEMS, BEAM_MAX_OUT = 64;
-constexpr size_t BEAM_MAX_SMEM = 160 * 1024;
+constexpr int BEAM_THREADS = 256, BEAM_ITEMS = 16, BEAM_CHUNK = BEAM_THREADS * BEAM_ITEMS, BEAM_GROUPS = 64, BEAM_MAX_OUT = BEAM_GROUPS;
+constexpr int BEAM_MAX_CAND = 2560;  // candidates of a group that shared memory holds
 
 struct beam_args {
   beam_params p;
@@ -36,13 +36,14 @@ __device__ __forceinline__ uint64_t double_order(double x) {
 __device__ __forceinline__ double order_double(uint64_t k) { return __longlong_as_double((long long)(k ^ ((k >> 63) ? 1ull << 63 : ~0ull))); }
 
 // One CTA per (row of logits, chunk of 4096): maximum, sum of exponentials, and the chunk's n best tokens.  A logit's order and its
-// token's complement make one 64-bit number that no other token has, so ties go to the lowest token by themselves.  Every thread keeps
-// the largest of its 16; the n-th largest of those 256 is below the n-th largest of all, and at most n threads hold numbers from it
-// on - 16 n candidates at most, about n as a rule - whose ranks are counted.
+// token's complement make one 64-bit number that no other token has, so ties go to the lowest token by themselves.  The chunk's
+// numbers lie in 64 groups of 64 (four lanes' sixteen); the n-th largest of the groups' largest is no more than the n-th largest of all, and
+// at most n groups hold numbers from it on: 64 n candidates at most, little more than n as a rule, whose ranks are counted.  (Counting
+// the ranks of 256 threads' largest in every thread took 15 of 35 us at 64 rows of 128000.)
 template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args a) {
-  __shared__ uint64_t tops[BEAM_THREADS];
-  __shared__ uint64_t cand[BEAM_MAX_OUT * BEAM_ITEMS];
+  extern __shared__ uint64_t cand[];  // [n_out * 64]
+  __shared__ uint64_t tops[BEAM_GROUPS];
   __shared__ float s_max[8];
   __shared__ double s_sum[8];
   __shared__ uint64_t s_threshold;
@@ -59,19 +60,31 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
 #pragma unroll
   for (int i = 0; i < BEAM_ITEMS; ++i) {
     const int v = v0 + i * BEAM_THREADS + tid;
-    float f = v < a.p.n_vocab ? logit_at(x, v) : -INFINITY;
-    if (f != f) f = -INFINITY;  // no number: never chosen before one
-    val[i] = f;
-    mx = fmaxf(mx, f);
-    if (v < a.p.n_vocab) top = max(top, (uint64_t)float_order(f) << 32 | (uint32_t)~v);
+    val[i] = v < a.p.n_vocab ? logit_at(x, v) : -INFINITY;
   }
-  tops[tid] = top;
+#pragma unroll
+  for (int i = 0; i < BEAM_ITEMS; ++i) {
+    const int v = v0 + i * BEAM_THREADS + tid;
+    if (val[i] != val[i]) val[i] = -INFINITY;  // no number: never chosen before one
+    mx = fmaxf(mx, val[i]);
+    if (v < a.p.n_vocab) top = max(top, (uint64_t)float_order(val[i]) << 32 | (uint32_t)~v);
+  }
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  if ((lane & 3) == 0) tops[tid >> 2] = top;
   mx = warp_max(mx);
   if (lane == 0) s_max[warp] = mx;
   __syncthreads();
   mx = s_max[0];
 #pragma unroll
   for (int w = 1; w < 8; ++w) mx = fmaxf(mx, s_max[w]);
+  if (tid < BEAM_GROUPS) {
+    const uint64_t mine = tops[tid];
+    int rank = 0;
+#pragma unroll 8
+    for (int t = 0; t < BEAM_GROUPS; ++t) rank += tops[t] > mine;
+    if (mine && rank == n_out - 1) s_threshold = mine;
+  }
   double sum = 0.0;
   if (mx > -INFINITY) {
     float part = 0.f;
@@ -82,10 +95,6 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_sum[warp] = sum;
-  int rank = 0;
-#pragma unroll 8
-  for (int t = 0; t < BEAM_THREADS; ++t) rank += tops[t] > top;
-  if (top && rank == n_out - 1) s_threshold = top;
   __syncthreads();
   if (tid == 0) {
     double s = 0.0;
@@ -93,11 +102,13 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
     a.stats[(size_t)row * a.chunks + chunk] = make_float2(mx, (float)s);
   }
   const uint64_t threshold = s_threshold;
+  if (top >= threshold) {  // (others' groups hold none)
 #pragma unroll
-  for (int i = 0; i < BEAM_ITEMS; ++i) {
-    const int v = v0 + i * BEAM_THREADS + tid;
-    const uint64_t k = (uint64_t)float_order(val[i]) << 32 | (uint32_t)~v;
-    if (v < a.p.n_vocab && k >= threshold) cand[atomicAdd(&s_count, 1)] = k;
+    for (int i = 0; i < BEAM_ITEMS; ++i) {
+      const int v = v0 + i * BEAM_THREADS + tid;
+      const uint64_t k = (uint64_t)float_order(val[i]) << 32 | (uint32_t)~v;
+      if (v < a.p.n_vocab && k >= threshold) cand[atomicAdd(&s_count, 1)] = k;
+    }
   }
   __syncthreads();
   const int count = s_count;
@@ -117,14 +128,16 @@ struct scored {
 };
 __device__ __forceinline__ bool better(const scored& a, const scored& b) { return a.order > b.order || (a.order == b.order && a.place < b.place); }
 
-// One CTA per group: log-sum-exp of every beam in 64 bits, then the n best of the chunks' candidates, in the way of the first kernel.
-__global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_args a) {
+// One CTA per group: log-sum-exp of every beam in 64 bits, then the n best of the chunks' candidates.  A thread owns chunks' lists, which are
+// sorted: their heads give a bound in the way of the first kernel, and lists are walked down to it.
+__global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_args a, int most) {
   __shared__ double lse[MAX_BEAMS], base[MAX_BEAMS];
   __shared__ scored tops[BEAM_THREADS];
   __shared__ scored s_threshold;
   __shared__ int s_count;
-  extern __shared__ scored cand[];
-  const int group = blockIdx.x, tid = threadIdx.x, n_out = a.p.n_out, per_beam = a.chunks * n_out;
+  extern __shared__ scored cand_scored[];
+  const int group = blockIdx.x, tid = threadIdx.x, n_out = a.p.n_out;
+  pdl_wait();
   if (tid == 0) {
     s_count = 0;
     s_threshold = scored{0, ~0ull};
@@ -148,36 +161,72 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
     }
   }
   __syncthreads();
-  const int total = a.p.beams * per_beam;
-  auto at = [&](int t) {
-    const int b = t / per_beam, e = t - b * per_beam;
-    if (base[b] == -INFINITY) return e < min(n_out, a.p.n_vocab) ? scored{double_order(-INFINITY), (uint64_t)b * a.p.n_vocab + e} : scored{0, ~0ull};
-    const uint64_t k = a.best[((size_t)group * a.p.beams + b) * per_beam + e];
-    if (!k) return scored{0, ~0ull};
+  const int lists = a.p.beams * a.chunks;
+  // entry e of a list (sorted, best first); a beam at minus infinity has one list of its first tokens
+  auto at = [&](int list, int e) {
+    const int b = list / a.chunks;
+    const uint64_t k = a.best[((size_t)group * lists + list) * n_out + e];
+    const bool fine = base[b] != -INFINITY;
+    if (fine ? !k : list != b * a.chunks || e >= a.p.n_vocab) return scored{0, ~0ull};
+    if (!fine) return scored{double_order(-INFINITY), (uint64_t)b * a.p.n_vocab + e};
     return scored{double_order((double)order_float((uint32_t)(k >> 32)) - lse[b] + base[b]), (uint64_t)b * a.p.n_vocab + (uint32_t)~(uint32_t)k};
   };
   scored top{0, ~0ull};
-  for (int t = tid; t < total; t += BEAM_THREADS) {
-    const scored s = at(t);
+#pragma unroll 4
+  for (int l = tid; l < lists; l += BEAM_THREADS) {
+    const scored s = at(l, 0);
     if (better(s, top)) top = s;
   }
   tops[tid] = top;
   __syncthreads();
   int rank = 0;
+#pragma unroll 8
   for (int t = 0; t < BEAM_THREADS; ++t) rank += better(tops[t], top);
   if (top.order && rank == n_out - 1) s_threshold = top;
   __syncthreads();
   const scored threshold = s_threshold;
-  for (int t = tid; t < total; t += BEAM_THREADS) {
-    const scored s = at(t);
-    if (s.order && !better(threshold, s)) cand[atomicAdd(&s_count, 1)] = s;
-  }
+  for (int l = tid; l < lists; l += BEAM_THREADS)
+    for (int e = 0; e < n_out; ++e) {
+      const scored s = at(l, e);
+      if (!s.order || better(threshold, s)) break;
+      const int place = atomicAdd(&s_count, 1);
+      if (place < most) cand_scored[place] = s;
+    }
   __syncthreads();
   const int count = s_count;
+  if (count > most) {
+    // (thousands above the bound, as where one beam's chunk holds nothing and the others' threads everything: one after another)
+    scored last{~0ull, 0ull};
+    for (int r = 0; r < n_out; ++r) {
+      scored best{0, ~0ull};
+      for (int l = tid; l < lists; l += BEAM_THREADS)
+        for (int e = 0; e < n_out; ++e) {
+          const scored s = at(l, e);
+          if (!s.order || !better(s, best)) break;
+          if (better(last, s)) {
+            best = s;
+            break;
+          }
+        }
+      __syncthreads();
+      tops[tid] = best;
+      __syncthreads();
+      for (int t = 0; t < BEAM_THREADS; ++t)
+        if (better(tops[t], best)) best = tops[t];
+      if (tid == 0) {
+        const size_t o = (size_t)group * n_out + r;
+        a.p.parents[o] = (int)(best.place / a.p.n_vocab);
+        a.p.tokens[o] = (int)(best.place % a.p.n_vocab);
+        a.p.scores_out[o] = (float)order_double(best.order);
+      }
+      last = best;
+    }
+    return;
+  }
   for (int c = tid; c < count; c += BEAM_THREADS) {
-    const scored s = cand[c];
+    const scored s = cand_scored[c];
     int r = 0;
-    for (int t = 0; t < count; ++t) r += better(cand[t], s);
+    for (int t = 0; t < count; ++t) r += better(cand_scored[t], s);
     if (r < n_out) {
       const size_t o = (size_t)group * n_out + r;
       a.p.parents[o] = (int)(s.place / a.p.n_vocab);
@@ -208,24 +257,17 @@ int launch_beam_select(const beam_params& p, int dtype, void* workspace, size_t 
   LCU_REQUIRE(rows * chunks < (1ull << 31), "beam_select: too many rows of logits");
   LCU_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, "beam_select: %zu bytes of 16-byte aligned workspace are needed, %zu are there", need,
               workspace ? workspace_bytes : (size_t)0);
-  // at most n_out threads hold candidates, each of them its share of all
-  const size_t total = (size_t)p.beams * chunks * p.n_out, most = std::min(total, (size_t)p.n_out * ceil_div(total, BEAM_THREADS));
-  const size_t smem = most * sizeof(scored);
-  LCU_REQUIRE(smem <= BEAM_MAX_SMEM, "beam_select: %d of %d beams over a vocabulary of %d are too many", p.n_out, p.beams, p.n_vocab);
+  // at most n_out threads hold candidates, n_out in each of their lists
+  const size_t lists = (size_t)p.beams * chunks;
+  const int most = (int)std::min<size_t>(BEAM_MAX_CAND, std::min(lists, (size_t)p.n_out * ceil_div(lists, BEAM_THREADS)) * p.n_out);
   if (int rc_dev = need_device()) return rc_dev;
-  static bool attr_done[16] = {};
-  int dev = 0;
-  LCU_CUDA(cudaGetDevice(&dev));
-  if (dev >= 16 || !attr_done[dev]) {
-    LCU_CUDA(cudaFuncSetAttribute(beam_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BEAM_MAX_SMEM));
-    if (dev < 16) attr_done[dev] = true;
-  }
   beam_args a{p, chunks, (float2*)workspace, (uint64_t*)((float2*)workspace + rows * chunks)};
   const unsigned ctas = (unsigned)(rows * chunks);
-  if (dtype == OP_F16) beam_rows_kernel<__half><<<ctas, BEAM_THREADS, 0, stream>>>(a);
-  else if (dtype == OP_BF16) beam_rows_kernel<__nv_bfloat16><<<ctas, BEAM_THREADS, 0, stream>>>(a);
-  else beam_rows_kernel<float><<<ctas, BEAM_THREADS, 0, stream>>>(a);
-  beam_group_kernel<<<p.n_groups, BEAM_THREADS, smem, stream>>>(a);
+  const size_t smem_rows = (size_t)p.n_out * (BEAM_CHUNK / BEAM_GROUPS) * sizeof(uint64_t);  // (up to 32 KiB)
+  if (dtype == OP_F16) beam_rows_kernel<__half><<<ctas, BEAM_THREADS, smem_rows, stream>>>(a);
+  else if (dtype == OP_BF16) beam_rows_kernel<__nv_bfloat16><<<ctas, BEAM_THREADS, smem_rows, stream>>>(a);
+  else beam_rows_kernel<float><<<ctas, BEAM_THREADS, smem_rows, stream>>>(a);
+  LCU_CUDA(launch_after(beam_group_kernel, dim3(p.n_groups), dim3(BEAM_THREADS), (size_t)most * sizeof(scored), stream, a, most));
   LCU_CUDA(cudaGetLastError());
   return LCU_OK;
 }

@@ -56,7 +56,9 @@ __device__ __forceinline__ int2 block_exclusive(int2 v, int2* s_warp) {
 
 // One CTA per (sequence, head): the `want` largest of the weights before the latest rows, by digits from the top - a histogram of 2048
 // bins, the bin in which the want-th largest lies, the next digit among that bin's weights - then one pass in row order that writes
-// the rows above the threshold and as many of those at it as are left to take, lowest rows first.
+// the rows above the threshold and as many of those at it as are left to take, lowest rows first.  A warp owns a run of rows; up to 16
+// weights of a thread (16384 of a CTA) stay in registers, so that they are read once: 32 heads of 16000 rows 28 -> SELECT us.
+template <int K>
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_args a) {
   __shared__ int hist[SEL_BINS];
   __shared__ int2 s_warp[32];
@@ -71,6 +73,28 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
   }
   const int old = len - a.recent, want = a.keep - a.recent;  // (len > keep: want < old)
   const float* w = a.weights + (size_t)sh * a.ctx;
+  // the rows of a warp; a thread's are 32 apart
+  const int run = (old + SEL_THREADS - 1) / SEL_THREADS * 32, from = warp * run, to = min(old, from + run);
+  uint32_t held[K > 0 ? K : 1];
+  if constexpr (K > 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = from + k * 32 + lane;
+      held[k] = i < to ? weight_key(w[i]) : 0u;
+    }
+  }
+  // each(f): f(row, its key, whether there is such a row) for the thread's rows, whole warps together
+  auto each = [&](auto&& f) {
+    if constexpr (K > 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (from + k * 32 >= to) break;
+        f(from + k * 32 + lane, held[k], from + k * 32 + lane < to);
+      }
+    } else {
+      for (int i0 = from; i0 < to; i0 += 32) f(i0 + lane, i0 + lane < to ? weight_key(w[i0 + lane]) : 0u, i0 + lane < to);
+    }
+  };
   for (int i = tid; i < a.recent; i += SEL_THREADS) kept[want + i] = old + i;
   if (want == 0) return;
   if (tid == 0) {
@@ -84,10 +108,8 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
     __syncthreads();
     const uint32_t prefix = s_prefix;
     const int left = s_left;
-    for (int i0 = warp * 32; i0 < old; i0 += SEL_THREADS) {
-      const int i = i0 + lane;
-      const uint32_t key = i < old ? weight_key(w[i]) : 0u;
-      const bool in = i < old && (pass == 0 || (key >> (shift + bits)) == prefix);
+    each([&](int, uint32_t key, bool there) {
+      const bool in = there && (pass == 0 || (key >> (shift + bits)) == prefix);
       const uint32_t digit = in ? (key >> shift) & ((1u << bits) - 1) : 0xffffffffu;
       int same = 0;
       __match_all_sync(0xffffffffu, digit, &same);  // (equal weights, all zero before the first step: one add instead of 32 on one address)
@@ -96,7 +118,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
       } else if (in) {
         atomicAdd(&hist[digit], 1);
       }
-    }
+    });
     __syncthreads();
     // bins from the top, two per thread
     const int hi = SEL_BINS - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1];
@@ -110,28 +132,23 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
   }
   const uint32_t threshold = s_prefix;
   const int ties = s_left;
-  // a warp owns a run of rows: counts, their sums over the warps before, places
-  const int run = (old + SEL_THREADS - 1) / SEL_THREADS * 32, from = warp * run, to = min(old, from + run);
+  // counts of the warps, their sums over the warps before, places
   int above = 0, equal = 0;
-  for (int i0 = from; i0 < to; i0 += 32) {
-    const uint32_t key = i0 + lane < to ? weight_key(w[i0 + lane]) : 0u;
-    above += __popc(__ballot_sync(0xffffffffu, i0 + lane < to && key > threshold));
-    equal += __popc(__ballot_sync(0xffffffffu, i0 + lane < to && key == threshold));
-  }
+  each([&](int, uint32_t key, bool there) {
+    above += __popc(__ballot_sync(0xffffffffu, there && key > threshold));
+    equal += __popc(__ballot_sync(0xffffffffu, there && key == threshold));
+  });
   int2 base = block_exclusive(lane == 0 ? make_int2(above, equal) : make_int2(0, 0), s_warp);
   base.x = __shfl_sync(0xffffffffu, base.x, 0);
   base.y = __shfl_sync(0xffffffffu, base.y, 0);
-  for (int i0 = from; i0 < to; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t key = i < to ? weight_key(w[i]) : 0u;
+  each([&](int i, uint32_t key, bool there) {
     const uint32_t mine = (1u << lane) - 1;
-    const uint32_t m_above = __ballot_sync(0xffffffffu, i < to && key > threshold), m_equal = __ballot_sync(0xffffffffu, i < to && key == threshold);
+    const uint32_t m_above = __ballot_sync(0xffffffffu, there && key > threshold), m_equal = __ballot_sync(0xffffffffu, there && key == threshold);
     const int tie = base.y + __popc(m_equal & mine);
-    const bool take = i < to && (key > threshold || (key == threshold && tie < ties));
-    if (take) kept[base.x + __popc(m_above & mine) + min(tie, ties)] = i;
+    if (there && (key > threshold || (key == threshold && tie < ties))) kept[base.x + __popc(m_above & mine) + min(tie, ties)] = i;
     base.x += __popc(m_above);
     base.y += __popc(m_equal);
-  }
+  });
 }
 
 struct plane {
@@ -183,9 +200,18 @@ __device__ __forceinline__ void gather_rows(const gather_args& a, const plane& p
   }
 }
 
+// by one CTA of the kernels that move rows, which go by the list of kept ones: lengths_out may be lengths
+__device__ __forceinline__ void write_lengths(const gather_args& a) {
+  if (a.lengths_out)
+    for (int s = threadIdx.x; s < a.n_seqs; s += blockDim.x) a.lengths_out[s] = min(min(a.lengths[s], a.ctx), a.keep);
+}
+__global__ void __launch_bounds__(256) evict_lengths_kernel(const gather_args a) { write_lengths(a); }
+
 // Rows into other planes: a CTA per (sequence, head, run of kept rows); bound by memory.
 __global__ void __launch_bounds__(256) evict_gather_kernel(const gather_args a, int rows_per_cta, int chunks) {
   const plane p = a.planes[blockIdx.y];
+  pdl_wait();
+  if (blockIdx.x == 0 && blockIdx.y == 0) write_lengths(a);
   const int sh = blockIdx.x / chunks, first = (blockIdx.x % chunks) * rows_per_cta, last = min(a.keep, first + rows_per_cta);
   switch (unit_bytes(p)) {
     case 16: gather_rows<uint4>(a, p, sh, first, last); break;
@@ -224,6 +250,8 @@ __device__ __forceinline__ void move_rows(const gather_args& a, const plane& p, 
 }
 __global__ void __launch_bounds__(256) evict_move_kernel(const gather_args a) {
   const plane p = a.planes[blockIdx.y];
+  pdl_wait();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) write_lengths(a);
   const int sh = blockIdx.x, unit = unit_bytes(p), col_units = max(1, 32 / unit), col = blockIdx.z * col_units;
   if (col >= p.row_bytes / unit) return;
   switch (unit) {
@@ -232,10 +260,6 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const gather_args a) {
     case 4: move_rows<uint32_t>(a, p, sh, col, col_units); break;
     default: move_rows<uint16_t>(a, p, sh, col, col_units); break;
   }
-}
-
-__global__ void evict_lengths_kernel(int* out, const int* lengths, int n, int ctx, int keep) {
-  for (int s = threadIdx.x; s < n; s += blockDim.x) out[s] = min(min(lengths[s], ctx), keep);
 }
 
 struct reorder_args {
@@ -363,12 +387,22 @@ int launch_cache_evict(const evict_params& p, cudaStream_t stream) {
   const int rows = std::max(1, 16384 / std::max(1, widest_away)), chunks = (p.keep + rows - 1) / rows;
   LCU_REQUIRE((long long)heads * chunks < (1ll << 31), "cache_evict: planes are too large");
   if (int rc_dev = need_device()) return rc_dev;
-  evict_select_kernel<<<heads, SEL_THREADS, 0, stream>>>(select_args{p.weights, p.kept, p.lengths, p.n_kv, p.ctx, p.keep, p.recent});
+  const select_args sel{p.weights, p.kept, p.lengths, p.n_kv, p.ctx, p.keep, p.recent};
+  if (p.ctx <= 4 * SEL_THREADS) evict_select_kernel<4><<<heads, SEL_THREADS, 0, stream>>>(sel);
+  else if (p.ctx <= 16 * SEL_THREADS) evict_select_kernel<16><<<heads, SEL_THREADS, 0, stream>>>(sel);
+  else evict_select_kernel<0><<<heads, SEL_THREADS, 0, stream>>>(sel);
   if (n_away) {
-    evict_gather_kernel<<<dim3((unsigned)(heads * chunks), n_away), 256, 0, stream>>>(away, rows, chunks);
+    away.lengths_out = p.lengths_out;
+    LCU_CUDA(launch_after(evict_gather_kernel, dim3((unsigned)(heads * chunks), n_away), dim3(256), 0, stream, away, rows, chunks));
   }
-  if (n_here) evict_move_kernel<<<dim3((unsigned)heads, n_here, (widest_here + 31) / 32), 256, 0, stream>>>(here);
-  if (p.lengths_out) evict_lengths_kernel<<<1, 256, 0, stream>>>(p.lengths_out, p.lengths, p.n_seqs, p.ctx, p.keep);
+  if (n_here) {
+    if (!n_away) here.lengths_out = p.lengths_out;
+    LCU_CUDA(launch_after(evict_move_kernel, dim3((unsigned)heads, n_here, (widest_here + 31) / 32), dim3(256), 0, stream, here));
+  }
+  if (!p.n_planes && p.lengths_out) {
+    away.lengths_out = p.lengths_out;
+    evict_lengths_kernel<<<1, 256, 0, stream>>>(away);
+  }
   LCU_CUDA(cudaGetLastError());
   return LCU_OK;
 }

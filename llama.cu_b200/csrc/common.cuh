@@ -43,8 +43,13 @@ const char* last_error();
 
 // for entry points that check their arguments before they look for a device
 inline int need_device() {
+  static bool seen = false;  // (devices do not go away)
+  if (seen) return LCU_OK;
   int n = 0;
-  if (cudaGetDeviceCount(&n) == cudaSuccess && n > 0) return LCU_OK;
+  if (cudaGetDeviceCount(&n) == cudaSuccess && n > 0) {
+    seen = true;
+    return LCU_OK;
+  }
   cudaGetLastError();
   set_last_error("no CUDA device is visible: this library has no CPU path");
   return LCU_ERR_CUDA;

@@ -491,6 +491,23 @@ def test_beam_select_ties_and_numbers_that_are_none(lcu):
             assert np.array_equal(np.isneginf(out[g]), ~fine) and (np.abs(out[g][fine] - s[fine]) <= 2.0 ** -19 + U * np.abs(s[fine])).all()
 
 
+def test_beam_select_with_thousands_of_candidates_above_the_bound(lcu):
+    """Eight of 32 beams are ahead of all others, so that the bound comes from the 64 threads that own their lists, and one of those has
+    nothing in any of its four: nearly all entries of the other 252 lists lie above it."""
+    rng = np.random.default_rng(77)
+    vocab, beams, n_out = 32 * 4096, 32, 64
+    x = rng.standard_normal((1, beams, vocab)).astype(np.float32)
+    scores = np.full((1, beams), -100.0, np.float32)
+    for b in (0, 1, 8, 9, 16, 17, 24, 25):
+        scores[0, b] = 0.01 * b
+        if b % 8 == 0:
+            x[0, b, :4096] -= 20.0
+    parents, tokens, out = lcu.beam_select(x, scores, n_out)
+    p, t, s = P.beam_select(x[0].astype(np.float64), scores[0].astype(np.float64), n_out)
+    assert np.abs(np.diff(s)).min() > 1e-6  # (nothing that rounding could turn)
+    assert parents[0].tolist() == p.tolist() and tokens[0].tolist() == t.tolist() and (np.abs(out[0] - s) <= 2.0 ** -19 + U * np.abs(s)).all()
+
+
 @pytest.mark.parametrize("groups,beams,kv,ctx,lengths", [
     (1, 1, 2, 5, [5]), (2, 4, 2, 70, [70, 69, 1, 33, 12, 0, -1, 80]), (1, 8, 3, 1000, [1000] * 8), (1, 13, 1, 301, [301] * 13), (1, 32, 1, 64, [40] * 32)])
 def test_reorder(lcu, groups, beams, kv, ctx, lengths):
