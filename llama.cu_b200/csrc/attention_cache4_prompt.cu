@@ -26,7 +26,7 @@
 namespace lcu {
 namespace {
 
-constexpr int PR_ROWS = 128, PR_KEYS = 128, PR_SOFT_WARPS = 4, PR_THREADS = 32 * (PR_SOFT_WARPS + 2);
+constexpr int PR_ROWS = 128, PR_KEYS = 128, PR_SOFT_WARPS = 8, PR_THREADS = 32 * (PR_SOFT_WARPS + 2);
 
 struct prompt_args {
   cache4_attention_params p;
@@ -182,6 +182,8 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ int s_bad[4];
+  __shared__ int s_raise[2][PR_SOFT_WARPS];
+  __shared__ float s_half[2][PR_ROWS];
   const cache4_attention_params& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // the last rows, which see most, first; all units' side by side
@@ -278,13 +280,15 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
       __syncwarp();
     }
   } else {
-    // ---- softmax: a thread owns row r0 + tid
-    const int r = r0 + tid, i = r / group, limit = r < rows ? limit_of(p, held, i) : 0;
-    const int warp_limit = __shfl_sync(0xffffffffu, limit, 0);  // (what the warp's first row sees; a row that is none: 0, see below)
+    // ---- softmax: a thread owns half the keys of a row, its warp and the one four further on 32 rows
+    const int quad = warp & 3, half = warp >> 2, in_tile = quad * 32 + lane;
+    const int r = r0 + in_tile, i = r / group, limit = r < rows ? limit_of(p, held, i) : 0;
+    const int warp_limit = __shfl_sync(0xffffffffu, limit, 0);  // (what the warp's first row sees)
     const bool all_there = __all_sync(0xffffffffu, r < rows);
-    const uint32_t s_at = tmem + ((uint32_t)(warp * 32) << 16), o_at = s_at + O_COL;
+    const uint32_t s_at = tmem + ((uint32_t)(quad * 32) << 16), o_at = s_at + O_COL + (uint32_t)(half * (HD / 2));
     const float f = a.row_stats[(size_t)unit * a.r_pad + r].x;
-    // the first tile that holds a row of no numbers among those this CTA sees
+    auto meet = [&]() { bar_sync(2 + quad, 64); };
+    // the first row of no numbers among those this CTA sees
     if (n_tiles) {
       const int nb = HD / p.c.bs;
       const int* list = a.bad + (size_t)unit * (a.t_pad / PR_KEYS) * 4;
@@ -299,21 +303,18 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
       const bool ok = mbar_wait(smem_u32(&bars[B_S]), (uint32_t)j & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
       tc_fence_after();
       go = __all_sync(0xffffffffu, ok && *failed == 0);
-      if (!go) break;
-      const int left = limit - j * PR_KEYS;  // keys of the tile that the row sees
+      const int left = limit - j * PR_KEYS - half * 64;  // keys of the half tile that the row sees
       const bool ragged = !all_there || warp_limit < (j + 1) * PR_KEYS;
-      uint32_t pw[64];
+      uint32_t pw[32];
       float top, part;
       auto tile = [&]() {
         top = -INFINITY;
         part = 0.f;
-        uint32_t x[2][32];
-        tc_ld_32x32(s_at, x[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32];
+          tc_ld_32x32(s_at + (uint32_t)(half * 64 + c * 32), s);
           tc_wait_ld();
-          if (c < 3) tc_ld_32x32(s_at + (uint32_t)((c + 1) * 32), x[(c + 1) & 1]);
-          uint32_t(&s)[32] = x[c & 1];
           if (ragged) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
@@ -335,7 +336,18 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         }
       };
       tile();
-      if (__any_sync(0xffffffffu, top > high)) {
+      const int mine = (__any_sync(0xffffffffu, top > high) ? 1 : 0) | (go ? 0 : 2);
+      if (lane == 0) s_raise[j & 1][warp] = mine;
+      meet();  // (both halves of the rows' scores are read: probabilities may take their place)
+      const int either = mine | s_raise[j & 1][warp ^ 4];
+      if (either & 2) {  // (the pair leaves together: its barriers count both)
+        go = false;
+        break;
+      }
+      if (either) {
+        s_half[half][in_tile] = top;
+        meet();
+        top = fmaxf(top, s_half[half ^ 1][in_tile]);
         const bool none = high == -INFINITY;
         float now = top * f;
         if (!none) now = fmaxf(now, -less);
@@ -345,26 +357,28 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         sum *= k;
         if (j) {
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
+          for (int c = 0; c < HD / 2; c += 32) {
             uint32_t x[32];
-            tc_ld_32x32(o_at + (uint32_t)(c * 32), x);
+            tc_ld_32x32(o_at + (uint32_t)c, x);
             tc_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * k);
-            st_32x32(o_at + (uint32_t)(c * 32), x);
+            st_32x32(o_at + (uint32_t)c, x);
           }
         }
         tile();
+        meet();
       }
       sum += part;
-      st_32x32(s_at, pw);
-      st_32x32(s_at + 32, pw + 32);
+      st_32x32(s_at + (uint32_t)(half * 32), pw);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bars[B_P]));
     }
-    bar_sync(1, 32 * PR_SOFT_WARPS);  // (s_bad)
+    s_half[half][in_tile] = sum;
+    bar_sync(1, 32 * PR_SOFT_WARPS);  // (sums, s_bad)
+    sum = s_half[0][in_tile] + s_half[1][in_tile];
     if (n_tiles) {
       const bool ok = mbar_wait(smem_u32(&bars[B_O]), 0, a.err, DEV_ERR_TMEM_WAIT, HEED);
       tc_fence_after();
@@ -372,26 +386,26 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
     }
     if (go) {
       const float rl = limit ? 1.f / sum : 0.f;
-      T* out = reinterpret_cast<T*>(p.out) + ((size_t)seq * p.m + i) * p.ld_out + (kvh * group + r % group) * HD;
+      T* out = reinterpret_cast<T*>(p.out) + ((size_t)seq * p.m + i) * p.ld_out + (kvh * group + r % group) * HD + half * (HD / 2);
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
+      for (int c = 0; c < HD / 2; c += 32) {
         uint32_t x[32];
         if (n_tiles) {
-          tc_ld_32x32(o_at + (uint32_t)(c * 32), x);
+          tc_ld_32x32(o_at + (uint32_t)c, x);
           tc_wait_ld();
         }
         if (r < rows) {
-          const bool none = limit && s_bad[c * 32 / p.c.bs] < limit;
+          const bool none = limit && s_bad[(half * (HD / 2) + c) / p.c.bs] < limit;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = none ? __int_as_float(0x7fffffff) : limit ? __uint_as_float(x[q * 8 + e]) * rl : 0.f;
-            reinterpret_cast<uint4*>(out)[c * 4 + q] = pack8<T>(y);
+            reinterpret_cast<uint4*>(out + c)[q] = pack8<T>(y);
           }
         }
       }
-      if (p.weights && r < rows) a.row_stats[(size_t)unit * a.r_pad + r].y = limit ? log2f(sum) - less : INFINITY;
+      if (p.weights && r < rows && half == 0) a.row_stats[(size_t)unit * a.r_pad + r].y = limit ? log2f(sum) - less : INFINITY;
     }
   }
   tc_fence_before();
@@ -417,18 +431,19 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t k_addr = base, ring_addr = base + OPERAND, stats_addr = ring_addr + 2 * OPERAND;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 3 * OPERAND + 2 * STATS);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 3 * OPERAND + 4 * STATS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + W_COUNT);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const cache4_attention_params& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ float s_total[PR_KEYS];
   const int block = (int)blockIdx.x / units, unit = (int)blockIdx.x % units, seq = unit / p.c.n_kv;
   const int group = p.n_heads / p.c.n_kv, rows = p.m * group, j0 = block * PR_KEYS;
   if (tid == 0) {
     mbar_init(smem_u32(&bars[W_KEYS]), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bars[W_FULL + i]), 1);
-      mbar_init(smem_u32(&bars[W_EMPTY + i]), 1 + PR_SOFT_WARPS);
+      mbar_init(smem_u32(&bars[W_EMPTY + i]), 1);
       mbar_init(smem_u32(&bars[W_S + i]), 1);
       mbar_init(smem_u32(&bars[W_FREE + i]), PR_SOFT_WARPS);
     }
@@ -456,7 +471,8 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
         const uint32_t full = smem_u32(&bars[W_FULL + r.slot]);
         mbar_arrive_expect_tx(full, STAGE);
         for (int kb = 0; kb < NKB; ++kb) tma_load_3d(ring_addr + (uint32_t)r.slot * OPERAND + kb * sh::BLOCK, &map_q, kb * 64, (first + it) * PR_ROWS, unit, full);
-        bulk_g2s(stats_addr + (uint32_t)r.slot * STATS, a.row_stats + (size_t)unit * a.r_pad + (first + it) * PR_ROWS, STATS, full);
+        // (the four places of row statistics: scores of four tiles ago are read before the product of two ago may start)
+        bulk_g2s(stats_addr + (uint32_t)(it & 3) * STATS, a.row_stats + (size_t)unit * a.r_pad + (first + it) * PR_ROWS, STATS, full);
       }
     }
     __syncwarp();
@@ -490,7 +506,8 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
       __syncwarp();
     }
   } else if (n_tiles > 0) {
-    const int j = j0 + tid;
+    // a thread owns half the rows of every tile for a key
+    const int quad = warp & 3, half = warp >> 2, j = j0 + quad * 32 + lane;
     // the first row that sees the key (none sees one behind the last)
     const int from = j >= seen ? 0x7fffffff : max(0, j - held) * group;
     float total = 0.f;
@@ -503,24 +520,22 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
       if (!go) break;
       const int q0 = (first + it) * PR_ROWS;
       const bool ragged = !__all_sync(0xffffffffu, from <= q0) || q0 + PR_ROWS > rows;
-      const uint32_t s_at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(r.slot * 128);
-      const float4* st = reinterpret_cast<const float4*>(smem + 3 * OPERAND + (size_t)r.slot * STATS);
+      const uint32_t s_at = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(r.slot * 128 + half * 64);
+      const float4* st = reinterpret_cast<const float4*>(smem + 3 * OPERAND + (size_t)(it & 3) * STATS) + half * 32;
       float part = 0.f;
       auto tile = [&](auto checked) {  // (checked: some of the keys, or of the rows, are none that count)
-        uint32_t x[2][32];
-        tc_ld_32x32(s_at, x[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32];
+          tc_ld_32x32(s_at + (uint32_t)(c * 32), s);
           tc_wait_ld();
-          if (c < 3) tc_ld_32x32(s_at + (uint32_t)((c + 1) * 32), x[(c + 1) & 1]);
-          const uint32_t(&s)[32] = x[c & 1];
           float a0 = 0.f, a1 = 0.f;
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float4 fl = st[c * 16 + e / 2];
             float e0 = ex2(fmaf(__uint_as_float(s[e]), fl.x, -fl.y)), e1 = ex2(fmaf(__uint_as_float(s[e + 1]), fl.z, -fl.w));
             if constexpr (decltype(checked)::value) {
-              const int row = q0 + c * 32 + e;
+              const int row = q0 + half * 64 + c * 32 + e;
               if (row < from || row >= rows) e0 = 0.f;
               if (row + 1 < from || row + 1 >= rows) e1 = 0.f;
             }
@@ -535,12 +550,12 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
       total += part;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&bars[W_FREE + r.slot]));
-        mbar_arrive(smem_u32(&bars[W_EMPTY + r.slot]));
-      }
+      if (lane == 0) mbar_arrive(smem_u32(&bars[W_FREE + r.slot]));
     }
-    if (go && j < seen) {
+    if (half) s_total[quad * 32 + lane] = total;
+    bar_sync(1, 32 * PR_SOFT_WARPS);
+    total += s_total[quad * 32 + lane];
+    if (go && j < seen && !half) {
       float* to = p.weights + (size_t)unit * p.c.ctx + j;
       *to = p.beta == 0.f || j >= held ? total : fmaf(p.beta, *to, total);
     }
@@ -612,7 +627,7 @@ int launch_prompt(const prompt_args& a, cudaStream_t stream) {
   if (rc) return rc;
   LCU_CUDA(launch_after(prompt_attention_kernel<T, HD>, dim3((unsigned)units * row_blocks), dim3(PR_THREADS), sh::SMEM, stream, map_q, map_k, map_v, a, row_blocks, units));
   if (p.weights) {
-    constexpr uint32_t SMEM_W = 3 * sh::OPERAND + 2 * 128 * sizeof(float2) + 1024 + 256;
+    constexpr uint32_t SMEM_W = 3 * sh::OPERAND + 4 * 128 * sizeof(float2) + 1024 + 256;
     rc = allow_smem(prompt_weights_kernel<HD>, SMEM_W, done_w);
     if (rc) return rc;
     LCU_CUDA(launch_after(prompt_weights_kernel<HD>, dim3((unsigned)units * key_blocks), dim3(PR_THREADS), SMEM_W, stream, map_q, map_k, a, key_blocks, units));
