@@ -150,10 +150,12 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
   constexpr int COLS = 8 * NT, ROW = HD / 2, CPR = ROW / 16;
   using ring_t = step_ring<HD, NB>;
   constexpr uint32_t PLANE = ring_t::PLANE, SCALES = ring_t::SCALES, STAGE = ring_t::STAGE;
-  extern __shared__ __align__(128) uint8_t s_raw[];         // rings of the warps; then sums [ST_WARPS][COLS][HD]
-  float* s_o = reinterpret_cast<float*>(s_raw);
+  extern __shared__ __align__(128) uint8_t s_raw[];         // rings of the warps; then their sums, in the order of the accumulators' registers
+  float2* s_o = reinterpret_cast<float2*>(s_raw);
   __shared__ float2 s_ml[ST_WARPS][COLS];
   __shared__ int s_bad[4];
+  __shared__ uint4 s_q[NT][G][32];                          // queries as operands, made by a warp each
+  __shared__ float s_most[NT][G][8], s_sum[NT][G][8], s_f[COLS];
   const cache4_attention_params& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / p.c.n_kv, n_cols = p.m * group, per_seq = p.c.n_kv * a.col_blocks;
@@ -239,63 +241,82 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
       else cp_async_commit();
     }
 
-  // ---- queries as the narrow operand: column g of each n-tile, octet t of every 32 dimensions, in the codes' order of pairs
+    // ---- queries as the narrow operand: column g of each n-tile, octet t of every 32 dimensions, in the codes' order of pairs.  A warp makes
+    // those of 32 dimensions.  A power of two takes the column's largest magnitude into [2^14, 2^15): halves, and their sixteenths,
+    // are exact from 2^-24 of it on.
+    {
+      const int n = warp / G, gd = warp % G, c = c0 + n * 8 + g;
+      float x[8];
+      if (n < NT) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (c < n_cols) v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + row_of(c) * p.ld_q + head_of(c) * HD + gd * 32 + t * 8);
+        unpack8<T>(v, x);
+        float most = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        if (t == 0) s_most[n][gd][g] = most;
+      }
+      __syncthreads();
+      if (n < NT) {
+        float most = s_most[n][0][g];
+#pragma unroll
+        for (int k = 1; k < G; ++k) most = fmaxf(most, s_most[n][k][g]);
+        float up = 1.f, down = 1.f;
+        const int ex = (int)(__float_as_uint(most) >> 23);
+        if (ex >= 20 && ex <= 230) {  // (what is smaller than 2^-107 gives scores of nothing as it is, what is larger than 2^103 infinities)
+          up = __uint_as_float((uint32_t)(127 + 14 + 127 - ex) << 23);
+          down = __uint_as_float((uint32_t)(ex - 14) << 23);
+        }
+        float total = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] *= up;
+          total += x[e];
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float m = i & 1 && !WEIGHTS ? 0.0625f : 1.f;
+          w[i] = pack2<__half>(x[i] * m, x[i + 4] * m);
+        }
+        s_q[n][gd][lane] = make_uint4(w[0], w[1], w[2], w[3]);
+        total += __shfl_xor_sync(0xffffffffu, total, 1);
+        total += __shfl_xor_sync(0xffffffffu, total, 2);
+        if (t == 0) {
+          s_sum[n][gd][g] = total;
+          if (gd == 0) s_f[n * 8 + g] = down * ((WEIGHTS ? 1.f : 16777216.f) * 1.4426950408889634f * rsqrtf((float)HD));
+        }
+      }
+      __syncthreads();
+    }
     uint32_t qf[NT][G][4];
     float f[NT][2], start[NT][NB][2];
     float* at_score[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int c = c0 + n * 8 + g;
-      float x[G][8], most = 0.f;
 #pragma unroll
       for (int gd = 0; gd < G; ++gd) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (c < n_cols) v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + row_of(c) * p.ld_q + head_of(c) * HD + gd * 32 + t * 8);
-        unpack8<T>(v, x[gd]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[gd][e]));
+        const uint4 v = s_q[n][gd][lane];
+        qf[n][gd][0] = v.x;
+        qf[n][gd][1] = v.y;
+        qf[n][gd][2] = v.z;
+        qf[n][gd][3] = v.w;
       }
-      // a power of two takes the column's largest magnitude into [2^14, 2^15): halves, and their sixteenths, are exact from 2^-24 of it on
-      float up = 1.f, down = 1.f;
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const int ex = (int)(__float_as_uint(most) >> 23);
-      if (ex >= 20 && ex <= 250) {  // (what is smaller than 2^-107 gives scores of nothing as it is)
-        up = __uint_as_float((uint32_t)(127 + 14 + 127 - ex) << 23);
-        down = __uint_as_float((uint32_t)(ex - 14) << 23);
-      }
-      float corr[NB];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) corr[b] = 0.f;
-#pragma unroll
-      for (int gd = 0; gd < G; ++gd) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) corr[gd / BG] += x[gd][e] * up;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float m = i & 1 && !WEIGHTS ? up * 0.0625f : up;
-          qf[n][gd][i] = pack2<__half>(x[gd][i] * m, x[gd][i + 4] * m);
-        }
-      }
-      const float factor = down * ((WEIGHTS ? 1.f : 16777216.f) * 1.4426950408889634f * rsqrtf((float)HD));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        f[n][e] = __shfl_sync(0xffffffffu, factor, (2 * t + e) * 4);
-      }
+        const int col = 2 * t + e;
+        f[n][e] = s_f[n * 8 + col];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        corr[b] += __shfl_xor_sync(0xffffffffu, corr[b], 1);
-        corr[b] += __shfl_xor_sync(0xffffffffu, corr[b], 2);
+        for (int b = 0; b < NB; ++b) {
+          float total = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float of_column = __shfl_sync(0xffffffffu, corr[b], (2 * t + e) * 4) * (-7.5f / 16777216.f);
-          start[n][b][e] = WEIGHTS ? 0.f : of_column;
+          for (int k = 0; k < BG; ++k) total += s_sum[n][b * BG + k][col];
+          start[n][b][e] = WEIGHTS ? 0.f : total * (-7.5f / 16777216.f);
         }
-      }
-      if constexpr (WEIGHTS) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int cc = min(c0 + n * 8 + 2 * t + e, n_cols - 1);
+        if constexpr (WEIGHTS) {
+          const int cc = min(c0 + n * 8 + col, n_cols - 1);
           at_score[n][e] = a.scores + (row_of(cc) * p.n_heads + head_of(cc)) * p.max_len;
         }
       }
@@ -498,15 +519,9 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
         l += __shfl_xor_sync(0xffffffffu, l, 4);
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
-        const int c = n * 8 + 2 * t + e;
-        if (g == 0) s_ml[warp][c] = make_float2(high[n][e] == -INFINITY ? -INFINITY : -less[n][e], l);
-        if (c < here) {
+        if (g == 0) s_ml[warp][n * 8 + 2 * t + e] = make_float2(high[n][e] == -INFINITY ? -INFINITY : -less[n][e], l);
 #pragma unroll
-          for (int i = 0; i < VW * 4; ++i) {
-            const int word = g * VW + i / 4, d = (word % G) * 32 + (word / G) * 8 + (i % 4) * 2;
-            *reinterpret_cast<float2*>(&s_o[(warp * COLS + c) * HD + d]) = make_float2(o[n][i][e], o[n][i][e + 2]);
-          }
-        }
+        for (int i = 0; i < VW * 4; ++i) s_o[(((warp * NT + n) * (VW * 4) + i) * 2 + e) * 32 + lane] = make_float2(o[n][i][e], o[n][i][e + 2]);
       }
     }
     if (bad0 != 0x7fffffff) atomicMin(&s_bad[v_block], bad0);
@@ -514,8 +529,10 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
     __syncthreads();
     const bool whole = lo == 0 && hi == chunks;
     const size_t slot = (size_t)blockIdx.x * 2 + (lo == 0);
-    for (int e = tid; e < here * (HD / 2); e += ST_THREADS) {
-      const int c = e / (HD / 2), d = 2 * (e % (HD / 2));
+    for (int e = tid; e < NT * VW * 256; e += ST_THREADS) {
+      const int word = (e & 31) / 4 * VW + (e >> 6) % (VW * 4) / 4, c = (e >> 6) / (VW * 4) * 8 + 2 * (e & 3) + (e >> 5 & 1);
+      const int d = (word % G) * 32 + (word / G) * 8 + (e >> 6) % 4 * 2;  // (register e >> 5 of lane e & 31)
+      if (c >= here) continue;
       float top = -INFINITY, l = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
       for (int w = 0; w < ST_WARPS; ++w) top = fmaxf(top, s_ml[w][c].x);
@@ -523,7 +540,7 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
       for (int w = 0; w < ST_WARPS; ++w) {
         const float2 ml = s_ml[w][c];
         const float k = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // (a maximum of nothing: sums of 0, or of NaN)
-        const float2 v = *reinterpret_cast<const float2*>(&s_o[(w * COLS + c) * HD + d]);
+        const float2 v = s_o[w * (NT * VW * 256) + e];
         l += ml.y * k;
         x += v.x * k;
         y += v.y * k;
@@ -543,87 +560,120 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
   }
 }
 
-// Joins the sums of units that several CTAs did (and gives zeros for sequences not in use): a CTA per unit; and behind those, with weights, a
-// CTA per (sequence, key/value head, 512 rows), which finds maxima and sums of all columns and adds the probabilities in their order.
+// Joins the sums of units that several CTAs did (and gives zeros for sequences not in use): a CTA per unit and column; and behind those, with
+// weights, a CTA per (sequence, key/value head, 512 rows), which finds maxima and sums of all columns and adds the probabilities in
+// their order.  Up to 296 CTAs may have worked on a unit: their maxima are read side by side, their sums by several groups of threads.
 constexpr int JOIN_THREADS = 128, JOIN_KEYS = 4 * JOIN_THREADS;
 template <typename T, int HD, int NB, int NT>
 __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step_args a) {
-  constexpr int COLS = 8 * NT;
+  constexpr int COLS = 8 * NT, LANES = HD / 2, GROUPS = JOIN_THREADS / LANES;
+  __shared__ float s_k[ST_CTAS];
+  __shared__ float2 s_part[GROUPS][LANES];
+  __shared__ float s_warp[JOIN_THREADS / 32];
   const cache4_attention_params& p = a.p;
-  const int tid = threadIdx.x, group = p.n_heads / p.c.n_kv, n_cols = p.m * group, per_seq = p.c.n_kv * a.col_blocks;
-  const int units = p.c.n_seqs * per_seq;
+  const int tid = threadIdx.x, lane = tid & 31, group = p.n_heads / p.c.n_kv, n_cols = p.m * group, per_seq = p.c.n_kv * a.col_blocks;
+  const int joins = p.c.n_seqs * per_seq * COLS;
   const int key_blocks = (p.max_len + JOIN_KEYS - 1) / JOIN_KEYS;
-  const bool joins = (int)blockIdx.x < units;
-  const int sh = joins ? 0 : ((int)blockIdx.x - units) / key_blocks;
-  const int seq = joins ? (int)blockIdx.x / per_seq : sh / p.c.n_kv;
+  const bool join = (int)blockIdx.x < joins;
+  const int sh = join ? 0 : ((int)blockIdx.x - joins) / key_blocks;
+  const int seq = join ? (int)blockIdx.x / (per_seq * COLS) : sh / p.c.n_kv;
   const int held = p.lengths[seq], chunks = step_plan::chunks(p, held);
-  if (!joins && held < 0) return;
+  if (!join && held < 0) return;
   unsigned before, sum_chunks;
   count_chunks(p, seq, before, sum_chunks);
   const step_plan plan(sum_chunks * per_seq, a.ctas);
   pdl_wait();
   auto row_of = [&](int c) { return (size_t)seq * p.m + c / group; };
-  // maximum and sum of column c of a unit, whoever did it
-  auto find = [&](int unit_in_seq, int c, int& first, int& last) {
+  auto ctas_of = [&](int unit_in_seq) {
     const unsigned unit_at = before * per_seq + (unsigned)(unit_in_seq * chunks);
-    first = (int)plan.cta_of(unit_at);
-    last = (int)plan.cta_of(unit_at + chunks - 1);
-    if (first == last) return a.unit_ml ? a.unit_ml[((size_t)seq * per_seq + unit_in_seq) * COLS + c] : make_float2(0.f, 1.f);
-    float2 all = make_float2(-INFINITY, 0.f);
-    for (int b = first; b <= last; ++b) all.x = fmaxf(all.x, a.part_ml[((size_t)b * 2 + (b == first)) * COLS + c].x);
-    for (int b = first; b <= last; ++b) {
-      const float2 ml = a.part_ml[((size_t)b * 2 + (b == first)) * COLS + c];
-      all.y += ml.y * (ml.x == -INFINITY ? 1.f : ex2(ml.x - all.x));
-    }
-    return all;
+    return make_int2((int)plan.cta_of(unit_at), (int)plan.cta_of(unit_at + chunks - 1));
   };
-  if (joins) {
-    const int unit_in_seq = (int)blockIdx.x % per_seq, kvh = unit_in_seq / a.col_blocks, c0 = unit_in_seq % a.col_blocks * COLS, here = min(COLS, n_cols - c0);
-    auto place = [&](int c, int d) {
-      return reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + row_of(c0 + c) * p.ld_out + (kvh * group + (c0 + c) % group) * HD) + d / 2;
-    };
+  auto part_of = [&](int cta, int first, int c) { return a.part_ml[((size_t)cta * 2 + (cta == first)) * COLS + c]; };
+  if (join) {
+    const int c = blockIdx.x % COLS, unit_in_seq = (int)(blockIdx.x / COLS) % per_seq, kvh = unit_in_seq / a.col_blocks, cc = unit_in_seq % a.col_blocks * COLS + c;
+    if (cc >= n_cols) return;
+    uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + row_of(cc) * p.ld_out + (kvh * group + cc % group) * HD);
     if (held < 0) {
-      for (int e = tid; e < here * (HD / 2); e += JOIN_THREADS) *place(e / (HD / 2), 2 * (e % (HD / 2))) = 0u;
+      if (tid < LANES) out[tid] = 0u;
       return;
     }
-    for (int e = tid; e < here * (HD / 2); e += JOIN_THREADS) {
-      const int c = e / (HD / 2), d = 2 * (e % (HD / 2));
-      int first, last, bad = 0x7fffffff;
-      const float2 ml = find(unit_in_seq, c, first, last);
-      if (first == last) return;
-      float x = 0.f, y = 0.f;
-      for (int b = first; b <= last; ++b) {
-        const size_t slot = (size_t)b * 2 + (b == first);
-        const float m1 = a.part_ml[slot * COLS + c].x, k = m1 == -INFINITY ? 1.f : ex2(m1 - ml.x);
-        const float2 v = *reinterpret_cast<const float2*>(&a.parts[(slot * COLS + c) * HD + d]);
-        x += v.x * k;
-        y += v.y * k;
-        bad = min(bad, a.part_bad[slot * 4 + d * NB / HD]);
-      }
-      const int limit = (int)min((long long)held + (c0 + c) / group + 1, (long long)min(p.c.ctx, p.max_len));
-      const float rl = bad < limit ? __int_as_float(0x7fffffff) : 1.f / ml.y;
-      *place(c, d) = pack2<T>(x * rl, y * rl);
+    const int2 ctas = ctas_of(unit_in_seq);
+    if (ctas.x == ctas.y) return;
+    float top = -INFINITY, l = 0.f;
+    for (int b = ctas.x + tid; b <= ctas.y; b += JOIN_THREADS) {
+      s_k[b - ctas.x] = part_of(b, ctas.x, c).x;
+      top = fmaxf(top, s_k[b - ctas.x]);
     }
+    top = warp_max(top);
+    if (lane == 0) s_warp[tid >> 5] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_warp[0], s_warp[1]), fmaxf(s_warp[2], s_warp[3]));
+    for (int b = ctas.x + tid; b <= ctas.y; b += JOIN_THREADS) s_k[b - ctas.x] = s_k[b - ctas.x] == -INFINITY ? 1.f : ex2(s_k[b - ctas.x] - top);  // (a maximum of nothing: sums of 0, or of NaN)
+    __syncthreads();
+    const int pair = tid % LANES, of = tid / LANES;
+    float x = 0.f, y = 0.f;
+    int bad = 0x7fffffff;
+#pragma unroll 4
+    for (int b = ctas.x + of; b <= ctas.y; b += GROUPS) {
+      const size_t slot = (size_t)b * 2 + (b == ctas.x);
+      const float k = s_k[b - ctas.x];
+      const float2 v = *reinterpret_cast<const float2*>(&a.parts[(slot * COLS + c) * HD + 2 * pair]);
+      l += a.part_ml[slot * COLS + c].y * k;
+      x += v.x * k;
+      y += v.y * k;
+      bad = min(bad, a.part_bad[slot * 4 + 2 * pair * NB / HD]);
+    }
+    s_part[of][pair] = make_float2(x, y);
+    __shared__ float s_l[GROUPS];
+    __shared__ int s_bad[4];
+    if (tid < 4) s_bad[tid] = 0x7fffffff;
+    if (pair == 0) s_l[of] = l;
+    __syncthreads();
+    if (bad != 0x7fffffff) atomicMin(&s_bad[2 * pair * NB / HD], bad);
+    __syncthreads();
+    if (tid >= LANES) return;
+    x = y = l = 0.f;
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      x += s_part[k][pair].x;
+      y += s_part[k][pair].y;
+      l += s_l[k];
+    }
+    const int bound = min(p.c.ctx, p.max_len), limit = held >= bound ? bound : min(held + cc / group + 1, bound);
+    const float rl = s_bad[2 * pair * NB / HD] < limit ? __int_as_float(0x7fffffff) : 1.f / l;
+    out[pair] = pack2<T>(x * rl, y * rl);
     return;
   }
   // ---- weights
   __shared__ float2 s_fin[64];
-  const int kvh = sh % p.c.n_kv, j0 = (((int)blockIdx.x - units) % key_blocks) * JOIN_KEYS, bound = min(p.c.ctx, p.max_len);
-  const int T_all = (int)min((long long)held + p.m, (long long)bound);
+  const int kvh = sh % p.c.n_kv, j0 = (((int)blockIdx.x - joins) % key_blocks) * JOIN_KEYS, bound = min(p.c.ctx, p.max_len);
+  const int T_all = held >= bound ? bound : min(held + p.m, bound);
   if (j0 >= T_all) return;
   float w[JOIN_KEYS / JOIN_THREADS] = {};
   for (int c64 = 0; c64 < n_cols; c64 += 64) {
     __syncthreads();
-    if (tid < 64 && c64 + tid < n_cols) {
-      const int c = c64 + tid;
-      int first, last;
-      const float2 ml = find(kvh * a.col_blocks + c / COLS, c % COLS, first, last);
-      s_fin[tid] = make_float2(ml.x, 1.f / ml.y);
+    for (int c = c64 + (tid >> 5); c < min(n_cols, c64 + 64); c += JOIN_THREADS / 32) {  // a column per warp
+      const int unit_in_seq = kvh * a.col_blocks + c / COLS;
+      const int2 ctas = ctas_of(unit_in_seq);
+      float2 all;
+      if (ctas.x == ctas.y) {
+        all = a.unit_ml[((size_t)seq * per_seq + unit_in_seq) * COLS + c % COLS];
+      } else {
+        all = make_float2(-INFINITY, 0.f);
+        for (int b = ctas.x + lane; b <= ctas.y; b += 32) all.x = fmaxf(all.x, part_of(b, ctas.x, c % COLS).x);
+        all.x = warp_max(all.x);
+        for (int b = ctas.x + lane; b <= ctas.y; b += 32) {
+          const float2 ml = part_of(b, ctas.x, c % COLS);
+          all.y += ml.y * (ml.x == -INFINITY ? 1.f : ex2(ml.x - all.x));
+        }
+        all.y = warp_sum(all.y);
+      }
+      if (lane == 0) s_fin[c - c64] = make_float2(all.x, 1.f / all.y);
     }
     __syncthreads();
     for (int c = c64; c < min(n_cols, c64 + 64); ++c) {
       const float* scores = a.scores + (row_of(c) * p.n_heads + kvh * group + c % group) * p.max_len;
-      const int limit = (int)min((long long)held + c / group + 1, (long long)bound);
+      const int limit = held >= bound ? bound : min(held + c / group + 1, bound);
       const float2 fin = s_fin[c - c64];
 #pragma unroll
       for (int i = 0; i < JOIN_KEYS / JOIN_THREADS; ++i) {
@@ -642,7 +692,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step
   }
 }
 
-// the work as the host knows it: units, and CTAs that find a chunk for each of their warps if sequences are as long as they may be
+// the work as the host knows it: units, and CTAs - one per unit, or as many as find a chunk for each of their warps if sequences are as
+// long as they may be, up to two per SM (one with 16 columns, whose accumulators take the registers)
 struct step_shape {
   int cols, col_blocks, ctas;
   long long units;
@@ -652,7 +703,7 @@ struct step_shape {
     col_blocks = (n_cols + cols - 1) / cols;
     units = (long long)n_seqs * n_kv * col_blocks;
     const long long chunks = units * ((max_len + ST_CHUNK - 1) / ST_CHUNK);
-    ctas = (int)std::max(1ll, std::min((long long)ST_CTAS / (cols / 8), (chunks + ST_WARPS - 1) / ST_WARPS));
+    ctas = (int)std::min((long long)ST_CTAS / (cols / 8), std::max(units, (chunks + ST_WARPS - 1) / ST_WARPS));
   }
 };
 
@@ -669,8 +720,8 @@ int launch_step(const step_args& a, cudaStream_t stream) {
     if (dev < 16) attr_done[dev] = true;
   }
   kernel<<<a.ctas, ST_THREADS, SMEM, stream>>>(a);
-  const long long units = (long long)a.p.c.n_seqs * a.p.c.n_kv * a.col_blocks;
-  const long long blocks = units + (WEIGHTS ? (long long)a.p.c.n_seqs * a.p.c.n_kv * ((a.p.max_len + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
+  const long long joins = (long long)a.p.c.n_seqs * a.p.c.n_kv * a.col_blocks * 8 * NT;
+  const long long blocks = joins + (WEIGHTS ? (long long)a.p.c.n_seqs * a.p.c.n_kv * ((a.p.max_len + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
   LCU_CUDA(launch_after(attention_join_kernel<T, HD, NB, NT>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, stream, a));
   return LCU_OK;
 }
