@@ -4,12 +4,14 @@
 
 namespace lcu {
 
-// rows that go to the kernel of few rows
-static bool few_rows(int m, int group) { return (long long)m * group <= 16 || m == 1; }
+// Up to 64 (row, query head) pairs per key/value head go to the kernel that walks the codes, 16 of them a time: one sequence, 8 key heads x 4
+// queries each, 8 rows behind 8000 / 30000: 18 / 35 us against 45 / 82 on tcgen05, 16 rows 27 / 58 against 45 / 82; 48 rows of 32 heads
+// behind 30000: 140 against 228.  A single row always does, however many heads share a key.
+static bool few_rows(int m, int group) { return (long long)m * group <= 64 || m == 1; }
 
 size_t cache4_attention_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
   if (few_rows(m, n_heads / n_kv)) return attention_cache4_step_workspace(n_seqs, m, n_heads, n_kv, hd, max_len, weights);
-  return attention_cache4_prompt_workspace(n_seqs, m, n_heads, n_kv, hd, max_len);
+  return attention_cache4_prompt_workspace(n_seqs, m, n_heads, n_kv, hd, max_len, weights);
 }
 
 int launch_attention_cache4(const cache4_attention_params& p, int dtype, void* workspace, size_t workspace_bytes, cudaStream_t stream) {

@@ -36,6 +36,12 @@ struct prompt_args {
   float2* row_stats;  // [units][r_pad] factor of a row's scores (powers of two); logarithm of its sum (weights; infinity: no such row)
   int* bad;           // [units][t_pad / 128][4] first row of each 128 whose values of a block are no numbers
   int t_pad, r_pad;
+  int ctas;           // split: CTAs that share the tiles of all items (0: a CTA per item)
+  int* prefix;        // split: [units * row blocks + 1] tiles of the items before each
+  float* part_o;      // split: [ctas][2][128][hd] sums of runs of tiles that begin, or end, inside an item
+  float2* part_ml;    // split: [ctas][2][128] their rows' maxima (powers of two) and sums
+  float* part_w;      // weights of runs of rows: [segments][units][t_pad]
+  int segments;
   int* err;
 };
 
@@ -48,6 +54,12 @@ __device__ __forceinline__ int limit_of(const cache4_attention_params& p, int he
   return held < 0 ? 0 : held >= room ? room : min(held + i + 1, room);
 }
 
+// An item is 128 rows of a unit; its tiles are the 128 cached rows each that its last row sees.
+__device__ __forceinline__ int tiles_of(const cache4_attention_params& p, int held, int block) {
+  const int group = p.n_heads / p.c.n_kv, last = min((block + 1) * PR_ROWS, p.m * group) - 1;
+  return (limit_of(p, held, last / group) + PR_KEYS - 1) / PR_KEYS;
+}
+
 // ------------------------------------------------------------------ expansion
 // One CTA per 128 rows of a unit's keys and values, or of its queries.
 template <typename T, int HD>
@@ -55,9 +67,35 @@ __global__ void __launch_bounds__(256) prompt_expand_kernel(const prompt_args a,
   const cache4_attention_params& p = a.p;
   __shared__ int s_bad[4];
   constexpr int WORDS = HD / 8, G = HD / 32;
+  pdl_launch_dependents();
+  if (a.ctas && blockIdx.x == gridDim.x - 1) {  // (the last CTA: where the items' tiles lie in the row of all tiles)
+    __shared__ int s_sum[8];
+    int carry = 0;
+    const int items = p.c.n_seqs * p.c.n_kv * row_blocks;
+    for (int i0 = 0; i0 < items; i0 += 256) {
+      const int i = i0 + threadIdx.x, unit = i / row_blocks;
+      const int n = i < items ? tiles_of(p, p.lengths[unit / p.c.n_kv], i - unit * row_blocks) : 0;
+      int x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if ((threadIdx.x & 31) >= o) x += y;
+      }
+      if ((threadIdx.x & 31) == 31) s_sum[threadIdx.x >> 5] = x;
+      __syncthreads();
+      int before = carry;
+      for (int w = 0; w < 8; ++w) {
+        if (w < (int)(threadIdx.x >> 5)) before += s_sum[w];
+        carry += s_sum[w];
+      }
+      __syncthreads();
+      if (i < items) a.prefix[i] = before + x - n;
+    }
+    if (threadIdx.x == 0) a.prefix[items] = carry;
+    return;
+  }
   const int unit = blockIdx.x / (key_blocks + row_blocks), b = blockIdx.x % (key_blocks + row_blocks), seq = unit / p.c.n_kv, kvh = unit % p.c.n_kv;
   const int held = p.lengths[seq], seen = rows_of(p, held);
-  pdl_launch_dependents();
   if (b < key_blocks) {
     if (b * PR_KEYS >= seen) return;
     if (threadIdx.x < 4) s_bad[threadIdx.x] = 0x7fffffff;
@@ -143,6 +181,14 @@ __device__ __forceinline__ void st_32x32(uint32_t taddr, const uint32_t* r) {
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
@@ -168,7 +214,7 @@ struct prompt_shape {
 constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + 4, B_S = B_EMPTY + 4, B_P = B_S + 1, B_O = B_P + 1, B_COUNT = B_O + 1;
 
 // ------------------------------------------------------------------ outputs
-template <typename T, int HD>
+template <typename T, int HD, bool SPLIT>
 __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                          const __grid_constant__ CUtensorMap map_v, const prompt_args a, int row_blocks, int units) {
   using sh = prompt_shape<HD>;
@@ -186,9 +232,9 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
   __shared__ float s_half[2][PR_ROWS];
   const cache4_attention_params& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // the last rows, which see most, first; all units' side by side
-  const int block = row_blocks - 1 - (int)blockIdx.x / units, unit = (int)blockIdx.x % units, seq = unit / p.c.n_kv, kvh = unit % p.c.n_kv;
-  const int group = p.n_heads / p.c.n_kv, rows = p.m * group, r0 = block * PR_ROWS;
+  const int group = p.n_heads / p.c.n_kv, rows = p.m * group;
+  __shared__ int s_first, s_gave_up;
+  volatile int* gave_up = &s_gave_up;
 
   if (tid == 0) {
     mbar_init(smem_u32(&bars[B_Q]), 1);
@@ -200,9 +246,9 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
     mbar_init(smem_u32(&bars[B_P]), PR_SOFT_WARPS);
     mbar_init(smem_u32(&bars[B_O]), 1);
     *failed = 0;
+    *gave_up = 0;
     fence_mbar_init();
   }
-  if (tid < 4) s_bad[tid] = 0x7fffffff;
   if (warp == PR_SOFT_WARPS + 1) tmem_alloc(tmem_slot, TMEM_COLS);
   tc_fence_before();
   __syncthreads();
@@ -211,66 +257,131 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
   pdl_launch_dependents();
   pdl_wait();
   constexpr bool HEED = false;  // (an earlier launch's error says nothing about this one)
-  const int held = p.lengths[seq];
-  const int n_tiles = (limit_of(p, held, min(r0 + PR_ROWS, rows) / group - (min(r0 + PR_ROWS, rows) % group == 0)) + PR_KEYS - 1) / PR_KEYS;
+  // This CTA's tiles: those of its item - the last rows, which see most, first; all units' side by side - or an equal share of all.
+  int lo = 0, hi = 0x7fffffff, item0 = (row_blocks - 1 - (int)blockIdx.x / units) + (int)blockIdx.x % units * row_blocks;
+  if constexpr (SPLIT) {
+    const int items = units * row_blocks, total = a.prefix[items];
+    const int ctas = min(a.ctas, total);  // (that have a tile at least)
+    lo = hi = total;
+    if ((int)blockIdx.x < ctas) {
+      lo = (int)((long long)total * blockIdx.x / ctas);
+      hi = (int)((long long)total * (blockIdx.x + 1) / ctas);
+    }
+    if (warp == 0) {  // the item that tile `lo` belongs to: the last whose tiles begin at or before it
+      int from = 0, to = items;  // (prefix[from] <= lo < prefix[to])
+      while (to - from > 1) {
+        const int step = (to - from + 32) / 33, i = from + step * (lane + 1);
+        const unsigned m = __ballot_sync(0xffffffffu, i < to && a.prefix[min(i, items)] <= lo);
+        const int k = __popc(m);
+        to = min(to, from + step * (k + 1));
+        from += step * k;
+      }
+      if (lane == 0) s_first = from;
+    }
+    __syncthreads();
+    item0 = s_first;
+  }
+  struct run {
+    int item, first, last, all;  // tiles [first, last) of an item's `all`
+    int seq, kvh, unit, r0, held;
+  };
+  int pos = lo;
+  auto next_run = [&](run& w, int& item) {  // (the same for all roles)
+    for (; !SPLIT || pos < hi; ++item) {
+      w.item = item;
+      w.unit = item / row_blocks;
+      w.seq = w.unit / p.c.n_kv;
+      w.kvh = w.unit - w.seq * p.c.n_kv;
+      w.r0 = (item - w.unit * row_blocks) * PR_ROWS;
+      w.held = p.lengths[w.seq];
+      w.all = tiles_of(p, w.held, w.r0 / PR_ROWS);
+      w.first = 0;
+      w.last = w.all;
+      if constexpr (!SPLIT) return true;
+      const int begin = a.prefix[item];
+      w.first = pos - begin;
+      w.last = min(w.all, hi - begin);
+      if (w.last > w.first) {
+        pos = begin + w.last;
+        ++item;
+        return true;
+      }
+    }
+    return false;
+  };
 
   if (warp == PR_SOFT_WARPS) {
-    if (n_tiles && tc_elect()) {  // ---- loads: queries; K_0, V_0, K_1, V_1, ..
-      mbar_arrive_expect_tx(smem_u32(&bars[B_Q]), OPERAND);
-      for (int kb = 0; kb < NKB; ++kb) tma_load_3d(q_addr + kb * sh::BLOCK, &map_q, kb * 64, r0, unit, smem_u32(&bars[B_Q]));
+    if (tc_elect()) {  // ---- loads: a run's queries; K, V, K, V, ..
       tc_ring r;
-      for (int it = 0; it < 2 * n_tiles; ++it, r.step(RING)) {
-        if (!mbar_wait(smem_u32(&bars[B_EMPTY + r.slot]), r.phase ^ 1u, a.err, DEV_ERR_EMPTY_WAIT, HEED)) break;
-        const uint32_t full = smem_u32(&bars[B_FULL + r.slot]), dst = ring_addr + (uint32_t)r.slot * OPERAND;
-        const int j0 = (it >> 1) * PR_KEYS;
-        mbar_arrive_expect_tx(full, OPERAND);
-        if (!(it & 1)) {
-          for (int kb = 0; kb < NKB; ++kb) tma_load_3d(dst + kb * sh::BLOCK, &map_k, kb * 64, j0, unit, full);
-        } else {
-          for (int kb2 = 0; kb2 < 2; ++kb2)
-            for (int c = 0; c < NKB; ++c) tma_load_3d(dst + (kb2 * NKB + c) * V_ATOM, &map_v, c * 64, j0 + kb2 * 64, unit, full);
+      run w;
+      bool ok = true;
+      for (int item = item0, n = 0; ok && (SPLIT || n == 0) && next_run(w, item); ++n) {
+        if (w.all == 0) break;
+        if (n) ok = mbar_wait(smem_u32(&bars[B_O]), (uint32_t)(n - 1) & 1u, a.err, DEV_ERR_EMPTY_WAIT, HEED);  // (the queries' last product is done)
+        if (!ok) break;
+        mbar_arrive_expect_tx(smem_u32(&bars[B_Q]), OPERAND);
+        for (int kb = 0; kb < NKB; ++kb) tma_load_3d(q_addr + kb * sh::BLOCK, &map_q, kb * 64, w.r0, w.unit, smem_u32(&bars[B_Q]));
+        for (int it = 2 * w.first; it < 2 * w.last; ++it, r.step(RING)) {
+          ok = mbar_wait(smem_u32(&bars[B_EMPTY + r.slot]), r.phase ^ 1u, a.err, DEV_ERR_EMPTY_WAIT, HEED);
+          if (!ok) break;
+          const uint32_t full = smem_u32(&bars[B_FULL + r.slot]), dst = ring_addr + (uint32_t)r.slot * OPERAND;
+          const int j0 = (it >> 1) * PR_KEYS;
+          mbar_arrive_expect_tx(full, OPERAND);
+          if (!(it & 1)) {
+            for (int kb = 0; kb < NKB; ++kb) tma_load_3d(dst + kb * sh::BLOCK, &map_k, kb * 64, j0, w.unit, full);
+          } else {
+            for (int kb2 = 0; kb2 < 2; ++kb2)
+              for (int c = 0; c < NKB; ++c) tma_load_3d(dst + (kb2 * NKB + c) * V_ATOM, &map_v, c * 64, j0 + kb2 * 64, w.unit, full);
+          }
         }
       }
     }
     __syncwarp();
   } else if (warp == PR_SOFT_WARPS + 1) {
     // ---- products, in this order: S_0, O += P_0 V_0, S_1, ..: scores only replace probabilities that have been read
-    bool ok = n_tiles > 0 && mbar_wait_warp(smem_u32(&bars[B_Q]), 0, a.err, DEV_ERR_FULL_WAIT, HEED);
     tc_ring r;
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      ok = mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
-      if (!ok) break;
-      tc_fence_after();
-      if (tc_elect()) {
+    run w;
+    bool ok = true;
+    int count = 0;
+    for (int item = item0, n = 0; ok && (SPLIT || n == 0) && next_run(w, item); ++n) {
+      if (w.all == 0) break;
+      ok = mbar_wait_warp(smem_u32(&bars[B_Q]), (uint32_t)n & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
+      for (int j = w.first; j < w.last && ok; ++j, ++count) {
+        ok = mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
+        if (!ok) break;
+        tc_fence_after();
+        if (tc_elect()) {
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-          const uint64_t a_desc = smem_desc_sw128(q_addr + kb * sh::BLOCK), b_desc = smem_desc_sw128(ring_addr + (uint32_t)r.slot * OPERAND + kb * sh::BLOCK);
+          for (int kb = 0; kb < NKB; ++kb) {
+            const uint64_t a_desc = smem_desc_sw128(q_addr + kb * sh::BLOCK), b_desc = smem_desc_sw128(ring_addr + (uint32_t)r.slot * OPERAND + kb * sh::BLOCK);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, a_desc + 2 * k, b_desc + 2 * k, sh::IDESC_S, (kb | k) != 0);
+            for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, a_desc + 2 * k, b_desc + 2 * k, sh::IDESC_S, (kb | k) != 0);
+          }
+          tc_commit(smem_u32(&bars[B_EMPTY + r.slot]));
+          tc_commit(smem_u32(&bars[B_S]));
         }
-        tc_commit(smem_u32(&bars[B_EMPTY + r.slot]));
-        tc_commit(smem_u32(&bars[B_S]));
-      }
-      __syncwarp();
-      r.step(RING);
-      ok = mbar_wait_warp(smem_u32(&bars[B_P]), (uint32_t)j & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
-      ok = ok && mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
-      if (!ok) break;
-      tc_fence_after();
-      if (tc_elect()) {
+        __syncwarp();
+        r.step(RING);
+        ok = mbar_wait_warp(smem_u32(&bars[B_P]), (uint32_t)count & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
+        ok = ok && mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
+        if (!ok) break;
+        tc_fence_after();
+        if (tc_elect()) {
 #pragma unroll
-        for (int kb2 = 0; kb2 < 2; ++kb2) {
-          const uint64_t b_desc = smem_desc_sw128_mn(ring_addr + (uint32_t)r.slot * OPERAND + kb2 * NKB * V_ATOM, V_ATOM);
+          for (int kb2 = 0; kb2 < 2; ++kb2) {
+            const uint64_t b_desc = smem_desc_sw128_mn(ring_addr + (uint32_t)r.slot * OPERAND + kb2 * NKB * V_ATOM, V_ATOM);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ts(tmem + O_COL, tmem + kb2 * 32 + k * 8, b_desc + (uint64_t)(k * 2048 >> 4), sh::IDESC_PV, (j | kb2 | k) != 0);
+            for (int k = 0; k < 4; ++k)
+              mma_ts(tmem + O_COL, tmem + kb2 * 32 + k * 8, b_desc + (uint64_t)(k * 2048 >> 4), sh::IDESC_PV, (uint32_t)(j > w.first || (kb2 | k) != 0));
+          }
+          tc_commit(smem_u32(&bars[B_EMPTY + r.slot]));
+          if (j + 1 == w.last) tc_commit(smem_u32(&bars[B_O]));
         }
-        tc_commit(smem_u32(&bars[B_EMPTY + r.slot]));
-        if (j + 1 == n_tiles) tc_commit(smem_u32(&bars[B_O]));
+        __syncwarp();
+        r.step(RING);
       }
-      __syncwarp();
-      r.step(RING);
     }
-    if (!ok && n_tiles) {  // (lets the softmax warps leave, without results)
+    if (!ok) {  // (lets the softmax warps leave, without results)
       if (tc_elect()) {
         *failed = 1;
         __threadfence_block();
@@ -282,25 +393,31 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
   } else {
     // ---- softmax: a thread owns half the keys of a row, its warp and the one four further on 32 rows
     const int quad = warp & 3, half = warp >> 2, in_tile = quad * 32 + lane;
-    const int r = r0 + in_tile, i = r / group, limit = r < rows ? limit_of(p, held, i) : 0;
-    const int warp_limit = __shfl_sync(0xffffffffu, limit, 0);  // (what the warp's first row sees)
-    const bool all_there = __all_sync(0xffffffffu, r < rows);
     const uint32_t s_at = tmem + ((uint32_t)(quad * 32) << 16), o_at = s_at + O_COL + (uint32_t)(half * (HD / 2));
-    const float f = a.row_stats[(size_t)unit * a.r_pad + r].x;
     auto meet = [&]() { bar_sync(2 + quad, 64); };
-    // the first row of no numbers among those this CTA sees
-    if (n_tiles) {
+    bool go = true;
+    int count = 0;
+    run w;
+    for (int item = item0, n = 0; go && (SPLIT || n == 0) && next_run(w, item); ++n) {
+    const int r = w.r0 + in_tile, i = r / group, limit = r < rows ? limit_of(p, w.held, i) : 0;
+    const int warp_limit = __shfl_sync(0xffffffffu, limit, 0);  // (what the warp's first row sees)
+    const bool all_there = __all_sync(0xffffffffu, r < rows), whole = !SPLIT || w.last - w.first == w.all;
+    const float f = a.row_stats[(size_t)w.unit * a.r_pad + r].x;
+    if (n) bar_sync(1, 32 * PR_SOFT_WARPS);  // (the run before has read s_half and s_bad)
+    if (tid < 4) s_bad[tid] = 0x7fffffff;
+    bar_sync(1, 32 * PR_SOFT_WARPS);
+    // the first row of no numbers among those this item sees
+    if (whole) {
       const int nb = HD / p.c.bs;
-      const int* list = a.bad + (size_t)unit * (a.t_pad / PR_KEYS) * 4;
-      for (int e = tid; e < n_tiles * nb; e += 32 * PR_SOFT_WARPS) {
+      const int* list = a.bad + (size_t)w.unit * (a.t_pad / PR_KEYS) * 4;
+      for (int e = tid; e < w.all * nb; e += 32 * PR_SOFT_WARPS) {
         const int v = list[(e / nb) * 4 + e % nb];
         if (v != 0x7fffffff) atomicMin(&s_bad[e % nb], v);
       }
     }
     float less = 0.f, high = -INFINITY, sum = 0.f;  // minus the maximum (0 while there is none); 8 above it, as the products give scores
-    bool go = true;
-    for (int j = 0; j < n_tiles; ++j) {
-      const bool ok = mbar_wait(smem_u32(&bars[B_S]), (uint32_t)j & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
+    for (int j = w.first; j < w.last; ++j, ++count) {
+      const bool ok = mbar_wait(smem_u32(&bars[B_S]), (uint32_t)count & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
       tc_fence_after();
       go = __all_sync(0xffffffffu, ok && *failed == 0);
       const int left = limit - j * PR_KEYS - half * 64;  // keys of the half tile that the row sees
@@ -311,25 +428,25 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         top = -INFINITY;
         part = 0.f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s[32];
-          tc_ld_32x32(s_at + (uint32_t)(half * 64 + c * 32), s);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t s[16];
+          ld_32x16(s_at + (uint32_t)(half * 64 + c * 16), s);
           tc_wait_ld();
           if (ragged) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c * 32 + e >= left) s[e] = 0xff800000u;
+            for (int e = 0; e < 16; ++e)
+              if (c * 16 + e >= left) s[e] = 0xff800000u;
           }
           float t0 = -INFINITY, t1 = -INFINITY, a0 = 0.f, a1 = 0.f;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
+          for (int e = 0; e < 16; e += 2) {
             const float s0 = __uint_as_float(s[e]), s1 = __uint_as_float(s[e + 1]);
             t0 = fmaxf(t0, s0);
             t1 = fmaxf(t1, s1);
             const float e0 = ex2(fmaf(s0, f, less)), e1 = ex2(fmaf(s1, f, less));
             a0 += e0;
             a1 += e1;
-            pw[c * 16 + e / 2] = pack2<__half>(e0, e1);
+            pw[c * 8 + e / 2] = pack2<__half>(e0, e1);
           }
           top = fmaxf(top, fmaxf(t0, t1));
           part += a0 + a1;
@@ -337,9 +454,9 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
       };
       tile();
       const int mine = (__any_sync(0xffffffffu, top > high) ? 1 : 0) | (go ? 0 : 2);
-      if (lane == 0) s_raise[j & 1][warp] = mine;
+      if (lane == 0) s_raise[count & 1][warp] = mine;
       meet();  // (both halves of the rows' scores are read: probabilities may take their place)
-      const int either = mine | s_raise[j & 1][warp ^ 4];
+      const int either = mine | s_raise[count & 1][warp ^ 4];
       if (either & 2) {  // (the pair leaves together: its barriers count both)
         go = false;
         break;
@@ -355,7 +472,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         less = now == -INFINITY ? 0.f : -now;
         high = (now + 8.f) / f;
         sum *= k;
-        if (j) {
+        if (j > w.first) {
 #pragma unroll 1
           for (int c = 0; c < HD / 2; c += 32) {
             uint32_t x[32];
@@ -379,18 +496,25 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
     s_half[half][in_tile] = sum;
     bar_sync(1, 32 * PR_SOFT_WARPS);  // (sums, s_bad)
     sum = s_half[0][in_tile] + s_half[1][in_tile];
-    if (n_tiles) {
-      const bool ok = mbar_wait(smem_u32(&bars[B_O]), 0, a.err, DEV_ERR_TMEM_WAIT, HEED);
+    if (w.all) {
+      const bool ok = go && mbar_wait(smem_u32(&bars[B_O]), (uint32_t)n & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
       tc_fence_after();
-      go = __all_sync(0xffffffffu, go && ok && *failed == 0);
+      go = __all_sync(0xffffffffu, ok && *failed == 0);
     }
-    if (go) {
+    // (all eight warps go on together, or none: the barriers of the next run count them)
+    if constexpr (SPLIT) {
+      if (!go && lane == 0) *gave_up = 1;
+      bar_sync(1, 32 * PR_SOFT_WARPS);
+      if (*gave_up) go = false;
+    }
+    if (!go) break;
+    if (whole) {
       const float rl = limit ? 1.f / sum : 0.f;
-      T* out = reinterpret_cast<T*>(p.out) + ((size_t)seq * p.m + i) * p.ld_out + (kvh * group + r % group) * HD + half * (HD / 2);
+      T* out = reinterpret_cast<T*>(p.out) + ((size_t)w.seq * p.m + i) * p.ld_out + (w.kvh * group + r % group) * HD + half * (HD / 2);
 #pragma unroll 1
       for (int c = 0; c < HD / 2; c += 32) {
         uint32_t x[32];
-        if (n_tiles) {
+        if (w.all) {
           tc_ld_32x32(o_at + (uint32_t)c, x);
           tc_wait_ld();
         }
@@ -405,7 +529,21 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
           }
         }
       }
-      if (p.weights && r < rows && half == 0) a.row_stats[(size_t)unit * a.r_pad + r].y = limit ? log2f(sum) - less : INFINITY;
+      if (p.weights && r < rows && half == 0) a.row_stats[(size_t)w.unit * a.r_pad + r].y = limit ? log2f(sum) - less : INFINITY;
+    } else {
+      const size_t place = ((size_t)blockIdx.x * 2 + (w.first == 0)) * PR_ROWS + in_tile;
+      float* to = a.part_o + place * HD + half * (HD / 2);
+#pragma unroll 1
+      for (int c = 0; c < HD / 2; c += 32) {
+        uint32_t x[32];
+        tc_ld_32x32(o_at + (uint32_t)c, x);
+        tc_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) reinterpret_cast<uint4*>(to + c)[q] = make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+      }
+      if (half == 0) a.part_ml[place] = make_float2(high == -INFINITY ? -INFINITY : -less, sum);
+    }
+    tc_fence_before();  // (the accumulator is read: the next run's products come behind this thread's arrival)
     }
   }
   tc_fence_before();
@@ -417,7 +555,84 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
   }
 }
 
+// Joins the runs of items that several CTAs did, and gives zeros for sequences not in use: a warp per row, 16 CTAs per item.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const prompt_args a, int row_blocks) {
+  const cache4_attention_params& p = a.p;
+  __shared__ int s_bad[4];
+  const int item = blockIdx.x / 16, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int unit = item / row_blocks, seq = unit / p.c.n_kv, kvh = unit - seq * p.c.n_kv, block = item - unit * row_blocks;
+  const int group = p.n_heads / p.c.n_kv, in_tile = blockIdx.x % 16 * 8 + warp, r = block * PR_ROWS + in_tile, i = r / group;
+  const bool there = r < p.m * group;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int held = p.lengths[seq], items = p.c.n_seqs * p.c.n_kv * row_blocks;
+  const int begin = a.prefix[item], end = a.prefix[item + 1], total = a.prefix[items];
+  T* out = reinterpret_cast<T*>(p.out) + ((size_t)seq * p.m + i) * p.ld_out + (kvh * group + r % group) * HD;
+  constexpr int EACH = HD / 32;
+  if (begin == end) {
+    if (there)
+      for (int e = 0; e < EACH; e += 2) reinterpret_cast<uint32_t*>(out)[(lane * EACH + e) / 2] = 0u;
+    return;
+  }
+  // the CTAs of its first and last tile
+  const int ctas = min(a.ctas, total), first = (int)(((long long)(begin + 1) * ctas - 1) / total), last = (int)(((long long)end * ctas - 1) / total);
+  if (first == last) return;
+  if (threadIdx.x < 4) s_bad[threadIdx.x] = 0x7fffffff;
+  __syncthreads();
+  const int nb = HD / p.c.bs;
+  const int* list = a.bad + (size_t)unit * (a.t_pad / PR_KEYS) * 4;
+  for (int e = threadIdx.x; e < (end - begin) * nb; e += 256) {
+    const int v = list[(e / nb) * 4 + e % nb];
+    if (v != 0x7fffffff) atomicMin(&s_bad[e % nb], v);
+  }
+  __syncthreads();
+  if (!there) return;
+  auto place = [&](int cta) { return ((size_t)cta * 2 + (cta == first)) * PR_ROWS + in_tile; };
+  float top = -INFINITY;
+  for (int b = first + lane; b <= last; b += 32) top = fmaxf(top, a.part_ml[place(b)].x);
+  top = warp_max(top);
+  float l = 0.f, x[EACH] = {};
+#pragma unroll 4
+  for (int b = first; b <= last; ++b) {
+    const float2 ml = a.part_ml[place(b)];
+    const float k = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // (a maximum of nothing: sums of 0, or of NaN)
+    l += ml.y * k;
+    const float* from = a.part_o + place(b) * HD + lane * EACH;
+    if constexpr (EACH == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(from);
+      x[0] += v.x * k;
+      x[1] += v.y * k;
+      x[2] += v.z * k;
+      x[3] += v.w * k;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(from);
+      x[0] += v.x * k;
+      x[1] += v.y * k;
+    }
+  }
+  const int limit = limit_of(p, held, i);
+  const float rl = s_bad[lane * EACH / p.c.bs] < limit ? __int_as_float(0x7fffffff) : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < EACH; e += 2) reinterpret_cast<uint32_t*>(out)[(lane * EACH + e) / 2] = pack2<T>(x[e] * rl, x[e + 1] * rl);
+  if (p.weights && lane == 0) a.row_stats[(size_t)unit * a.r_pad + r].y = log2f(l) + top;
+}
+
 // ------------------------------------------------------------------ weights
+__device__ __forceinline__ void store_weight(const cache4_attention_params& p, int unit, int j, int held, float total) {
+  float* to = p.weights + (size_t)unit * p.c.ctx + j;
+  *to = p.beta == 0.f || j >= held ? total : fmaf(p.beta, *to, total);
+}
+__global__ void __launch_bounds__(256) prompt_add_kernel(const prompt_args a, int units) {
+  const int unit = blockIdx.y;
+  pdl_wait();
+  const int held = a.p.lengths[unit / a.p.c.n_kv], seen = rows_of(a.p, held);
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= seen) return;
+  float total = 0.f;
+  for (int s = 0; s < a.segments; ++s) total += a.part_w[((size_t)s * units + unit) * a.t_pad + j];
+  store_weight(a.p, unit, j, held, total);
+}
 // One CTA per (sequence, key/value head, 128 cached rows), two per SM; rows of the call in tiles of 128 through a ring.  Two score
 // accumulators: one tile's exponentials run under the next one's product.
 constexpr int W_KEYS = 0, W_FULL = 1, W_EMPTY = W_FULL + 2, W_S = W_EMPTY + 2, W_FREE = W_S + 2, W_COUNT = W_FREE + 2;
@@ -437,7 +652,8 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
   const cache4_attention_params& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ float s_total[PR_KEYS];
-  const int block = (int)blockIdx.x / units, unit = (int)blockIdx.x % units, seq = unit / p.c.n_kv;
+  const int segment = (int)blockIdx.x % a.segments, at = (int)blockIdx.x / a.segments;
+  const int block = at / units, unit = at % units, seq = unit / p.c.n_kv;
   const int group = p.n_heads / p.c.n_kv, rows = p.m * group, j0 = block * PR_KEYS;
   if (tid == 0) {
     mbar_init(smem_u32(&bars[W_KEYS]), 1);
@@ -458,8 +674,10 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
   pdl_wait();
   constexpr bool HEED = false;
   const int held = p.lengths[seq], seen = rows_of(p, held);
-  // rows from the first that sees the first key on
-  const int first = max(0, j0 - held) * group / PR_ROWS, n_tiles = j0 < seen ? (rows + PR_ROWS - 1) / PR_ROWS - first : 0;
+  // rows from the first that sees the first key on; this CTA's run of their tiles
+  const int from_tile = max(0, j0 - held) * group / PR_ROWS, all_tiles = j0 < seen ? (rows + PR_ROWS - 1) / PR_ROWS - from_tile : 0;
+  const int first = from_tile + (int)((long long)all_tiles * segment / a.segments);
+  const int n_tiles = from_tile + (int)((long long)all_tiles * (segment + 1) / a.segments) - first;
 
   if (warp == PR_SOFT_WARPS) {
     if (n_tiles > 0 && tc_elect()) {
@@ -556,9 +774,11 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
     bar_sync(1, 32 * PR_SOFT_WARPS);
     total += s_total[quad * 32 + lane];
     if (go && j < seen && !half) {
-      float* to = p.weights + (size_t)unit * p.c.ctx + j;
-      *to = p.beta == 0.f || j >= held ? total : fmaf(p.beta, *to, total);
+      if (a.segments > 1) a.part_w[((size_t)segment * units + unit) * a.t_pad + j] = total;
+      else store_weight(p, unit, j, held, total);
     }
+  } else if (a.segments > 1 && j0 < seen && tid < PR_KEYS) {  // (a segment of no rows)
+    a.part_w[((size_t)segment * units + unit) * a.t_pad + j0 + tid] = 0.f;
   }
   tc_fence_before();
   __syncthreads();
@@ -570,19 +790,42 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
 }
 
 // ------------------------------------------------------------------ host
-size_t prompt_layout(prompt_args* a, void* workspace, int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len) {
+// How the work is shared, from the sizes as the host knows them.  A CTA per item leaves slots idle where items are few or their last wave is
+// half full; an equal share of all tiles per CTA costs each the start of another run, the partial sums of two and their join, about what
+// eight tiles take.  8 key heads x 4 queries each: 8 rows behind 30000 (16 tiles of 128 rows at once) 510 us per item, 82 shared; 2000 rows
+// behind 6000 (504 items of 47 to 63 tiles, 296 slots) 414 us per item, 464 shared.
+struct prompt_plan {
+  int ctas, segments;
+  prompt_plan(int n_seqs, int m, int n_heads, int n_kv, int max_len) {
+    const double slots = 2 * 148;
+    const long long units = (long long)n_seqs * n_kv, rows = (long long)m * (n_heads / n_kv), blocks = (rows + PR_ROWS - 1) / PR_ROWS;
+    const long long most = (max_len + PR_KEYS - 1) / PR_KEYS, least = std::max(1ll, (long long)(std::max(0, max_len - m) + PR_KEYS) / PR_KEYS);
+    const double total = (double)units * blocks * (most + least) / 2, share = total / slots;
+    const double items = units * blocks <= slots ? (double)most : share + most / 2.0;
+    ctas = share + 8 < 0.7 * items ? (int)std::min(slots, std::max(1.0, total)) : 0;
+    // weights: rows are dealt to several CTAs per 128 keys where there are fewer of those than slots
+    segments = (int)std::max(1ll, std::min({16ll, blocks, (long long)slots / std::max(1ll, units * most)}));
+  }
+};
+
+size_t prompt_layout(prompt_args* a, void* workspace, int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
   size_t used = 0;
   auto take = [&](size_t bytes) {
     const size_t at = used;
     used += round_up(bytes, 128);
     return (uint8_t*)workspace + at;
   };
+  const prompt_plan plan(n_seqs, m, n_heads, n_kv, max_len);
   const size_t units = (size_t)n_seqs * n_kv, t_pad = round_up(max_len, PR_KEYS), r_pad = round_up((size_t)m * (n_heads / n_kv), PR_ROWS);
   uint8_t* k = take(units * t_pad * hd * 2);
   uint8_t* v = take(units * t_pad * hd * 2);
   uint8_t* q = take(units * r_pad * hd * 2);
   uint8_t* stats = take(units * r_pad * sizeof(float2));
   uint8_t* bad = take(units * (t_pad / PR_KEYS) * 4 * sizeof(int));
+  uint8_t* prefix = take(plan.ctas ? (units * (r_pad / PR_ROWS) + 1) * sizeof(int) : 0);
+  uint8_t* part_o = take((size_t)plan.ctas * 2 * PR_ROWS * hd * sizeof(float));
+  uint8_t* part_ml = take((size_t)plan.ctas * 2 * PR_ROWS * sizeof(float2));
+  uint8_t* part_w = take(weights && plan.segments > 1 ? (size_t)plan.segments * units * t_pad * sizeof(float) : 0);
   if (a) {
     a->k_half = (__half*)k;
     a->v_half = (__half*)v;
@@ -591,6 +834,12 @@ size_t prompt_layout(prompt_args* a, void* workspace, int n_seqs, int m, int n_h
     a->bad = (int*)bad;
     a->t_pad = (int)t_pad;
     a->r_pad = (int)r_pad;
+    a->ctas = plan.ctas;
+    a->prefix = (int*)prefix;
+    a->part_o = (float*)part_o;
+    a->part_ml = (float2*)part_ml;
+    a->part_w = (float*)part_w;
+    a->segments = plan.segments;
   }
   return used;
 }
@@ -621,35 +870,38 @@ int launch_prompt(const prompt_args& a, cudaStream_t stream) {
     if (!rc) rc = tc_encode_map(&map_v, a.v_half, 3, rows_k, step_k, box_v);
     if (rc) return rc;
   }
-  prompt_expand_kernel<T, HD><<<(unsigned)units * (key_blocks + row_blocks), 256, 0, stream>>>(a, key_blocks, row_blocks);
-  static bool done[16] = {}, done_w[16] = {};
-  int rc = allow_smem(prompt_attention_kernel<T, HD>, sh::SMEM, done);
+  prompt_expand_kernel<T, HD><<<(unsigned)units * (key_blocks + row_blocks) + (a.ctas ? 1 : 0), 256, 0, stream>>>(a, key_blocks, row_blocks);
+  static bool done[2][16] = {}, done_w[16] = {};
+  auto* kernel = a.ctas ? prompt_attention_kernel<T, HD, true> : prompt_attention_kernel<T, HD, false>;
+  int rc = allow_smem(kernel, sh::SMEM, done[a.ctas > 0]);
   if (rc) return rc;
-  LCU_CUDA(launch_after(prompt_attention_kernel<T, HD>, dim3((unsigned)units * row_blocks), dim3(PR_THREADS), sh::SMEM, stream, map_q, map_k, map_v, a, row_blocks, units));
+  LCU_CUDA(launch_after(kernel, dim3(a.ctas ? (unsigned)a.ctas : (unsigned)units * row_blocks), dim3(PR_THREADS), sh::SMEM, stream, map_q, map_k, map_v, a, row_blocks, units));
+  if (a.ctas) LCU_CUDA(launch_after(prompt_join_kernel<T, HD>, dim3((unsigned)units * row_blocks * 16), dim3(256), 0, stream, a, row_blocks));
   if (p.weights) {
     constexpr uint32_t SMEM_W = 3 * sh::OPERAND + 4 * 128 * sizeof(float2) + 1024 + 256;
     rc = allow_smem(prompt_weights_kernel<HD>, SMEM_W, done_w);
     if (rc) return rc;
-    LCU_CUDA(launch_after(prompt_weights_kernel<HD>, dim3((unsigned)units * key_blocks), dim3(PR_THREADS), SMEM_W, stream, map_q, map_k, a, key_blocks, units));
+    LCU_CUDA(launch_after(prompt_weights_kernel<HD>, dim3((unsigned)units * key_blocks * a.segments), dim3(PR_THREADS), SMEM_W, stream, map_q, map_k, a, key_blocks, units));
+    if (a.segments > 1) LCU_CUDA(launch_after(prompt_add_kernel, dim3((p.max_len + 255) / 256, (unsigned)units), dim3(256), 0, stream, a, units));
   }
   return LCU_OK;
 }
 
 }  // namespace
 
-size_t attention_cache4_prompt_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len) {
-  return prompt_layout(nullptr, nullptr, n_seqs, m, n_heads, n_kv, hd, max_len);
+size_t attention_cache4_prompt_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
+  return prompt_layout(nullptr, nullptr, n_seqs, m, n_heads, n_kv, hd, max_len, weights);
 }
 
 int launch_attention_cache4_prompt(const cache4_attention_params& p, int dtype, void* workspace, cudaStream_t stream) {
   const long long units = (long long)p.c.n_seqs * p.c.n_kv, rows = (long long)p.m * (p.n_heads / p.c.n_kv);
-  LCU_REQUIRE(rows < (1ll << 30) && units * ((p.max_len + rows) / 128 + 2) < (1ll << 31), "attention_cache4: %d sequences of %d rows of %d heads over %d rows are too many", p.c.n_seqs,
+  LCU_REQUIRE(rows < (1ll << 30) && units * ((p.max_len + rows) / 128 + 2) * 16 < (1ll << 31) && units * (rows / 128 + 1) * (p.max_len / 128 + 1) < (1ll << 31), "attention_cache4: %d sequences of %d rows of %d heads over %d rows are too many", p.c.n_seqs,
               p.m, p.n_heads, p.max_len);
   prompt_args a{};
   a.p = p;
   a.err = device_scratch_words();
   LCU_REQUIRE(a.err != nullptr, "attention_cache4: no error word");
-  prompt_layout(&a, workspace, p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.c.hd, p.max_len);
+  prompt_layout(&a, workspace, p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.c.hd, p.max_len, p.weights != nullptr);
   if (dtype == OP_F16) return p.c.hd == 128 ? launch_prompt<__half, 128>(a, stream) : launch_prompt<__half, 64>(a, stream);
   return p.c.hd == 128 ? launch_prompt<__nv_bfloat16, 128>(a, stream) : launch_prompt<__nv_bfloat16, 64>(a, stream);
 }
