@@ -33,45 +33,23 @@ __device__ __forceinline__ float seven_bits(float s) {
 }
 
 // A CTA takes R rows (four of a prompt's, whose 64-bit angles then keep all its threads busy; a single token's heads are shared by `parts`
-// CTAs).  Bound by memory for prompts, by the launch and the chain load - angle - store for a token.  Angles are formed once per row and
-// CTA, in 64 bits (a position of a hundred thousand leaves seven digits of a binary32 angle's turn).  A thread owns eight neighbouring
-// dimensions at a time: one 16-byte load, the first ones requested ahead of the angles, its four rotation pairs, one word of codes; a block's
-// threads find its maximum by shuffles.
+// CTAs).  Bound by memory for prompts, with the arithmetic of rounding close behind, by the launch and the chain load - angle - store for a token.
+// Angles are formed once per row and CTA, in 64 bits (a position of a hundred thousand leaves seven digits of a binary32 angle's turn).  A
+// thread owns the same eight dimensions of every head it comes to, so it reads a row's four rotations once; its first queries are
+// requested ahead of the angles.  A block's threads find its maximum by shuffles.
 template <typename T, int HD, int R>
 __global__ void __launch_bounds__(256) cache4_append_kernel(const append_args a) {
   const cache4_append_params& p = a.p;
-  constexpr int PER_HEAD = HD / 8;
+  constexpr int PER_HEAD = HD / 8, AHEAD = 2;
   __shared__ float2 turn[R][HD / 2];
-  __shared__ int s_seq[R], s_at[R];  // sequence and place of every row (-1: it is not written)
-  const int rows = p.c.n_seqs * p.m, row0 = (int)(blockIdx.x / a.parts) * R, part = blockIdx.x % a.parts, lane = threadIdx.x & 31;
-  // a row's octets: queries, keys, values, in units of 32 that each lie within one of the three; a warp takes every eighth of the CTA's
+  const int rows = p.c.n_seqs * p.m, row0 = (int)(blockIdx.x / a.parts) * R;
+  const int start = (int)(blockIdx.x % a.parts) * 256 + (int)threadIdx.x, stride = 256 * a.parts, o8 = start % PER_HEAD;  // (stride: whole heads)
   const int n_q = p.q ? p.n_heads * PER_HEAD : 0, n_kv = p.c.n_kv * PER_HEAD;
-  const int q_units = (n_q + 31) / 32, kv_units = (n_kv + 31) / 32, units = q_units + 2 * kv_units, step = 8 * a.parts;
-  struct place {
-    int r, u, o, kind;  // row and unit; octet within the row's queries (0), keys (1), values (2)
-  };
-  auto settle = [&](place& w) {
-    while (w.u >= units) {
-      w.u -= units;
-      ++w.r;
-    }
-    w.kind = w.u < q_units ? 0 : w.u < q_units + kv_units ? 1 : 2;
-    w.o = (w.u - (w.kind == 0 ? 0 : w.kind == 1 ? q_units : q_units + kv_units)) * 32 + lane;
-  };
-  auto load = [&](const place& w) {
-    const int row = row0 + w.r;
-    if (w.r >= R || row >= rows || w.o >= (w.kind ? n_kv : n_q)) return make_uint4(0, 0, 0, 0);
-    const T* from = reinterpret_cast<const T*>(w.kind == 0 ? p.q : w.kind == 1 ? p.k_new : p.v_new) + (size_t)row * (w.kind ? p.ld_kv : p.ld_q);
-    return reinterpret_cast<const uint4*>(from)[w.o];
-  };
-  place now{0, part * 8 + (int)(threadIdx.x >> 5), 0, 0};
-  settle(now);
-  uint4 v = load(now);
-  if (threadIdx.x < R) {
-    const int row = row0 + threadIdx.x, seq = min(row, rows - 1) / p.m, i = row - seq * p.m, held = p.lengths[seq];
-    s_seq[threadIdx.x] = seq;
-    s_at[threadIdx.x] = row < rows && held >= 0 && held < p.c.ctx - i ? held + i : -1;  // (a sequence in use, and room for the row)
-  }
+  auto q_row = [&](int row) { return reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (size_t)row * p.ld_q); };
+  uint4 ahead[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (start + k * stride < n_q) ahead[k] = q_row(row0)[start + k * stride];
   if (p.theta > 0.f) {
     for (int t = threadIdx.x; t < R * (HD / 2); t += 256) {
       const int r = t / (HD / 2), e = t % (HD / 2), row = min(row0 + r, rows - 1), seq = row / p.m;
@@ -86,30 +64,54 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const append_args a)
       sincos(fma(-turns, TWO_PI_LO, fma(-turns, TWO_PI_HI, angle)), &s, &c);
       turn[r][e] = make_float2((float)c, (float)s);
     }
+    __syncthreads();
   }
-  __syncthreads();
-  while (now.r < R && row0 + now.r < rows) {
-    place ahead = now;
-    ahead.u += step;
-    settle(ahead);
-    const uint4 v_ahead = load(ahead);
-    const int o8 = now.o % PER_HEAD, head = now.o / PER_HEAD;
-    const bool there = now.o < (now.kind ? n_kv : n_q);
-    float x[8];
-    unpack8<T>(v, x);
-    if (now.kind < 2 && p.theta > 0.f) {
+#pragma unroll 1
+  for (int r = 0; r < R && row0 + r < rows; ++r) {
+    const int row = row0 + r;
+    float2 cs[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) cs[e] = p.theta > 0.f ? turn[r][o8 * 4 + e] : make_float2(1.f, 0.f);
+    auto rotate = [&](float (&x)[8]) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 cs = turn[now.r][o8 * 4 + e];
         const float re = x[2 * e], im = x[2 * e + 1];
         // (products and sums rounded one by one: the codes of values at a border do not depend on how a compiler fuses them)
-        x[2 * e] = __fsub_rn(__fmul_rn(re, cs.x), __fmul_rn(im, cs.y));
-        x[2 * e + 1] = __fadd_rn(__fmul_rn(re, cs.y), __fmul_rn(im, cs.x));
+        x[2 * e] = __fsub_rn(__fmul_rn(re, cs[e].x), __fmul_rn(im, cs[e].y));
+        x[2 * e + 1] = __fadd_rn(__fmul_rn(re, cs[e].y), __fmul_rn(im, cs[e].x));
+      }
+    };
+    uint4* q_out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.q_out) + (size_t)row * (p.n_heads * HD));
+    for (int o = start; o < n_q; o += AHEAD * stride) {
+      uint4 v[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        v[k] = ahead[k];
+        // the next ones: of this row, or the next row's first
+        const int next = o + (AHEAD + k) * stride;
+        if (next < n_q) ahead[k] = q_row(row)[next];
+        else if (o + AHEAD * stride >= n_q && r + 1 < R && row + 1 < rows && start + k * stride < n_q) ahead[k] = q_row(row + 1)[start + k * stride];
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (o + k * stride >= n_q) break;
+        if (p.theta > 0.f) {
+          float x[8];
+          unpack8<T>(v[k], x);
+          rotate(x);
+          v[k] = pack8<T>(x);
+        }
+        q_out[o + k * stride] = v[k];
       }
     }
-    if (now.kind == 0) {
-      if (there) reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.q_out) + (size_t)(row0 + now.r) * (p.n_heads * HD))[now.o] = p.theta > 0.f ? pack8<T>(x) : v;
-    } else {
+    const int seq = row / p.m, i = row - seq * p.m, held = p.lengths[seq];
+    if (held < 0 || held >= p.c.ctx - i) continue;  // no such sequence, or no room for the row (for all threads alike)
+    for (int o = start; o < ((2 * n_kv + 31) & ~31); o += stride) {
+      const bool there = o < 2 * n_kv, is_v = o >= n_kv;
+      const int ok = there ? (is_v ? o - n_kv : o) : o8;
+      float x[8];
+      unpack8<T>(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(is_v ? p.v_new : p.k_new) + (size_t)row * p.ld_kv)[ok], x);
+      if (!is_v && p.theta > 0.f) rotate(x);
       float most = 0.f;
       bool odd = false;
 #pragma unroll
@@ -122,22 +124,21 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const append_args a)
       const float s7 = seven_bits(__fdiv_rn(most, 7.5f));
       const __half scale = __float2half_rn(s7 > 8704.f ? 8704.f : s7);  // (a NaN stays)
       const float s = __half2float(scale);
-      uint32_t word = 0;
+      uint32_t word = 0x88888888u;
+      if (s > 0.f) {
+        // floor by a sum rounded down (its last bits are the whole number), codes put together by multiplying, less the eight exponents
+        word = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float c = s > 0.f ? fminf(fmaxf(floorf(__fadd_rn(__fdiv_rn(x[e], s), 8.f)), 0.f), 15.f) : 8.f;
-        word |= (uint32_t)c << (4 * e);
+        for (int e = 7; e >= 0; --e) word = word * 16u + __float_as_uint(__fadd_rd(fminf(fmaxf(__fadd_rn(__fdiv_rn(x[e], s), 8.f), 0.f), 15.5f), 8388608.f));
+        word -= 0x4b000000u * 0x11111111u;
       }
-      const int slot = s_at[now.r];
-      if (there && slot >= 0) {
-        const size_t at = ((size_t)s_seq[now.r] * p.c.n_kv + head) * p.c.ctx + slot;
-        uint8_t* codes = (now.kind == 2 ? p.c.v_codes : p.c.k_codes) + at * (HD / 2);
+      if (there) {
+        const size_t at = ((size_t)seq * p.c.n_kv + ok / PER_HEAD) * p.c.ctx + held + i;
+        uint8_t* codes = (is_v ? p.c.v_codes : p.c.k_codes) + at * (HD / 2);
         reinterpret_cast<uint32_t*>(codes)[cache4_word(o8, HD / 32)] = word;
-        if ((o8 * 8) % p.c.bs == 0) ((now.kind == 2 ? p.c.v_scales : p.c.k_scales) + at * (HD / p.c.bs))[o8 * 8 / p.c.bs] = scale;
+        if ((o8 * 8) % p.c.bs == 0) ((is_v ? p.c.v_scales : p.c.k_scales) + at * (HD / p.c.bs))[o8 * 8 / p.c.bs] = scale;
       }
     }
-    now = ahead;
-    v = v_ahead;
   }
 }
 
@@ -202,11 +203,10 @@ int launch_cache4_append(const cache4_append_params& p, int dtype, cudaStream_t 
   append_args a{p, {}, 1};
   if (p.theta > 0.f)
     for (int b = 0; b < 6; ++b) a.powers[b] = exp2(-(double)(2 << b) / p.c.hd * log2((double)p.theta));
-  // four rows per CTA from four waves of CTAs on; a row's units shared by CTAs while there are fewer rows than that
-  const int rows = p.c.n_seqs * p.m, per_head = p.c.hd / 8;
-  const int units = p.q ? (p.n_heads * per_head + 31) / 32 + 2 * ((p.c.n_kv * per_head + 31) / 32) : 2 * ((p.c.n_kv * per_head + 31) / 32);
+  // four rows per CTA from four CTAs per SM on; a row's heads shared by CTAs while there are fewer
+  const int rows = p.c.n_seqs * p.m, octets = std::max(p.q ? p.n_heads : 0, 2 * p.c.n_kv) * (p.c.hd / 8);
   const bool four = rows >= 4 * 148;
-  if (!four) a.parts = std::max(1, std::min((units + 7) / 8, 8 * 148 / rows));
+  if (!four) a.parts = std::max(1, std::min((octets + 255) / 256, 8 * 148 / rows));
   const unsigned ctas = four ? (unsigned)((rows + 3) / 4) : (unsigned)rows * a.parts;
   if (dtype == OP_F16) launch_append<__half>(a, four, ctas, stream);
   else launch_append<__nv_bfloat16>(a, four, ctas, stream);
