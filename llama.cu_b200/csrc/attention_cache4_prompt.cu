@@ -101,29 +101,40 @@ __global__ void __launch_bounds__(256) prompt_expand_kernel(const prompt_args a,
     if (threadIdx.x < 4) s_bad[threadIdx.x] = 0x7fffffff;
     __syncthreads();
     const int nb = HD / p.c.bs;
-    for (int w = threadIdx.x; w < PR_KEYS * WORDS; w += 256) {
-      const int r = w / WORDS, word = w % WORDS, j = b * PR_KEYS + r, d = (word % G) * 32 + (word / G) * 8;
-      uint4 k = make_uint4(0, 0, 0, 0), v = k;
-      if (j < seen) {
-        const size_t at = (size_t)unit * p.c.ctx + j;
-        const uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_codes + at * (HD / 2)) + word), vw = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_codes + at * (HD / 2)) + word);
-        const float ks = __half2float(p.c.k_scales[at * nb + d / p.c.bs]);
-        float vs = __half2float(p.c.v_scales[at * nb + d / p.c.bs]);
-        if (vs != vs) {
-          atomicMin(&s_bad[d / p.c.bs], j);
-          vs = 0.f;
+    constexpr int UNROLL = 4;  // (words requested before the first is used)
+    for (int w0 = threadIdx.x; w0 < PR_KEYS * WORDS; w0 += 256 * UNROLL) {
+      uint32_t kw[UNROLL], vw[UNROLL];
+      float ks[UNROLL], vs[UNROLL];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int w = w0 + u * 256, word = w % WORDS, j = b * PR_KEYS + w / WORDS, d = (word % G) * 32 + (word / G) * 8;
+        kw[u] = vw[u] = 0;
+        ks[u] = vs[u] = 0.f;
+        if (j < seen) {
+          const size_t at = (size_t)unit * p.c.ctx + j;
+          kw[u] = __ldg(reinterpret_cast<const uint32_t*>(p.c.k_codes + at * (HD / 2)) + word);
+          vw[u] = __ldg(reinterpret_cast<const uint32_t*>(p.c.v_codes + at * (HD / 2)) + word);
+          ks[u] = __half2float(p.c.k_scales[at * nb + d / p.c.bs]);
+          vs[u] = __half2float(p.c.v_scales[at * nb + d / p.c.bs]);
         }
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = cache4_value(kw, e, ks);
-        k = pack8<__half>(x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = cache4_value(vw, e, vs);
-        v = pack8<__half>(x);
       }
-      const size_t to = ((size_t)unit * a.t_pad + j) * HD + d;
-      *reinterpret_cast<uint4*>(a.k_half + to) = k;
-      *reinterpret_cast<uint4*>(a.v_half + to) = v;
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        const int w = w0 + u * 256, word = w % WORDS, j = b * PR_KEYS + w / WORDS, d = (word % G) * 32 + (word / G) * 8;
+        if (vs[u] != vs[u]) {
+          atomicMin(&s_bad[d / p.c.bs], j);
+          vs[u] = 0.f;
+        }
+        float x[8], y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = cache4_value(kw[u], e, ks[u]);
+          y[e] = cache4_value(vw[u], e, vs[u]);
+        }
+        const size_t to = ((size_t)unit * a.t_pad + j) * HD + d;  // (rows behind the last one, to the block's end: zeros)
+        *reinterpret_cast<uint4*>(a.k_half + to) = pack8<__half>(x);
+        *reinterpret_cast<uint4*>(a.v_half + to) = pack8<__half>(y);
+      }
     }
     __syncthreads();
     if (threadIdx.x < 4) a.bad[((size_t)unit * key_blocks + b) * 4 + threadIdx.x] = s_bad[threadIdx.x];

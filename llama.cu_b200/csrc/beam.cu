@@ -23,6 +23,11 @@ __device__ __forceinline__ float logit_at(const float* p, size_t i) { return p[i
 __device__ __forceinline__ float logit_at(const __half* p, size_t i) { return __half2float(p[i]); }
 __device__ __forceinline__ float logit_at(const __nv_bfloat16* p, size_t i) { return __bfloat162float(p[i]); }
 
+__device__ __forceinline__ float ex2(float y) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+  return r;
+}
 // order of binary32 numbers as unsigned integers (-0 as 0), and back
 __device__ __forceinline__ uint32_t float_order(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
@@ -55,20 +60,25 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
     s_count = 0;
     s_threshold = 0;
   }
-  uint64_t top = 0;
-  float mx = -INFINITY, val[BEAM_ITEMS];
+  const bool full = v0 + BEAM_CHUNK <= a.p.n_vocab;
+  float val[BEAM_ITEMS];
 #pragma unroll
   for (int i = 0; i < BEAM_ITEMS; ++i) {
     const int v = v0 + i * BEAM_THREADS + tid;
-    val[i] = v < a.p.n_vocab ? logit_at(x, v) : -INFINITY;
+    val[i] = full || v < a.p.n_vocab ? logit_at(x, v) : -INFINITY;
   }
+  // the thread's largest and its first place, by comparing numbers; orders are formed for that one alone
+  float mx = -INFINITY;
+  int at = 0;
 #pragma unroll
   for (int i = 0; i < BEAM_ITEMS; ++i) {
-    const int v = v0 + i * BEAM_THREADS + tid;
     if (val[i] != val[i]) val[i] = -INFINITY;  // no number: never chosen before one
-    mx = fmaxf(mx, val[i]);
-    if (v < a.p.n_vocab) top = max(top, (uint64_t)float_order(val[i]) << 32 | (uint32_t)~v);
+    if (val[i] > mx) {
+      mx = val[i];
+      at = i;
+    }
   }
+  uint64_t top = v0 + at * BEAM_THREADS + tid < a.p.n_vocab ? (uint64_t)float_order(mx) << 32 | (uint32_t)~(v0 + at * BEAM_THREADS + tid) : 0ull;
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   if ((lane & 3) == 0) tops[tid >> 2] = top;
@@ -87,9 +97,10 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
   }
   double sum = 0.0;
   if (mx > -INFINITY) {
+    constexpr float LOG2E = 1.4426950408889634f;  // (2^-22 of a term, and 2^-24 of its distance from the maximum)
     float part = 0.f;
 #pragma unroll
-    for (int i = 0; i < BEAM_ITEMS; ++i) part += expf(val[i] - mx);
+    for (int i = 0; i < BEAM_ITEMS; ++i) part += ex2(fmaf(val[i], LOG2E, -mx * LOG2E));
     sum = part;
   }
 #pragma unroll
@@ -103,8 +114,10 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
   }
   const uint64_t threshold = s_threshold;
   if (top >= threshold) {  // (others' groups hold none)
+    const float bound = threshold ? order_float((uint32_t)(threshold >> 32)) : -INFINITY;
 #pragma unroll
     for (int i = 0; i < BEAM_ITEMS; ++i) {
+      if (val[i] < bound) continue;
       const int v = v0 + i * BEAM_THREADS + tid;
       const uint64_t k = (uint64_t)float_order(val[i]) << 32 | (uint32_t)~v;
       if (v < a.p.n_vocab && k >= threshold) cand[atomicAdd(&s_count, 1)] = k;
@@ -124,7 +137,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
 
 struct scored {
   uint64_t order;   // of the score in 64 bits; 0: nothing
-  uint64_t place;   // beam * n_vocab + token
+  uint64_t place;   // beam, token
 };
 __device__ __forceinline__ bool better(const scored& a, const scored& b) { return a.order > b.order || (a.order == b.order && a.place < b.place); }
 
@@ -168,8 +181,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
     const uint64_t k = a.best[((size_t)group * lists + list) * n_out + e];
     const bool fine = base[b] != -INFINITY;
     if (fine ? !k : list != b * a.chunks || e >= a.p.n_vocab) return scored{0, ~0ull};
-    if (!fine) return scored{double_order(-INFINITY), (uint64_t)b * a.p.n_vocab + e};
-    return scored{double_order((double)order_float((uint32_t)(k >> 32)) - lse[b] + base[b]), (uint64_t)b * a.p.n_vocab + (uint32_t)~(uint32_t)k};
+    if (!fine) return scored{double_order(-INFINITY), (uint64_t)b << 32 | (uint32_t)e};
+    return scored{double_order((double)order_float((uint32_t)(k >> 32)) - lse[b] + base[b]), (uint64_t)b << 32 | (uint32_t)~(uint32_t)k};
   };
   scored top{0, ~0ull};
 #pragma unroll 4
@@ -179,10 +192,13 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
   }
   tops[tid] = top;
   __syncthreads();
-  int rank = 0;
+  if (top.order) {
+    int rank = 0;
+    const int owners = min(lists, BEAM_THREADS);  // threads that own a list
 #pragma unroll 8
-  for (int t = 0; t < BEAM_THREADS; ++t) rank += better(tops[t], top);
-  if (top.order && rank == n_out - 1) s_threshold = top;
+    for (int t = 0; t < owners; ++t) rank += better(tops[t], top);
+    if (rank == n_out - 1) s_threshold = top;
+  }
   __syncthreads();
   const scored threshold = s_threshold;
   for (int l = tid; l < lists; l += BEAM_THREADS)
@@ -215,8 +231,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
         if (better(tops[t], best)) best = tops[t];
       if (tid == 0) {
         const size_t o = (size_t)group * n_out + r;
-        a.p.parents[o] = (int)(best.place / a.p.n_vocab);
-        a.p.tokens[o] = (int)(best.place % a.p.n_vocab);
+        a.p.parents[o] = (int)(best.place >> 32);
+        a.p.tokens[o] = (int)(uint32_t)best.place;
         a.p.scores_out[o] = (float)order_double(best.order);
       }
       last = best;
@@ -229,8 +245,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
     for (int t = 0; t < count; ++t) r += better(cand_scored[t], s);
     if (r < n_out) {
       const size_t o = (size_t)group * n_out + r;
-      a.p.parents[o] = (int)(s.place / a.p.n_vocab);
-      a.p.tokens[o] = (int)(s.place % a.p.n_vocab);
+      a.p.parents[o] = (int)(s.place >> 32);
+      a.p.tokens[o] = (int)(uint32_t)s.place;
       a.p.scores_out[o] = (float)order_double(s.order);
     }
   }
