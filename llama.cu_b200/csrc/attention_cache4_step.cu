@@ -35,6 +35,7 @@ struct step_args {
   cache4_attention_params p;
   int ctas, col_blocks;  // of the first kernel; units per (sequence, key/value head)
   int per_unit;          // CTAs of a unit, for a single sequence (0: chunks are dealt evenly, whatever the units)
+  bool alone;            // short caches: a CTA per unit and nothing to join
   float* parts;          // [ctas][2][cols][hd] sums of runs that begin, or end, inside a unit
   float2* part_ml;       // [ctas][2][cols] their maxima (powers of two) and sums
   int* part_bad;         // [ctas][2][4] first row whose values of a block are no numbers
@@ -178,12 +179,30 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
   const int group = p.n_heads / p.c.n_kv, n_cols = p.m * group, per_seq = p.c.n_kv * a.col_blocks;
   pdl_launch_dependents();
   const int bound = min(p.c.ctx, p.max_len);
-  unsigned before, sum_chunks;
-  count_chunks(p, 0, before, sum_chunks);
-  const step_plan plan(sum_chunks, per_seq, a);
-  if (blockIdx.x >= plan.ctas) return;
-  unsigned at = plan.first_of(blockIdx.x);
-  const unsigned end = plan.first_of(blockIdx.x + 1);
+  unsigned at, end;
+  int seq = 0;
+  unsigned seq_at = 0;                       // the sequence's first chunk
+  if (a.alone) {
+    seq = blockIdx.x / per_seq;
+    const int unit_in_seq = blockIdx.x - seq * per_seq, chunks = step_plan::chunks(p, p.lengths[seq]);
+    if (chunks == 0) {
+      const int kvh = unit_in_seq / a.col_blocks, c0 = unit_in_seq % a.col_blocks * COLS, here = min(COLS, n_cols - c0);
+      for (int e = tid; e < here * (HD / 2); e += ST_THREADS) {
+        const int c = c0 + e / (HD / 2);
+        reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + ((size_t)seq * p.m + c / group) * p.ld_out + (kvh * group + c % group) * HD)[e % (HD / 2)] = 0u;
+      }
+      return;
+    }
+    at = (unsigned)(unit_in_seq * chunks);
+    end = at + chunks;
+  } else {
+    unsigned before, sum_chunks;
+    count_chunks(p, 0, before, sum_chunks);
+    const step_plan plan(sum_chunks, per_seq, a);
+    if (blockIdx.x >= plan.ctas) return;
+    at = plan.first_of(blockIdx.x);
+    end = plan.first_of(blockIdx.x + 1);
+  }
   // tile row r stands for key perm(r): rows 2t, 2t+1, 2t+8, 2t+9, whose probabilities a lane multiplies with values, are keys 4t .. 4t+3
   const int key_a = 4 * (g >> 1) + (g & 1);  // rows g and g + 8: keys key_a and key_a + 2
   const uint32_t ring = smem_u32(s_raw) + warp * (ST_STAGES * STAGE);
@@ -194,8 +213,6 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
   auto word_at = [&](int i) { return (uint32_t)((((4 * t + i) * CPR + g * (4 * VW) / 16) ^ (t << 1)) * 16 + g * (4 * VW) % 16); };
   const uint32_t from_v0 = word_at(0), from_v1 = word_at(1), from_v2 = word_at(2), from_v3 = word_at(3);
   const uint32_t from_k = (uint32_t)(key_a * ROW + t * (4 * G));
-  int seq = 0;
-  unsigned seq_at = 0;                       // the sequence's first chunk
 
   while (at < end) {
     // ---- the unit that chunk `at` belongs to
@@ -572,6 +589,44 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
       }
     }
     if (!whole && tid < 4) a.part_bad[slot * 4 + tid] = s_bad[tid];
+    if constexpr (WEIGHTS) {
+      if (a.alone && a.col_blocks == 1) {  // every lane reads the scores that it wrote
+        float fin[NT][2], rl[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = n * 8 + 2 * t + e;
+            float top = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < ST_WARPS; ++w) top = fmaxf(top, s_ml[w][c].x);
+#pragma unroll
+            for (int w = 0; w < ST_WARPS; ++w) l += s_ml[w][c].y * (s_ml[w][c].x == -INFINITY ? 1.f : ex2(s_ml[w][c].x - top));
+            fin[n][e] = top;
+            rl[n][e] = 1.f / l;
+          }
+        for (int u = 2 * (lo + warp); u < 2 * hi; u += u & 1 ? 2 * ST_WARPS - 1 : 1) {
+          float add[2] = {0.f, 0.f};
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int c = n * 8 + 2 * t + (e & 1), j = u * ST_TILE + key_a + (e & 2);
+              if (j < limit_of(c)) add[e >> 1] += ex2(at_score[n][e & 1][j] - fin[n][e & 1]) * rl[n][e & 1];
+            }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            add[r] += __shfl_xor_sync(0xffffffffu, add[r], 1);
+            add[r] += __shfl_xor_sync(0xffffffffu, add[r], 2);
+            const int j = u * ST_TILE + key_a + 2 * r;
+            if (t == 0 && j < T_all) {
+              float* to = p.weights + head_rows + j;
+              *to = p.beta == 0.f || j >= held ? add[r] : fmaf(p.beta, *to, add[r]);
+            }
+          }
+        }
+      }
+    }
     __syncthreads();  // (the rings are free)
     at = unit_at + hi;
   }
@@ -614,8 +669,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step
       if (tid < LANES) out[tid] = 0u;
       return;
     }
-    const int2 ctas = ctas_of(unit_in_seq);
-    if (ctas.x == ctas.y) return;
+    const int2 ctas = a.alone ? make_int2(0, 0) : ctas_of(unit_in_seq);
+    if (a.alone || ctas.x == ctas.y) return;
     float top = -INFINITY, l = 0.f;
     for (int b = ctas.x + tid; b <= ctas.y; b += JOIN_THREADS) {
       s_k[b - ctas.x] = part_of(b, ctas.x, c).x;
@@ -671,7 +726,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step
     __syncthreads();
     for (int c = c64 + (tid >> 5); c < min(n_cols, c64 + 64); c += JOIN_THREADS / 32) {  // a column per warp
       const int unit_in_seq = kvh * a.col_blocks + c / COLS;
-      const int2 ctas = ctas_of(unit_in_seq);
+      const int2 ctas = a.alone ? make_int2(0, 0) : ctas_of(unit_in_seq);
       float2 all;
       if (ctas.x == ctas.y) {
         all = a.unit_ml[((size_t)seq * per_seq + unit_in_seq) * COLS + c % COLS];
@@ -713,8 +768,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step
 // long as they may be, up to two per SM (one with 16 columns, whose accumulators take the registers)
 struct step_shape {
   int cols, col_blocks, ctas, per_unit;
+  bool alone;
   long long units;
-  step_shape(int n_seqs, int m, int n_heads, int n_kv, int max_len) {
+  step_shape(int n_seqs, int m, int n_heads, int n_kv, int max_len, bool weights) {
     const int n_cols = m * (n_heads / n_kv);
     cols = n_cols <= 8 ? 8 : 16;
     col_blocks = (n_cols + cols - 1) / cols;
@@ -728,6 +784,15 @@ struct step_shape {
     const long long each = units > 0 && units <= most ? std::min(most / units, std::max(1ll, (chunks / units + ST_WARPS - 1) / ST_WARPS)) : 0;
     per_unit = n_seqs == 1 && (each >= 6 || (each && each * ST_WARPS * units >= chunks)) ? (int)each : 0;
     if (per_unit) ctas = (int)(per_unit * units);
+    // Short caches: a CTA per unit, one launch.  Its rounds of eight chunks (1.5 us each) against the even deal's other overheads, which grow
+    // with the units; the weights' second look at the scores costs as much again.  Alone / shared, us: 32 units x 500 rows 7.5 / 8.5,
+    // 700 8.9 / 8.9, 1000 10.7 / 9.6; 64 x 1400 13.3 / 15.3, 2000 16.3 / 16.7; 512 x 3000 52 / 63; with weights 32 x 250 8.3 / 9.2, 500
+    // 11.6 / 9.4; 64 x 500 13.8 / 15.2; 512 x 1000 42 / 45.
+    alone = chunks / units <= (weights ? 8 * std::min(4ll, std::max(1ll, units / 32)) : 22 * std::min(8ll, std::max(1ll, units / 32)));
+    if (alone) {
+      per_unit = 0;
+      ctas = (int)units;
+    }
   }
 };
 
@@ -744,6 +809,10 @@ int launch_step(const step_args& a, cudaStream_t stream) {
     if (dev < 16) attr_done[dev] = true;
   }
   kernel<<<a.ctas, ST_THREADS, SMEM, stream>>>(a);
+  if (a.alone && (!WEIGHTS || a.col_blocks == 1)) {
+    LCU_CUDA(cudaGetLastError());
+    return LCU_OK;
+  }
   const long long joins = (long long)a.p.c.n_seqs * a.p.c.n_kv * a.col_blocks * 8 * NT;
   const long long blocks = joins + (WEIGHTS ? (long long)a.p.c.n_seqs * a.p.c.n_kv * ((a.p.max_len + JOIN_KEYS - 1) / JOIN_KEYS) : 0);
   LCU_CUDA(launch_after(attention_join_kernel<T, HD, NB, NT>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, stream, a));
@@ -776,7 +845,7 @@ size_t step_layout(step_args* a, void* workspace, const step_shape& w, int n_seq
     used += round_up(bytes, 16);
     return (uint8_t*)workspace + at;
   };
-  const size_t slots = (size_t)w.ctas * 2;
+  const size_t slots = w.alone ? 0 : (size_t)w.ctas * 2;  // (one CTA per unit leaves no parts)
   uint8_t* parts = take(slots * w.cols * hd * sizeof(float));
   uint8_t* part_ml = take(slots * w.cols * sizeof(float2));
   uint8_t* part_bad = take(slots * 4 * sizeof(int));
@@ -795,14 +864,14 @@ size_t step_layout(step_args* a, void* workspace, const step_shape& w, int n_seq
 }  // namespace
 
 size_t attention_cache4_step_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
-  return step_layout(nullptr, nullptr, step_shape(n_seqs, m, n_heads, n_kv, max_len), n_seqs, m, n_heads, hd, max_len, weights);
+  return step_layout(nullptr, nullptr, step_shape(n_seqs, m, n_heads, n_kv, max_len, weights), n_seqs, m, n_heads, hd, max_len, weights);
 }
 
 int launch_attention_cache4_step(const cache4_attention_params& p, int dtype, void* workspace, cudaStream_t stream) {
   const long long chunks = (long long)p.c.n_seqs * p.c.n_kv * ((p.m * (p.n_heads / p.c.n_kv) + 7) / 8) * ((p.max_len + ST_CHUNK - 1) / ST_CHUNK);
   LCU_REQUIRE(chunks < (1ll << 31), "attention_cache4: %d sequences of %d heads over %d rows are too many", p.c.n_seqs, p.n_heads, p.max_len);
-  const step_shape w(p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.max_len);
-  step_args a{p, w.ctas, w.col_blocks, w.per_unit};
+  const step_shape w(p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.max_len, p.weights != nullptr);
+  step_args a{p, w.ctas, w.col_blocks, w.per_unit, w.alone};
   step_layout(&a, workspace, w, p.c.n_seqs, p.m, p.n_heads, p.c.hd, p.max_len, p.weights != nullptr);
   return dtype == OP_F16 ? launch_shape<__half>(a, w.cols, stream) : launch_shape<__nv_bfloat16>(a, w.cols, stream);
 }
