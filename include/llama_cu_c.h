@@ -132,8 +132,10 @@ int lcu_logits_head(void* probs_dev, const void* logits_dev, int n_vocab, float 
 /* ---- long contexts: a cache in 4 bits, eviction, beams ---------------------------------------- */
 /* No counterpart in the reference, whose caches are halves and whose client runs one sequence.  dtype of these operators: 0 half,
  * 1 bfloat16, 2 binary32 (logits only).  Lengths and positions are read on the device (a captured step replays with new ones) and
- * are the caller's to advance.  No call allocates, waits or keeps anything; workspaces belong to the caller, 16-byte aligned, with any
- * contents, and calls that may overlap on the GPU need one each.  Arguments are checked before anything is launched.
+ * are the caller's to advance.  No call waits or keeps anything, and none allocates but the first attention of more than 64 (row, query head) pairs per key/value
+ * head on a device, which takes 256 bytes for the operators' error word (make one outside stream capture; kernels are loaded then, too).
+ * Workspaces belong to the caller, 16-byte aligned, with any contents, and calls that may overlap on the GPU need one each.  Arguments are
+ * checked before anything is launched.
  *
  * A 4-bit cache of one layer is four planes, 16-byte aligned: codes, u8 [n_seqs][n_kv_heads][ctx_len][head_dim / 2], and scales, half
  * [n_seqs][n_kv_heads][ctx_len][head_dim / bs], for keys and for values.  head_dim 64 or 128; bs 32, 64 or 128, at most head_dim.

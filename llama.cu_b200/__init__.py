@@ -403,7 +403,8 @@ class Cache4:
         dp, dl, planes = DeviceBuffer.from_host(parents), DeviceBuffer.from_host(self.lengths), _pointers(self.planes)
         check(lib.lcu_cache_reorder(planes, planes, (C.c_int * 5)(*self.row_bytes), 5, dp.ptr, dl.ptr, groups, beams, self.n_kv, self.ctx, None))
         check(lib.lcu_synchronize())
-        at = (np.arange(groups)[:, None] * beams + parents).ravel()
+        own = np.arange(beams)[None]
+        at = (np.arange(groups)[:, None] * beams + np.where((parents >= 0) & (parents < beams), parents, own)).ravel()
         self.lengths, self.positions = self.lengths[at].copy(), self.positions[at].copy()
 
     def read(self, count, first=None):

@@ -27,6 +27,7 @@ int launch_attention_cache4(const cache4_attention_params& p, int dtype, void* w
   LCU_REQUIRE(p.ld_q % 8 == 0 && p.ld_out % 8 == 0 && p.ld_q >= p.n_heads * p.c.hd && p.ld_out >= p.n_heads * p.c.hd,
               "attention_cache4: row strides must be multiples of 8 that hold a row");
   LCU_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.out) & 15) == 0, "attention_cache4: rows must be 16-byte aligned");
+  LCU_REQUIRE(words_aligned(p.lengths, p.weights), "attention_cache4: lengths and weights must be 4-byte aligned");
   const size_t need = cache4_attention_workspace(p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.c.hd, p.max_len, p.weights != nullptr);
   LCU_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
               "attention_cache4: %zu bytes of 16-byte aligned workspace are needed, %zu are there", need, workspace ? workspace_bytes : (size_t)0);

@@ -262,6 +262,7 @@ size_t beam_select_workspace(int n_groups, int beams, int n_vocab, int n_out) {
 
 int launch_beam_select(const beam_params& p, int dtype, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   LCU_REQUIRE(p.parents && p.tokens && p.scores_out && p.logits && p.scores, "beam_select: a null pointer");
+  LCU_REQUIRE(words_aligned(p.parents, p.tokens, p.scores_out, p.scores), "beam_select: parents, tokens and scores must be 4-byte aligned");
   LCU_REQUIRE(dtype == OP_F16 || dtype == OP_BF16 || dtype == OP_F32, "beam_select: number format %d is not 0 (half), 1 (bfloat16) or 2 (binary32)", dtype);
   LCU_REQUIRE(p.n_groups >= 1 && p.beams >= 1 && p.beams <= MAX_BEAMS, "beam_select: %d groups of %d beams (1 to %d)", p.n_groups, p.beams, MAX_BEAMS);
   LCU_REQUIRE(p.n_vocab >= 1 && p.n_vocab <= (1 << 24) && p.ld >= p.n_vocab, "beam_select: a vocabulary of %d in rows of %d", p.n_vocab, p.ld);

@@ -22,6 +22,11 @@ struct cache4_view {
 enum op_dtype : int { OP_F16 = 0, OP_BF16 = 1, OP_F32 = 2 };
 
 int check_cache4(const char* who, const cache4_view& c);
+// numbers of four bytes at addresses that are multiples of four (null pointers pass)
+template <typename... P>
+bool words_aligned(const P*... p) {
+  return (((uintptr_t)p | ... | (uintptr_t)0) & 3) == 0;
+}
 
 struct cache4_append_params {
   cache4_view c;

@@ -197,6 +197,7 @@ int launch_cache4_append(const cache4_append_params& p, int dtype, cudaStream_t 
   LCU_REQUIRE(p.ld_kv % 8 == 0 && p.ld_kv >= p.c.n_kv * p.c.hd && (!p.q || (p.ld_q % 8 == 0 && p.ld_q >= p.n_heads * p.c.hd)),
               "cache4_append: row strides must be multiples of 8 that hold a row");
   LCU_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.q_out | (uintptr_t)p.k_new | (uintptr_t)p.v_new) & 15) == 0, "cache4_append: rows must be 16-byte aligned");
+  LCU_REQUIRE(words_aligned(p.lengths, p.positions), "cache4_append: lengths and positions must be 4-byte aligned");
   LCU_REQUIRE(!p.q || p.q_out != p.q || p.ld_q == p.n_heads * p.c.hd, "cache4_append: queries rotated in place must be dense");
   LCU_REQUIRE(p.theta == 0.f || (p.theta > 0.f && p.theta < 1e30f), "cache4_append: theta %g", (double)p.theta);
   if (int rc_dev = need_device()) return rc_dev;
@@ -220,8 +221,9 @@ int launch_cache4_read(void* k_out, void* v_out, const cache4_view& c, const int
   LCU_REQUIRE(dtype == OP_F16 || dtype == OP_BF16, "cache4_read: number format %d is not 0 (half) or 1 (bfloat16)", dtype);
   LCU_REQUIRE((k_out || v_out) && count >= 1, "cache4_read: nothing to read");
   LCU_REQUIRE((((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "cache4_read: outputs must be 16-byte aligned");
-  if (int rc_dev = need_device()) return rc_dev;
+  LCU_REQUIRE(words_aligned(first), "cache4_read: first rows must be 4-byte aligned");
   LCU_REQUIRE((long long)c.n_seqs * c.n_kv < (1ll << 31), "cache4_read: %d sequences of %d heads are too many", c.n_seqs, c.n_kv);
+  if (int rc_dev = need_device()) return rc_dev;
   if (dtype == OP_F16) launch_read((__half*)k_out, (__half*)v_out, c, first, count, stream);
   else launch_read((__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, c, first, count, stream);
   LCU_CUDA(cudaGetLastError());

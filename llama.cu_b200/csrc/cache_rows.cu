@@ -1,5 +1,6 @@
 // Eviction of cached rows by the attention weight they received, and reordering of the caches of a group of beams.
 #include "cache_rows.cuh"
+#include "cache4.cuh"
 
 #include <algorithm>
 
@@ -357,6 +358,7 @@ int launch_cache_evict(const evict_params& p, cudaStream_t stream) {
     if (rc) return rc;
   }
   LCU_REQUIRE(p.weights && p.kept && p.lengths, "cache_evict: a null pointer");
+  LCU_REQUIRE(words_aligned(p.weights, p.kept, p.lengths, p.lengths_out), "cache_evict: weights, lengths and the list must be 4-byte aligned");
   LCU_REQUIRE(p.n_seqs >= 1 && p.n_kv >= 1 && (long long)p.n_seqs * p.n_kv < (1 << 20) && p.ctx >= 1 && p.ctx < (1 << 26), "cache_evict: %d sequences of %d heads of %d rows", p.n_seqs,
               p.n_kv, p.ctx);
   LCU_REQUIRE(p.keep >= 1 && p.keep <= p.dst_ctx && p.keep <= p.ctx && p.recent >= 0 && p.recent <= p.keep,
@@ -411,6 +413,7 @@ int launch_cache_reorder(const reorder_params& p, cudaStream_t stream) {
   int rc = check_planes("cache_reorder", p.dst, p.src, p.row_bytes, p.n_planes);
   if (rc) return rc;
   LCU_REQUIRE(p.parents && p.lengths, "cache_reorder: a null pointer");
+  LCU_REQUIRE(words_aligned(p.parents, p.lengths), "cache_reorder: parents and lengths must be 4-byte aligned");
   LCU_REQUIRE(p.n_groups >= 1 && p.beams >= 1 && p.beams <= MAX_BEAMS, "cache_reorder: %d groups of %d beams (1 to %d)", p.n_groups, p.beams, MAX_BEAMS);
   LCU_REQUIRE(p.n_kv >= 1 && p.ctx >= 1 && p.ctx < (1 << 26) && (long long)p.n_groups * p.beams * p.n_kv < (1 << 20), "cache_reorder: %d groups of %d beams, %d heads of %d rows",
               p.n_groups, p.beams, p.n_kv, p.ctx);

@@ -26,7 +26,7 @@ def append(**k):
     (dict(hd=96), "head_dim 96"), (dict(hd=64, bs=128), "block size 128"), (dict(bs=16), "block size 16"), (dict(bs=0), "block size 0"), (dict(seqs=0), "no sequences"),
     (dict(kv=0), "no sequences"), (dict(ctx=0), "no sequences"), (dict(kc=A + 8), "16-byte aligned"), (dict(ks=A + 2), "16-byte aligned"), (dict(dtype=2), "number format 2"),
     (dict(m=0), "no rows"), (dict(heads=0), "no rows"), (dict(ldkv=248), "row strides"), (dict(ldq=516), "row strides"), (dict(k=A + 4), "16-byte aligned"),
-    (dict(ldq=520, qo=A), "must be dense"), (dict(theta=-1.0), "theta"), (dict(theta=float("nan")), "theta"), (dict(seqs=1 << 16, m=1 << 16), "too many")])
+    (dict(ldq=520, qo=A), "must be dense"), (dict(lengths=A + 2), "4-byte aligned"), (dict(positions=A + 1), "4-byte aligned"), (dict(theta=-1.0), "theta"), (dict(theta=float("nan")), "theta"), (dict(seqs=1 << 16, m=1 << 16), "too many")])
 def test_append_refuses(change, words):
     refused(append(**change), words)
 
@@ -41,7 +41,7 @@ def attend(**k):
     (dict(out=None), "null pointer"), (dict(q=None), "null pointer"), (dict(lengths=None), "null pointer"), (dict(kc=None), "null pointer"), (dict(heads=3), "3 heads over 2"),
     (dict(m=0), "0 rows"), (dict(most=65), "exceed the cache"), (dict(most=0), "exceed the cache"), (dict(ldo=504), "row strides"), (dict(ldq=500), "row strides"),
     (dict(q=A + 8), "16-byte aligned"), (dict(out=A + 2), "16-byte aligned"), (dict(dtype=2), "number format 2"), (dict(hd=80), "head_dim 80"),
-    (dict(w=A, ws=None), "workspace"), (dict(w=A, bytes=0), "workspace"), (dict(w=A, ws=A + 4), "workspace"), (dict(seqs=40000), "too many")])
+    (dict(m=200, ws=None), "workspace"), (dict(lengths=A + 1), "4-byte aligned"), (dict(w=A + 2), "4-byte aligned"), (dict(w=A, ws=None), "workspace"), (dict(w=A, bytes=0), "workspace"), (dict(w=A, ws=A + 4), "workspace"), (dict(seqs=40000), "too many")])
 def test_attention_refuses(change, words):
     refused(attend(**change), words)
 
@@ -56,6 +56,7 @@ def test_read_refuses():
     refused(read(ko=A + 4), "16-byte aligned")
     refused(read(dtype=5), "number format 5")
     refused(read(bs=24), "block size 24")
+    refused(read(first=A + 2), "4-byte aligned")
 
 
 def planes(*addresses):
@@ -82,6 +83,8 @@ def test_evict_refuses():
     refused(evict(dst=planes(1 << 24), dctx=9), "into 9")
     refused(evict(dctx=32), "in place")
     refused(evict(seqs=0), "0 sequences")
+    refused(evict(w=A + 2), "4-byte aligned")
+    refused(evict(lo=A + 1), "4-byte aligned")
 
 
 def test_reorder_refuses():
@@ -95,6 +98,7 @@ def test_reorder_refuses():
     refused(reorder(beams=33), "33 beams")
     refused(reorder(groups=0), "0 groups")
     refused(reorder(ctx=0), "0 rows")
+    refused(reorder(parents=A + 2), "4-byte aligned")
 
 
 def test_beam_select_refuses():
@@ -115,6 +119,18 @@ def test_beam_select_refuses():
     refused(select(dtype=2, logits=A + 2), "aligned to their type")
     refused(select(bytes=16), "workspace")
     refused(select(ws=None), "workspace")
+    refused(select(tokens=A + 2), "4-byte aligned")
+
+
+def test_workspaces_of_senseless_sizes():
+    """Queries of sizes that a call would refuse return 0; sensible ones grow with the rows."""
+    w = lcu.lib.lcu_attention_cache4_workspace
+    assert w(0, 1, 4, 2, 128, 64, 1) == 0 and w(1, 0, 4, 2, 128, 64, 1) == 0 and w(1, 1, 1, 2, 128, 64, 0) == 0 and w(1, 1, 4, 0, 128, 64, 0) == 0
+    assert w(1, 1, 4, 2, 128, 0, 0) == 0 and w(1, -5, 4, 2, 128, 64, 0) == 0
+    assert 0 < w(1, 500, 4, 2, 128, 600, 0) < w(1, 500, 4, 2, 128, 6000, 0)
+    assert w(1, 1, 32, 32, 128, 40000, 1) >= 32 * 40000 * 4 + w(1, 1, 32, 32, 128, 40000, 0)
+    b = lcu.lib.lcu_beam_select_workspace
+    assert b(0, 1, 5, 1) == 0 and b(1, 1, -5, 1) == 0 and b(2, 4, 32000, 4) > 0
 
 
 def test_valid_calls_need_a_device():
