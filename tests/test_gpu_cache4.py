@@ -254,6 +254,87 @@ def test_attention(lcu, dtype, hd, bs, seqs, m, lengths, heads, kv):
         assert torch.equal(third.view(torch.int16), again.view(torch.int16)) and torch.equal(twice.view(torch.int32), w.view(torch.int32))
 
 
+LONG = [
+    # seqs, m, lengths before, heads, kv: runs of chunks over several sequences and heads, columns in several blocks, tiles shared by CTAs
+    (3, 1, [3000, 0, 1700], 4, 2),
+    (4, 1, [900, -1, 2100, 31], 12, 1),
+    (1, 1, [4500], 40, 1),
+    (2, 5, [1500, 2222], 16, 4),
+    (1, 13, [3333], 8, 2),
+    (1, 40, [2500], 8, 4),
+    (3, 33, [1200, -1, 100], 6, 2),
+]
+
+
+@pytest.mark.parametrize("dtype,hd,bs", [("float16", 128, 32), ("bfloat16", 128, 64), ("float16", 128, 128), ("bfloat16", 64, 32), ("float16", 64, 64)])
+@pytest.mark.parametrize("seqs,m,lengths,heads,kv", LONG)
+def test_attention_of_long_caches(lcu, dtype, hd, bs, seqs, m, lengths, heads, kv):
+    rng = np.random.default_rng(m + heads + hd + bs)
+    ctx = max(lengths) + m + 1  # (an odd number of rows where blocks are whole rows: scales between words)
+    cache = Cache(lcu, seqs, kv, hd, ctx, bs, dtype)
+    for s, n in enumerate(lengths):
+        one = Cache(lcu, 1, kv, hd, ctx, bs, dtype)
+        if n >= 0:
+            one.fill(rng, n + m)
+        for p, o in zip(cache.planes, one.planes):
+            p[s] = o[0]
+    qb = P.float_to_bits(rng.standard_normal((seqs * m, heads * hd)) * 1.5, dtype)
+    old = torch.rand(seqs, kv, ctx, device="cuda")
+    plain = cache.attend(tensor(qb, dtype), i32(lengths), m, heads)
+    near_attention(cache, plain, qb, lengths, m, heads)
+    w = old.clone()
+    out = cache.attend(tensor(qb, dtype), i32(lengths), m, heads, weights=w, beta=0.5)
+    near_attention(cache, out, qb, lengths, m, heads, weights=w, old=old, beta=0.5)
+    # a block of values, and one of keys, without numbers: all dimensions of the rows that see the key, that block of those that see the values
+    group = heads // kv
+    row_v, row_k = lengths[0] // 3, lengths[0] + m // 2
+    cache.scales[1][0, 0, row_v, 0] = float("nan")
+    cache.scales[0][0, kv - 1, row_k, hd // bs - 1] = float("nan")
+    odd = cache.attend(tensor(qb, dtype), i32(lengths), m, heads).float().view(seqs, m, heads, hd)
+    want = plain.float().view(seqs, m, heads, hd).clone()
+    want[0, :, :group, :bs] = float("nan")
+    want[0, m // 2:, heads - group:] = float("nan")
+    assert torch.equal(torch.isnan(odd), torch.isnan(want))
+    assert torch.equal(odd[~torch.isnan(want)], want[~torch.isnan(want)])
+
+
+def test_captured_prompts_and_two_calls_at_once(lcu):
+    """A prompt's attention with weights captured and replayed on other rows; the same on two streams at the same time, a workspace each."""
+    hd, bs, kv, heads, dtype, m, held = 128, 32, 2, 8, "float16", 70, 130
+    rng = np.random.default_rng(6)
+    caches = [Cache(lcu, 1, kv, hd, held + m, bs, dtype) for _ in range(2)]
+    bits_of, qs, outs, ws, weights, streams = [], [], [], [], [], [torch.cuda.Stream() for _ in range(2)]
+    need = lcu.lib.lcu_attention_cache4_workspace(1, m, heads, kv, hd, held + m, 1)
+    for c in caches:
+        c.fill(rng, held + m)
+        bits_of.append(P.float_to_bits(rng.standard_normal((m, heads * hd)), dtype))
+        qs.append(tensor(bits_of[-1], dtype))
+        outs.append(torch.zeros(m, heads * hd, dtype=torch.float16, device="cuda"))
+        ws.append(torch.empty(need, dtype=torch.uint8, device="cuda"))
+        weights.append(torch.zeros(1, kv, held + m, device="cuda"))
+    lengths = i32([held])
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                caches[k].attend(qs[k], lengths, m, heads, weights=weights[k], beta=0.0, out=outs[k], ws=ws[k], stream=streams[k].cuda_stream)
+    torch.cuda.synchronize()
+    zero = torch.zeros_like(weights[0])
+    for k in range(2):
+        near_attention(caches[k], outs[k], bits_of[k], [held], m, heads, weights=weights[k], old=zero)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        caches[0].attend(qs[0], lengths, m, heads, weights=weights[0], beta=0.0, out=outs[0], ws=ws[0], stream=torch.cuda.current_stream().cuda_stream)
+    for n in (held, 60, 0):
+        b = P.float_to_bits(rng.standard_normal((m, heads * hd)), dtype)
+        qs[0].copy_(tensor(b, dtype))
+        lengths.copy_(i32([n]))
+        old = weights[0].clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        near_attention(caches[0], outs[0], b, [n], m, heads, weights=weights[0], old=old)
+
+
 @pytest.mark.parametrize("m", [1, 4, 130])
 def test_attention_of_extreme_scores(lcu, m):
     """Scores of thousands either way, one key that takes everything, equal keys, queries of zero, tiny and large bfloat16 queries."""
