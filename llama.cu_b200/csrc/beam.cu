@@ -142,10 +142,10 @@ struct scored {
 __device__ __forceinline__ bool better(const scored& a, const scored& b) { return a.order > b.order || (a.order == b.order && a.place < b.place); }
 
 // One CTA per group: log-sum-exp of every beam in 64 bits, then the n best of the chunks' candidates.  A thread owns chunks' lists, which are
-// sorted: their heads give a bound in the way of the first kernel, and lists are walked down to it.
+// sorted: the heads of 64 groups of lists give a bound in the way of the first kernel, and lists are walked down to it.
 __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_args a, int most) {
   __shared__ double lse[MAX_BEAMS], base[MAX_BEAMS];
-  __shared__ scored tops[BEAM_THREADS];
+  __shared__ scored tops[BEAM_THREADS];  // (the largest of four threads' lists each; of every thread in the other way)
   __shared__ scored s_threshold;
   __shared__ int s_count;
   extern __shared__ scored cand_scored[];
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
     mx = warp_max(mx);
     double sum = 0.0;
     if (mx > -INFINITY && mx < INFINITY)
-      for (int c = tid & 31; c < a.chunks; c += 32) sum += (double)st[c].y * exp((double)st[c].x - (double)mx);
+      for (int c = tid & 31; c < a.chunks; c += 32) sum += (double)(st[c].y * expf(st[c].x - mx));  // (2^-22 of a chunk's sum, as that is)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if ((tid & 31) == 0) {
@@ -190,14 +190,24 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
     const scored s = at(l, 0);
     if (better(s, top)) top = s;
   }
-  tops[tid] = top;
+  // (few lists: each a group of its own, the bound is closer then)
+  const int width = lists <= BEAM_GROUPS ? 1 : BEAM_THREADS / BEAM_GROUPS;
+  if (width > 1) {
+#pragma unroll
+    for (int o = 1; o < BEAM_THREADS / BEAM_GROUPS; o <<= 1) {
+      const scored other{__shfl_xor_sync(0xffffffffu, top.order, o), __shfl_xor_sync(0xffffffffu, top.place, o)};
+      if (better(other, top)) top = other;
+    }
+  }
+  if (tid % width == 0 && tid / width < BEAM_GROUPS) tops[tid / width] = top;
   __syncthreads();
-  if (top.order) {
+  const int groups = width > 1 ? BEAM_GROUPS : lists;
+  if (tid < groups && tops[tid].order) {
+    const scored mine = tops[tid];
     int rank = 0;
-    const int owners = min(lists, BEAM_THREADS);  // threads that own a list
 #pragma unroll 8
-    for (int t = 0; t < owners; ++t) rank += better(tops[t], top);
-    if (rank == n_out - 1) s_threshold = top;
+    for (int t = 0; t < groups; ++t) rank += better(tops[t], mine);
+    if (rank == n_out - 1) s_threshold = mine;
   }
   __syncthreads();
   const scored threshold = s_threshold;
@@ -274,9 +284,7 @@ int launch_beam_select(const beam_params& p, int dtype, void* workspace, size_t 
   LCU_REQUIRE(rows * chunks < (1ull << 31), "beam_select: too many rows of logits");
   LCU_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, "beam_select: %zu bytes of 16-byte aligned workspace are needed, %zu are there", need,
               workspace ? workspace_bytes : (size_t)0);
-  // at most n_out threads hold candidates, n_out in each of their lists
-  const size_t lists = (size_t)p.beams * chunks;
-  const int most = (int)std::min<size_t>(BEAM_MAX_CAND, std::min(lists, (size_t)p.n_out * ceil_div(lists, BEAM_THREADS)) * p.n_out);
+  const int most = (int)std::min<size_t>(BEAM_MAX_CAND, (size_t)p.beams * chunks * p.n_out);
   if (int rc_dev = need_device()) return rc_dev;
   beam_args a{p, chunks, (float2*)workspace, (uint64_t*)((float2*)workspace + rows * chunks)};
   const unsigned ctas = (unsigned)(rows * chunks);

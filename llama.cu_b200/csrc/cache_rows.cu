@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
     const int left = s_left;
     each([&](int, uint32_t key, bool there) {
       const bool in = there && (pass == 0 || (key >> (shift + bits)) == prefix);
+      if (pass && !__any_sync(0xffffffffu, in)) return;  // (most of a later pass)
       const uint32_t digit = in ? (key >> shift) & ((1u << bits) - 1) : 0xffffffffu;
       int same = 0;
       __match_all_sync(0xffffffffu, digit, &same);  // (equal weights, all zero before the first step: one add instead of 32 on one address)
