@@ -179,26 +179,34 @@ __device__ __forceinline__ int unit_bytes(const plane& p) {
 
 template <typename V>
 __device__ __forceinline__ void gather_rows(const gather_args& a, const plane& p, int sh, int first, int last) {
-  constexpr int UNROLL = 4;
+  constexpr int UNROLL = 2;
   const int units = p.row_bytes / (int)sizeof(V);
   const int* kept = a.kept + (size_t)sh * a.keep;
   const V* src = reinterpret_cast<const V*>(p.src) + (size_t)sh * a.ctx * units;
   V* dst = reinterpret_cast<V*>(p.dst) + (size_t)sh * a.dst_ctx * units;
-  const int n = (last - first) * units;
-  for (int t0 = threadIdx.x; t0 < n; t0 += blockDim.x * UNROLL) {
+  // unit u of row r; the next of this thread is 256 units on (no division on the way: it took a third of the time)
+  const int rows_on = 256 / units, units_on = 256 - rows_on * units;
+  int r = (int)threadIdx.x / units, u = (int)threadIdx.x - r * units;
+  for (r += first; r < last;) {
     V v[UNROLL];
-    int from[UNROLL];
+    int to[UNROLL];
+    size_t at[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int t = t0 + u * (int)blockDim.x;
-      from[u] = t < n ? kept[first + t / units] : -1;
-      if (from[u] >= 0) v[u] = src[(size_t)from[u] * units + t % units];
+    for (int k = 0; k < UNROLL; ++k) {
+      const int from = r < last ? kept[r] : -1;
+      to[k] = from;
+      at[k] = (size_t)r * units + u;
+      if (from >= 0) v[k] = src[(size_t)from * units + u];
+      r += rows_on;
+      u += units_on;
+      if (u >= units) {
+        u -= units;
+        ++r;
+      }
     }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int t = t0 + u * (int)blockDim.x;
-      if (from[u] >= 0) dst[(size_t)first * units + t] = v[u];
-    }
+    for (int k = 0; k < UNROLL; ++k)
+      if (to[k] >= 0) dst[at[k]] = v[k];
   }
 }
 
