@@ -325,6 +325,12 @@ def synth_f16(n, seed, name, scale, first=0):
 OP_DTYPES = {"float16": 0, "bfloat16": 1, "float32": 2}  # number formats of the operators over 4-bit caches and of the beam selection
 
 
+def _need(ok, words):
+    """For host arrays whose shapes say how much the library reads."""
+    if not ok:
+        raise LcuError(words)
+
+
 def _pointers(buffers):
     return (vp * len(buffers))(*[b.ptr for b in buffers])
 
@@ -332,9 +338,11 @@ def _pointers(buffers):
 def beam_select(logits, scores, n_out, dtype="float32"):
     """The n_out best continuations of every group of beams: logits [groups, beams, n_vocab] (binary32, or 16-bit patterns as uint16),
     scores [groups, beams]; returns (parents, tokens, scores), each [groups, n_out], best first."""
-    logits = np.ascontiguousarray(logits)
+    logits, scores = np.ascontiguousarray(logits), np.ascontiguousarray(scores, np.float32)
+    _need(dtype in OP_DTYPES and logits.dtype == (np.float32 if dtype == "float32" else np.uint16), f"beam_select: logits of {dtype} in an array of {logits.dtype}")
+    _need(logits.ndim == 3 and logits.size > 0 and scores.shape == logits.shape[:2] and n_out >= 1, f"beam_select: {n_out} of logits {logits.shape} with scores {scores.shape}")
     groups, beams, n_vocab = logits.shape
-    dl, ds = DeviceBuffer.from_host(logits), DeviceBuffer.from_host(np.asarray(scores, np.float32))
+    dl, ds = DeviceBuffer.from_host(logits), DeviceBuffer.from_host(scores)
     out = [DeviceBuffer(groups * n_out * 4) for _ in range(3)]
     ws = DeviceBuffer(max(16, lib.lcu_beam_select_workspace(groups, beams, n_vocab, n_out)))
     check(lib.lcu_beam_select(out[0].ptr, out[1].ptr, out[2].ptr, dl.ptr, n_vocab, OP_DTYPES[dtype], ds.ptr, groups, beams, n_vocab, n_out, ws.ptr, ws.nbytes, None))
@@ -347,6 +355,8 @@ class Cache4:
     patterns as uint16); `lengths` rows are held, the next row's position is `positions`."""
 
     def __init__(self, n_seqs, n_kv_heads, head_dim, ctx_len, bs=32, dtype="float16"):
+        _need(dtype in ("float16", "bfloat16") and min(n_seqs, n_kv_heads, ctx_len) >= 1 and head_dim in (64, 128) and bs in (32, 64, 128) and bs <= head_dim,
+              f"Cache4: {n_seqs} sequences of {n_kv_heads} heads of {ctx_len} rows of {head_dim} {dtype} in blocks of {bs}")
         self.n_seqs, self.n_kv, self.hd, self.ctx, self.bs, self.dtype = n_seqs, n_kv_heads, head_dim, ctx_len, bs, OP_DTYPES[dtype]
         rows = n_seqs * n_kv_heads * ctx_len
         self.row_bytes = [head_dim // 2, 2 * head_dim // bs] * 2 + [4]
@@ -358,11 +368,25 @@ class Cache4:
     def _shape(self):
         return self.n_kv, self.hd, self.bs, self.ctx
 
+    def _per_seq(self, a):
+        a = np.ascontiguousarray(a)
+        _need(a.shape == (self.n_seqs,) and a.dtype.kind in "iu", f"Cache4: {a.shape} numbers of {a.dtype} for {self.n_seqs} sequences")
+        return a.astype(np.int32)
+
+    def _rows(self, a, width):
+        """Rows of the call, [seqs, m, heads * hd]; width None: any number of heads."""
+        a = np.ascontiguousarray(a, np.uint16)
+        _need(a.ndim == 3 and a.size > 0 and a.shape[0] == self.n_seqs and a.shape[2] % self.hd == 0 and width in (None, a.shape[2]),
+              f"Cache4: rows {a.shape} for {self.n_seqs} sequences and heads of {self.hd}")
+        return a
+
     def append(self, q, k, v, theta=10000.0):
         """Rows q [seqs, m, heads * hd], k, v [seqs, m, kv * hd] at the sequences' ends; returns the rotated queries.  `advance` counts them."""
-        q, k, v = (np.ascontiguousarray(a, np.uint16) for a in (q, k, v))
+        q, k, v = self._rows(q, None), self._rows(k, self.n_kv * self.hd), self._rows(v, self.n_kv * self.hd)
         m, heads = q.shape[1], q.shape[2] // self.hd
-        dq, dk, dv, dl, dp = (DeviceBuffer.from_host(a) for a in (q, k, v, self.lengths, self.positions))
+        _need(k.shape[1] == v.shape[1] == m, f"Cache4: {m} queries, {k.shape[1]} keys and {v.shape[1]} values per sequence")
+        lengths, positions = self._per_seq(self.lengths), self._per_seq(self.positions)
+        dq, dk, dv, dl, dp = (DeviceBuffer.from_host(a) for a in (q, k, v, lengths, positions))
         check(lib.lcu_cache4_append(*[p.ptr for p in self.planes[:4]], dq.ptr, dq.ptr, q.shape[2], dk.ptr, dv.ptr, k.shape[2], dl.ptr, dp.ptr,
                                     self.n_seqs, m, heads, *self._shape(), theta, self.dtype, None))
         check(lib.lcu_synchronize())
@@ -371,9 +395,9 @@ class Cache4:
     def attend(self, q, beta=1.0):
         """Attention of rotated queries [seqs, m, heads * hd] whose own rows are in the cache but not yet counted; the rows' weights become
         beta times the old ones plus what they receive now."""
-        q = np.ascontiguousarray(q, np.uint16)
-        m, heads, most = q.shape[1], q.shape[2] // self.hd, min(self.ctx, max(1, int(self.lengths.max()) + q.shape[1]))
-        dq, dl, do = DeviceBuffer.from_host(q), DeviceBuffer.from_host(self.lengths), DeviceBuffer(q.nbytes)
+        q, lengths = self._rows(q, None), self._per_seq(self.lengths)
+        m, heads, most = q.shape[1], q.shape[2] // self.hd, min(self.ctx, max(1, int(lengths.max()) + q.shape[1]))
+        dq, dl, do = DeviceBuffer.from_host(q), DeviceBuffer.from_host(lengths), DeviceBuffer(q.nbytes)
         ws = DeviceBuffer(max(16, lib.lcu_attention_cache4_workspace(self.n_seqs, m, heads, self.n_kv, self.hd, most, 1)))
         check(lib.lcu_attention_cache4(do.ptr, q.shape[2], self.planes[4].ptr, beta, dq.ptr, q.shape[2], *[p.ptr for p in self.planes[:4]], dl.ptr, self.n_seqs, m,
                                        heads, *self._shape(), most, self.dtype, ws.ptr, ws.nbytes, None))
@@ -388,7 +412,8 @@ class Cache4:
 
     def evict(self, keep, recent):
         """Leaves `keep` rows of every sequence and head: the `recent` latest and the ones with most weight.  Returns their old places."""
-        dl, kept = DeviceBuffer.from_host(self.lengths), DeviceBuffer(self.n_seqs * self.n_kv * keep * 4)
+        _need(1 <= keep <= self.ctx, f"Cache4: keep {keep} rows of {self.ctx}")
+        dl, kept = DeviceBuffer.from_host(self._per_seq(self.lengths)), DeviceBuffer(self.n_seqs * self.n_kv * keep * 4)
         planes = _pointers(self.planes)
         check(lib.lcu_cache_evict(planes, planes, (C.c_int * 5)(*self.row_bytes), 5, self.planes[4].ptr, kept.ptr, dl.ptr, dl.ptr, self.n_seqs, self.n_kv, self.ctx,
                                   self.ctx, keep, recent, None))
@@ -399,8 +424,10 @@ class Cache4:
     def reorder(self, parents):
         """Sequences as beams of groups, parents [groups, beams]: beam b goes on from beam parents[g, b]."""
         parents = np.ascontiguousarray(parents, np.int32)
+        _need(parents.ndim == 2 and parents.size == self.n_seqs, f"Cache4: parents {parents.shape} for {self.n_seqs} sequences")
         groups, beams = parents.shape
-        dp, dl, planes = DeviceBuffer.from_host(parents), DeviceBuffer.from_host(self.lengths), _pointers(self.planes)
+        lengths = self._per_seq(self.lengths)
+        dp, dl, planes = DeviceBuffer.from_host(parents), DeviceBuffer.from_host(lengths), _pointers(self.planes)
         check(lib.lcu_cache_reorder(planes, planes, (C.c_int * 5)(*self.row_bytes), 5, dp.ptr, dl.ptr, groups, beams, self.n_kv, self.ctx, None))
         check(lib.lcu_synchronize())
         own = np.arange(beams)[None]
@@ -409,7 +436,8 @@ class Cache4:
 
     def read(self, count, first=None):
         """Keys and values of `count` rows from row first[s] on, as 16-bit patterns [seqs, kv, count, hd]."""
-        df = None if first is None else DeviceBuffer.from_host(np.asarray(first, np.int32))
+        _need(count >= 1, f"Cache4: {count} rows to read")
+        df = None if first is None else DeviceBuffer.from_host(self._per_seq(first))
         out = [DeviceBuffer(self.n_seqs * self.n_kv * count * self.hd * 2) for _ in range(2)]
         check(lib.lcu_cache4_read(out[0].ptr, out[1].ptr, *[p.ptr for p in self.planes[:4]], df.ptr if df else None, self.n_seqs, count, *self._shape(), self.dtype, None))
         check(lib.lcu_synchronize())

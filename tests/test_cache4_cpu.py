@@ -163,3 +163,66 @@ def test_plain_eviction_and_beams():
     assert P.evict(w, 3, 4, 1) == [0, 1, 2] and P.evict(w, -1, 4, 1) == []
     p, t, s = P.beam_select(np.array([[0.0, 1.0], [0.0, 1.0]]), np.array([-1.0, -1.0]), 4)
     assert p.tolist() == [0, 1, 0, 1] and t.tolist() == [1, 1, 0, 0]
+
+
+def cache_without_planes(**k):
+    """As Cache4 makes it, without a device: the calls below are refused before anything is allocated."""
+    c = object.__new__(lcu.Cache4)
+    a = dict(n_seqs=4, n_kv=2, hd=64, ctx=32, bs=32, dtype=0, lengths=np.zeros(4, np.int32), positions=np.zeros(4, np.int32), planes=[], row_bytes=[])
+    c.__dict__.update({**a, **k})
+    return c
+
+
+def rows(seqs, m, width):
+    return np.zeros((seqs, m, width), np.uint16)
+
+
+@pytest.mark.parametrize("call", [
+    lambda c: c.append(rows(3, 2, 256), rows(4, 2, 128), rows(4, 2, 128)),   # fewer sequences than the cache has
+    lambda c: c.append(rows(4, 2, 256), rows(4, 1, 128), rows(4, 2, 128)),   # fewer keys than queries
+    lambda c: c.append(rows(4, 2, 256), rows(4, 2, 128), rows(4, 1, 128)),
+    lambda c: c.append(rows(4, 2, 256), rows(4, 2, 128), rows(4, 2, 64)),    # values of one head
+    lambda c: c.append(rows(4, 2, 200), rows(4, 2, 128), rows(4, 2, 128)),   # heads cut off
+    lambda c: c.append(rows(4, 0, 256), rows(4, 0, 128), rows(4, 0, 128)),
+    lambda c: c.attend(rows(1, 2, 256)),
+    lambda c: c.attend(rows(4, 2, 100)),
+    lambda c: c.attend(np.zeros((4, 256), np.uint16)),
+    lambda c: c.evict(0, 0),
+    lambda c: c.evict(33, 0),
+    lambda c: c.reorder(np.zeros((1, 2), np.int32)),                         # two beams of four sequences
+    lambda c: c.reorder(np.zeros((2, 4), np.int32)),                         # eight
+    lambda c: c.reorder(np.zeros(4, np.int32)),
+    lambda c: c.read(0),
+    lambda c: c.read(2, first=[0, 0])])
+def test_cache_refuses_arrays_of_other_shapes(call):
+    with pytest.raises(lcu.LcuError, match="Cache4"):
+        call(cache_without_planes())
+
+
+@pytest.mark.parametrize("lengths", [np.zeros(3, np.int32), np.zeros(4), np.zeros((4, 1), np.int32)])
+def test_cache_refuses_lengths_of_other_shapes(lengths):
+    c = cache_without_planes(lengths=lengths)
+    for call in (lambda: c.append(rows(4, 1, 256), rows(4, 1, 128), rows(4, 1, 128)), lambda: c.attend(rows(4, 1, 256)), lambda: c.evict(8, 0),
+                 lambda: c.reorder(np.zeros((1, 4), np.int32))):
+        with pytest.raises(lcu.LcuError, match="Cache4"):
+            call()
+
+
+@pytest.mark.parametrize("change", [dict(n_seqs=0), dict(n_kv_heads=0), dict(ctx_len=0), dict(head_dim=96), dict(bs=16), dict(head_dim=64, bs=128), dict(dtype="float32")])
+def test_cache_of_senseless_sizes(change):
+    with pytest.raises(lcu.LcuError, match="Cache4"):
+        lcu.Cache4(**{**dict(n_seqs=1, n_kv_heads=1, head_dim=128, ctx_len=8), **change})
+
+
+@pytest.mark.parametrize("logits,scores,n_out,dtype", [
+    (np.zeros((1, 2, 8), np.uint16), np.zeros((1, 2)), 2, "float32"),    # half as many bytes as the format says
+    (np.zeros((1, 2, 8)), np.zeros((1, 2)), 2, "float32"),
+    (np.zeros((1, 2, 8), np.float32), np.zeros((1, 2)), 2, "bfloat16"),
+    (np.zeros((1, 2, 8), np.float32), np.zeros((1, 2)), 2, "float64"),
+    (np.zeros((1, 2, 8), np.float32), np.zeros((1, 1)), 2, "float32"),
+    (np.zeros((2, 8), np.float32), np.zeros(2), 2, "float32"),
+    (np.zeros((0, 2, 8), np.float32), np.zeros((0, 2)), 2, "float32"),
+    (np.zeros((1, 2, 8), np.float32), np.zeros((1, 2)), 0, "float32")])
+def test_beam_selection_refuses_arrays_of_other_shapes(logits, scores, n_out, dtype):
+    with pytest.raises(lcu.LcuError, match="beam_select"):
+        lcu.beam_select(logits, scores, n_out, dtype)
