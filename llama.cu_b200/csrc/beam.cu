@@ -137,8 +137,10 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
 
 struct scored {
   uint64_t order;   // of the score in 64 bits; 0: nothing
-  uint64_t place;   // beam, token
+  uint64_t place;   // beam, complement of the logit's order, token: logits whose difference 64 bits of a score lose keep the order of their list
 };
+__device__ __forceinline__ int beam_of(uint64_t place) { return (int)(place >> 56); }
+__device__ __forceinline__ int token_of(uint64_t place) { return (int)(place & 0xffffffu); }
 __device__ __forceinline__ bool better(const scored& a, const scored& b) { return a.order > b.order || (a.order == b.order && a.place < b.place); }
 
 // One CTA per group: log-sum-exp of every beam in 64 bits, then the n best of the chunks' candidates.  A thread owns chunks' lists, which are
@@ -181,8 +183,9 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
     const uint64_t k = a.best[((size_t)group * lists + list) * n_out + e];
     const bool fine = base[b] != -INFINITY;
     if (fine ? !k : list != b * a.chunks || e >= a.p.n_vocab) return scored{0, ~0ull};
-    if (!fine) return scored{double_order(-INFINITY), (uint64_t)b << 32 | (uint32_t)e};
-    return scored{double_order((double)order_float((uint32_t)(k >> 32)) - lse[b] + base[b]), (uint64_t)b << 32 | (uint32_t)~(uint32_t)k};
+    if (!fine) return scored{double_order(-INFINITY), (uint64_t)b << 56 | (uint32_t)e};
+    const uint32_t logit = (uint32_t)(k >> 32);
+    return scored{double_order((double)order_float(logit) - lse[b] + base[b]), (uint64_t)b << 56 | (uint64_t)~logit << 24 | (uint32_t)~(uint32_t)k};
   };
   scored top{0, ~0ull};
 #pragma unroll 4
@@ -241,8 +244,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
         if (better(tops[t], best)) best = tops[t];
       if (tid == 0) {
         const size_t o = (size_t)group * n_out + r;
-        a.p.parents[o] = (int)(best.place >> 32);
-        a.p.tokens[o] = (int)(uint32_t)best.place;
+        a.p.parents[o] = beam_of(best.place);
+        a.p.tokens[o] = token_of(best.place);
         a.p.scores_out[o] = (float)order_double(best.order);
       }
       last = best;
@@ -255,8 +258,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
     for (int t = 0; t < count; ++t) r += better(cand_scored[t], s);
     if (r < n_out) {
       const size_t o = (size_t)group * n_out + r;
-      a.p.parents[o] = (int)(s.place >> 32);
-      a.p.tokens[o] = (int)(uint32_t)s.place;
+      a.p.parents[o] = beam_of(s.place);
+      a.p.tokens[o] = token_of(s.place);
       a.p.scores_out[o] = (float)order_double(s.order);
     }
   }

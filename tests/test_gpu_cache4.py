@@ -526,6 +526,20 @@ def test_evict_unaligned_planes(lcu):
 
 
 # ------------------------------------------------------------------ beams
+@pytest.mark.parametrize("beams,vocab,n_out", [(1, 50, 6), (1, 4096, 64), (3, 9000, 64), (2, 70000, 17)])
+@pytest.mark.parametrize("tiny", [1e-30, 1.0])
+def test_beam_logits_whose_difference_a_score_loses(lcu, beams, vocab, n_out, tiny):
+    """Equal scores, distinct logits: the lowest beam's, in the order of logits, then of tokens (scores of 1e30 lose any logit)."""
+    rng = np.random.default_rng(vocab)
+    x = (rng.integers(-300, 300, (1, beams, vocab)) * tiny).astype(np.float32)
+    scores = np.full((1, beams), -1.0 if tiny < 1 else -1e30, np.float32)
+    parents, tokens, out = lcu.beam_select(x, scores, n_out)
+    order = np.lexsort((np.arange(vocab), -x[0, 0]))[:n_out]
+    assert (parents == 0).all() and tokens[0].tolist() == order.tolist()
+    lse = np.log(np.exp(x[0, 0].astype(np.float64) - x.max()).sum()) + x.max()
+    assert np.allclose(out[0], -lse - 1 if tiny < 1 else -1e30, rtol=1e-6)
+
+
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
 @pytest.mark.parametrize("groups,beams,vocab,n_out", [(1, 1, 1, 1), (1, 1, 7, 7), (2, 3, 50, 6), (1, 4, 4095, 4), (3, 2, 4097, 64), (2, 5, 32000, 10), (1, 32, 12289, 32), (1, 16, 128000, 32)])
 def test_beam_select(lcu, dtype, groups, beams, vocab, n_out):
