@@ -26,7 +26,9 @@
 namespace lcu {
 namespace {
 
-constexpr int PR_ROWS = 128, PR_KEYS = 128, PR_SOFT_WARPS = 8, PR_THREADS = 32 * (PR_SOFT_WARPS + 2);
+constexpr int PR_ROWS = 128, PR_KEYS = 128, PR_STEP = 64;
+constexpr int PR_SOFT_WARPS = 4, PR_THREADS = 32 * (PR_SOFT_WARPS + 2);  // of the kernel of the outputs
+constexpr int PW_SOFT_WARPS = 8, PW_THREADS = 32 * (PW_SOFT_WARPS + 2);  // of the weights'
 
 struct prompt_args {
   cache4_attention_params p;
@@ -192,14 +194,6 @@ __device__ __forceinline__ void st_32x32(uint32_t taddr, const uint32_t* r) {
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
@@ -215,14 +209,16 @@ struct prompt_shape {
   static constexpr int NKB = HD / 64;                        // 64-wide blocks of the head dimension
   static constexpr uint32_t BLOCK = 128 * 64 * 2;            // 128 rows x 64 dimensions
   static constexpr uint32_t OPERAND = NKB * BLOCK;           // queries, keys or values (2 x NKB atoms of 64 keys x 64 dimensions)
-  static constexpr int RING = HD == 128 ? 2 : 4;             // two CTAs per SM
-  static constexpr uint32_t SMEM = (1 + RING) * OPERAND + 1024 /* alignment slack */ + 256 /* barriers, tensor-memory slot */;
+  static constexpr uint32_t STEP = NKB * 64 * 64 * 2;        // 64 keys, or 64 values
+  static constexpr int RING = 4;                             // two CTAs per SM
+  static constexpr uint32_t SMEM = OPERAND + RING * STEP + 1024 /* alignment slack */ + 256 /* barriers, tensor-memory slot */;
   static constexpr uint32_t IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+  static constexpr uint32_t IDESC_S64 = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
   static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);  // values: contiguous along the dimension
 };
 
 // barriers
-constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + 4, B_S = B_EMPTY + 4, B_P = B_S + 1, B_O = B_P + 1, B_COUNT = B_O + 1;
+constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + 4, B_S = B_EMPTY + 4, B_P = B_S + 2, B_V = B_P + 2, B_O = B_V + 1, B_COUNT = B_O + 1;
 
 // ------------------------------------------------------------------ outputs
 template <typename T, int HD, bool SPLIT>
@@ -230,17 +226,15 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
                                                                          const __grid_constant__ CUtensorMap map_v, const prompt_args a, int row_blocks, int units) {
   using sh = prompt_shape<HD>;
   constexpr int NKB = sh::NKB, RING = sh::RING;
-  constexpr uint32_t OPERAND = sh::OPERAND, V_ATOM = 64 * 64 * 2, TMEM_COLS = 256, O_COL = 128;
+  constexpr uint32_t OPERAND = sh::OPERAND, STEP = sh::STEP, ATOM = 64 * 64 * 2, TMEM_COLS = 256, O_COL = 128;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t q_addr = base, ring_addr = base + OPERAND;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (1 + RING) * OPERAND);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + OPERAND + RING * STEP);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ int s_bad[4];
-  __shared__ int s_raise[2][PR_SOFT_WARPS];
-  __shared__ float s_half[2][PR_ROWS];
   const cache4_attention_params& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.n_heads / p.c.n_kv, rows = p.m * group;
@@ -253,8 +247,11 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
       mbar_init(smem_u32(&bars[B_FULL + i]), 1);
       mbar_init(smem_u32(&bars[B_EMPTY + i]), 1);
     }
-    mbar_init(smem_u32(&bars[B_S]), 1);
-    mbar_init(smem_u32(&bars[B_P]), PR_SOFT_WARPS);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars[B_S + i]), 1);
+      mbar_init(smem_u32(&bars[B_P + i]), PR_SOFT_WARPS);
+    }
+    mbar_init(smem_u32(&bars[B_V]), 1);
     mbar_init(smem_u32(&bars[B_O]), 1);
     *failed = 0;
     *gave_up = 0;
@@ -294,6 +291,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
   }
   struct run {
     int item, first, last, all;  // tiles [first, last) of an item's `all`
+    int from, to;                // and steps of 64 keys: as far as the last row sees
     int seq, kvh, unit, r0, held;
   };
   int pos = lo;
@@ -308,10 +306,15 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
       w.all = tiles_of(p, w.held, w.r0 / PR_ROWS);
       w.first = 0;
       w.last = w.all;
+      const int steps = w.all ? (limit_of(p, w.held, (min(w.r0 + PR_ROWS, rows) - 1) / group) + PR_STEP - 1) / PR_STEP : 0;
+      w.from = 0;
+      w.to = steps;
       if constexpr (!SPLIT) return true;
       const int begin = a.prefix[item];
       w.first = pos - begin;
       w.last = min(w.all, hi - begin);
+      w.from = 2 * w.first;
+      w.to = min(2 * w.last, steps);
       if (w.last > w.first) {
         pos = begin + w.last;
         ++item;
@@ -332,64 +335,67 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         if (!ok) break;
         mbar_arrive_expect_tx(smem_u32(&bars[B_Q]), OPERAND);
         for (int kb = 0; kb < NKB; ++kb) tma_load_3d(q_addr + kb * sh::BLOCK, &map_q, kb * 64, w.r0, w.unit, smem_u32(&bars[B_Q]));
-        for (int it = 2 * w.first; it < 2 * w.last; ++it, r.step(RING)) {
+        for (int it = 2 * w.from; it < 2 * w.to; ++it, r.step(RING)) {
           ok = mbar_wait(smem_u32(&bars[B_EMPTY + r.slot]), r.phase ^ 1u, a.err, DEV_ERR_EMPTY_WAIT, HEED);
           if (!ok) break;
-          const uint32_t full = smem_u32(&bars[B_FULL + r.slot]), dst = ring_addr + (uint32_t)r.slot * OPERAND;
-          const int j0 = (it >> 1) * PR_KEYS;
-          mbar_arrive_expect_tx(full, OPERAND);
+          const uint32_t full = smem_u32(&bars[B_FULL + r.slot]), dst = ring_addr + (uint32_t)r.slot * STEP;
+          mbar_arrive_expect_tx(full, STEP);
           if (!(it & 1)) {
-            for (int kb = 0; kb < NKB; ++kb) tma_load_3d(dst + kb * sh::BLOCK, &map_k, kb * 64, j0, w.unit, full);
+            for (int c = 0; c < NKB; ++c) tma_load_3d(dst + c * ATOM, &map_k, c * 64, (it >> 1) * PR_STEP, w.unit, full);
           } else {
-            for (int kb2 = 0; kb2 < 2; ++kb2)
-              for (int c = 0; c < NKB; ++c) tma_load_3d(dst + (kb2 * NKB + c) * V_ATOM, &map_v, c * 64, j0 + kb2 * 64, w.unit, full);
+            for (int c = 0; c < NKB; ++c) tma_load_3d(dst + c * ATOM, &map_v, c * 64, (it >> 1) * PR_STEP, w.unit, full);
           }
         }
       }
     }
     __syncwarp();
   } else if (warp == PR_SOFT_WARPS + 1) {
-    // ---- products, in this order: S_0, O += P_0 V_0, S_1, ..: scores only replace probabilities that have been read
-    tc_ring r;
+    // ---- products, in this order: S_0, S_1, O += P_0 V_0, S_2, O += P_1 V_1, ..: a step's scores are there when the step before is done, and
+    // only replace probabilities whose product comes before them
+    tc_ring r;  // (keys and values in the loads' order: K_0, V_0, K_1, ..)
     run w;
     bool ok = true;
     int count = 0;
     for (int item = item0, n = 0; ok && (SPLIT || n == 0) && next_run(w, item); ++n) {
       if (w.all == 0) break;
       ok = mbar_wait_warp(smem_u32(&bars[B_Q]), (uint32_t)n & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
-      for (int j = w.first; j < w.last && ok; ++j, ++count) {
-        ok = mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
-        if (!ok) break;
+      auto scores = [&](const tc_ring& keys, int buffer) {
+        ok = ok && mbar_wait_warp(smem_u32(&bars[B_FULL + keys.slot]), keys.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
+        if (!ok) return;
         tc_fence_after();
         if (tc_elect()) {
 #pragma unroll
           for (int kb = 0; kb < NKB; ++kb) {
-            const uint64_t a_desc = smem_desc_sw128(q_addr + kb * sh::BLOCK), b_desc = smem_desc_sw128(ring_addr + (uint32_t)r.slot * OPERAND + kb * sh::BLOCK);
+            const uint64_t a_desc = smem_desc_sw128(q_addr + kb * sh::BLOCK), b_desc = smem_desc_sw128(ring_addr + (uint32_t)keys.slot * STEP + kb * ATOM);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, a_desc + 2 * k, b_desc + 2 * k, sh::IDESC_S, (kb | k) != 0);
+            for (int k = 0; k < 4; ++k) tc_mma_f16(tmem + (uint32_t)(buffer * PR_STEP), a_desc + 2 * k, b_desc + 2 * k, sh::IDESC_S64, (kb | k) != 0);
           }
-          tc_commit(smem_u32(&bars[B_EMPTY + r.slot]));
-          tc_commit(smem_u32(&bars[B_S]));
+          tc_commit(smem_u32(&bars[B_EMPTY + keys.slot]));
+          tc_commit(smem_u32(&bars[B_S + buffer]));
         }
         __syncwarp();
-        r.step(RING);
-        ok = mbar_wait_warp(smem_u32(&bars[B_P]), (uint32_t)count & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
+      };
+      scores(r, count & 1);
+      for (int u = w.from; u < w.to && ok; ++u, ++count) {
+        r.step(RING);  // to this step's values
+        tc_ring next = r;
+        next.step(RING);
+        if (u + 1 < w.to) scores(next, (count + 1) & 1);
+        ok = ok && mbar_wait_warp(smem_u32(&bars[B_P + (count & 1)]), (uint32_t)(count >> 1) & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
         ok = ok && mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
         if (!ok) break;
         tc_fence_after();
         if (tc_elect()) {
+          const uint64_t b_desc = smem_desc_sw128_mn(ring_addr + (uint32_t)r.slot * STEP, ATOM);
 #pragma unroll
-          for (int kb2 = 0; kb2 < 2; ++kb2) {
-            const uint64_t b_desc = smem_desc_sw128_mn(ring_addr + (uint32_t)r.slot * OPERAND + kb2 * NKB * V_ATOM, V_ATOM);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ts(tmem + O_COL, tmem + kb2 * 32 + k * 8, b_desc + (uint64_t)(k * 2048 >> 4), sh::IDESC_PV, (uint32_t)(j > w.first || (kb2 | k) != 0));
-          }
+          for (int k = 0; k < 4; ++k)
+            mma_ts(tmem + O_COL, tmem + (uint32_t)((count & 1) * PR_STEP) + k * 8, b_desc + (uint64_t)(k * 2048 >> 4), sh::IDESC_PV, (uint32_t)(u > w.from || k != 0));
           tc_commit(smem_u32(&bars[B_EMPTY + r.slot]));
-          if (j + 1 == w.last) tc_commit(smem_u32(&bars[B_O]));
+          tc_commit(smem_u32(&bars[B_V]));
+          if (u + 1 == w.to) tc_commit(smem_u32(&bars[B_O]));
         }
         __syncwarp();
-        r.step(RING);
+        r = next;
       }
     }
     if (!ok) {  // (lets the softmax warps leave, without results)
@@ -397,15 +403,16 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         *failed = 1;
         __threadfence_block();
         tc_commit(smem_u32(&bars[B_S]));
+        tc_commit(smem_u32(&bars[B_S + 1]));
+        tc_commit(smem_u32(&bars[B_V]));
         tc_commit(smem_u32(&bars[B_O]));
       }
       __syncwarp();
     }
   } else {
-    // ---- softmax: a thread owns half the keys of a row, its warp and the one four further on 32 rows
-    const int quad = warp & 3, half = warp >> 2, in_tile = quad * 32 + lane;
-    const uint32_t s_at = tmem + ((uint32_t)(quad * 32) << 16), o_at = s_at + O_COL + (uint32_t)(half * (HD / 2));
-    auto meet = [&]() { bar_sync(2 + quad, 64); };
+    // ---- softmax: a thread owns a row
+    const int in_tile = warp * 32 + lane;
+    const uint32_t row_at = tmem + ((uint32_t)(warp * 32) << 16), o_at = row_at + O_COL;
     bool go = true;
     int count = 0;
     run w;
@@ -414,7 +421,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
     const int warp_limit = __shfl_sync(0xffffffffu, limit, 0);  // (what the warp's first row sees)
     const bool all_there = __all_sync(0xffffffffu, r < rows), whole = !SPLIT || w.last - w.first == w.all;
     const float f = a.row_stats[(size_t)w.unit * a.r_pad + r].x;
-    if (n) bar_sync(1, 32 * PR_SOFT_WARPS);  // (the run before has read s_half and s_bad)
+    if (n) bar_sync(1, 32 * PR_SOFT_WARPS);  // (the run before has read s_bad)
     if (tid < 4) s_bad[tid] = 0x7fffffff;
     bar_sync(1, 32 * PR_SOFT_WARPS);
     // the first row of no numbers among those this item sees
@@ -427,55 +434,47 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
       }
     }
     float less = 0.f, high = -INFINITY, sum = 0.f;  // minus the maximum (0 while there is none); 8 above it, as the products give scores
-    for (int j = w.first; j < w.last; ++j, ++count) {
-      const bool ok = mbar_wait(smem_u32(&bars[B_S]), (uint32_t)count & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
+    for (int u = w.from; u < w.to; ++u, ++count) {
+      const bool ok = mbar_wait(smem_u32(&bars[B_S + (count & 1)]), (uint32_t)(count >> 1) & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
       tc_fence_after();
       go = __all_sync(0xffffffffu, ok && *failed == 0);
-      const int left = limit - j * PR_KEYS - half * 64;  // keys of the half tile that the row sees
-      const bool ragged = !all_there || warp_limit < (j + 1) * PR_KEYS;
+      if (!go) break;
+      const uint32_t s_at = row_at + (uint32_t)((count & 1) * PR_STEP);
+      const int left = limit - u * PR_STEP;  // keys of the step that the row sees
+      const bool ragged = !all_there || warp_limit < (u + 1) * PR_STEP;
       uint32_t pw[32];
       float top, part;
-      auto tile = [&]() {
-        top = -INFINITY;
-        part = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t s[16];
-          ld_32x16(s_at + (uint32_t)(half * 64 + c * 16), s);
-          tc_wait_ld();
+      auto step = [&]() {
+        float t0 = -INFINITY, t1 = -INFINITY, a0 = 0.f, a1 = 0.f;
+        uint32_t s[2][32];
+        auto half = [&](uint32_t (&x)[32], int c) {
           if (ragged) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (c * 16 + e >= left) s[e] = 0xff800000u;
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= left) x[e] = 0xff800000u;
           }
-          float t0 = -INFINITY, t1 = -INFINITY, a0 = 0.f, a1 = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float s0 = __uint_as_float(s[e]), s1 = __uint_as_float(s[e + 1]);
+          for (int e = 0; e < 32; e += 2) {
+            const float s0 = __uint_as_float(x[e]), s1 = __uint_as_float(x[e + 1]);
             t0 = fmaxf(t0, s0);
             t1 = fmaxf(t1, s1);
             const float e0 = ex2(fmaf(s0, f, less)), e1 = ex2(fmaf(s1, f, less));
             a0 += e0;
             a1 += e1;
-            pw[c * 8 + e / 2] = pack2<__half>(e0, e1);
+            pw[c * 16 + e / 2] = pack2<__half>(e0, e1);
           }
-          top = fmaxf(top, fmaxf(t0, t1));
-          part += a0 + a1;
-        }
+        };
+        tc_ld_32x32(s_at, s[0]);
+        tc_wait_ld();
+        tc_ld_32x32(s_at + 32, s[1]);  // (on its way under the first half's exponentials)
+        half(s[0], 0);
+        tc_wait_ld();
+        half(s[1], 1);
+        top = fmaxf(t0, t1);
+        part = a0 + a1;
       };
-      tile();
-      const int mine = (__any_sync(0xffffffffu, top > high) ? 1 : 0) | (go ? 0 : 2);
-      if (lane == 0) s_raise[count & 1][warp] = mine;
-      meet();  // (both halves of the rows' scores are read: probabilities may take their place)
-      const int either = mine | s_raise[count & 1][warp ^ 4];
-      if (either & 2) {  // (the pair leaves together: its barriers count both)
-        go = false;
-        break;
-      }
-      if (either) {
-        s_half[half][in_tile] = top;
-        meet();
-        top = fmaxf(top, s_half[half ^ 1][in_tile]);
+      step();
+      if (__any_sync(0xffffffffu, top > high)) {
         const bool none = high == -INFINITY;
         float now = top * f;
         if (!none) now = fmaxf(now, -less);
@@ -483,9 +482,14 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         less = now == -INFINITY ? 0.f : -now;
         high = (now + 8.f) / f;
         sum *= k;
-        if (j > w.first) {
+        if (u > w.from) {
+          // the output as the product before left it (this step's waits for this warp's probabilities)
+          const bool done = mbar_wait(smem_u32(&bars[B_V]), (uint32_t)(count - 1) & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
+          tc_fence_after();
+          go = __all_sync(0xffffffffu, done && *failed == 0);
+          if (!go) break;
 #pragma unroll 1
-          for (int c = 0; c < HD / 2; c += 32) {
+          for (int c = 0; c < HD; c += 32) {
             uint32_t x[32];
             tc_ld_32x32(o_at + (uint32_t)c, x);
             tc_wait_ld();
@@ -494,25 +498,22 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
             st_32x32(o_at + (uint32_t)c, x);
           }
         }
-        tile();
-        meet();
+        step();
       }
       sum += part;
-      st_32x32(s_at + (uint32_t)(half * 32), pw);
+      st_32x32(s_at, pw);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bars[B_P]));
+      if (lane == 0) mbar_arrive(smem_u32(&bars[B_P + (count & 1)]));
     }
-    s_half[half][in_tile] = sum;
-    bar_sync(1, 32 * PR_SOFT_WARPS);  // (sums, s_bad)
-    sum = s_half[0][in_tile] + s_half[1][in_tile];
+    bar_sync(1, 32 * PR_SOFT_WARPS);  // (s_bad)
     if (w.all) {
       const bool ok = go && mbar_wait(smem_u32(&bars[B_O]), (uint32_t)n & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
       tc_fence_after();
       go = __all_sync(0xffffffffu, ok && *failed == 0);
     }
-    // (all eight warps go on together, or none: the barriers of the next run count them)
+    // (all warps go on together, or none: the barriers of the next run count them)
     if constexpr (SPLIT) {
       if (!go && lane == 0) *gave_up = 1;
       bar_sync(1, 32 * PR_SOFT_WARPS);
@@ -521,16 +522,16 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
     if (!go) break;
     if (whole) {
       const float rl = limit ? 1.f / sum : 0.f;
-      T* out = reinterpret_cast<T*>(p.out) + ((size_t)w.seq * p.m + i) * p.ld_out + (w.kvh * group + r % group) * HD + half * (HD / 2);
+      T* out = reinterpret_cast<T*>(p.out) + ((size_t)w.seq * p.m + i) * p.ld_out + (w.kvh * group + r % group) * HD;
 #pragma unroll 1
-      for (int c = 0; c < HD / 2; c += 32) {
+      for (int c = 0; c < HD; c += 32) {
         uint32_t x[32];
         if (w.all) {
           tc_ld_32x32(o_at + (uint32_t)c, x);
           tc_wait_ld();
         }
         if (r < rows) {
-          const bool none = limit && s_bad[(half * (HD / 2) + c) / p.c.bs] < limit;
+          const bool none = limit && s_bad[c / p.c.bs] < limit;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float y[8];
@@ -540,19 +541,19 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
           }
         }
       }
-      if (p.weights && r < rows && half == 0) a.row_stats[(size_t)w.unit * a.r_pad + r].y = limit ? log2f(sum) - less : INFINITY;
+      if (p.weights && r < rows) a.row_stats[(size_t)w.unit * a.r_pad + r].y = limit ? log2f(sum) - less : INFINITY;
     } else {
       const size_t place = ((size_t)blockIdx.x * 2 + (w.first == 0)) * PR_ROWS + in_tile;
-      float* to = a.part_o + place * HD + half * (HD / 2);
+      float* to = a.part_o + place * HD;
 #pragma unroll 1
-      for (int c = 0; c < HD / 2; c += 32) {
+      for (int c = 0; c < HD; c += 32) {
         uint32_t x[32];
         tc_ld_32x32(o_at + (uint32_t)c, x);
         tc_wait_ld();
 #pragma unroll
         for (int q = 0; q < 8; ++q) reinterpret_cast<uint4*>(to + c)[q] = make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
       }
-      if (half == 0) a.part_ml[place] = make_float2(high == -INFINITY ? -INFINITY : -less, sum);
+      a.part_ml[place] = make_float2(high == -INFINITY ? -INFINITY : -less, sum);
     }
     tc_fence_before();  // (the accumulator is read: the next run's products come behind this thread's arrival)
     }
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(256) prompt_add_kernel(const prompt_args a, in
 // accumulators: one tile's exponentials run under the next one's product.
 constexpr int W_KEYS = 0, W_FULL = 1, W_EMPTY = W_FULL + 2, W_S = W_EMPTY + 2, W_FREE = W_S + 2, W_COUNT = W_FREE + 2;
 template <int HD>
-__global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const prompt_args a,
+__global__ void __launch_bounds__(PW_THREADS, 2) prompt_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const prompt_args a,
                                                                        int key_blocks, int units) {
   using sh = prompt_shape<HD>;
   constexpr int NKB = sh::NKB;
@@ -672,12 +673,12 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
       mbar_init(smem_u32(&bars[W_FULL + i]), 1);
       mbar_init(smem_u32(&bars[W_EMPTY + i]), 1);
       mbar_init(smem_u32(&bars[W_S + i]), 1);
-      mbar_init(smem_u32(&bars[W_FREE + i]), PR_SOFT_WARPS);
+      mbar_init(smem_u32(&bars[W_FREE + i]), PW_SOFT_WARPS);
     }
     *failed = 0;
     fence_mbar_init();
   }
-  if (warp == PR_SOFT_WARPS + 1) tmem_alloc(tmem_slot, TMEM_COLS);
+  if (warp == PW_SOFT_WARPS + 1) tmem_alloc(tmem_slot, TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -690,7 +691,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
   const int first = from_tile + (int)((long long)all_tiles * segment / a.segments);
   const int n_tiles = from_tile + (int)((long long)all_tiles * (segment + 1) / a.segments) - first;
 
-  if (warp == PR_SOFT_WARPS) {
+  if (warp == PW_SOFT_WARPS) {
     if (n_tiles > 0 && tc_elect()) {
       mbar_arrive_expect_tx(smem_u32(&bars[W_KEYS]), OPERAND);
       for (int kb = 0; kb < NKB; ++kb) tma_load_3d(k_addr + kb * sh::BLOCK, &map_k, kb * 64, j0, unit, smem_u32(&bars[W_KEYS]));
@@ -705,7 +706,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
       }
     }
     __syncwarp();
-  } else if (warp == PR_SOFT_WARPS + 1) {
+  } else if (warp == PW_SOFT_WARPS + 1) {
     bool ok = n_tiles > 0 && mbar_wait_warp(smem_u32(&bars[W_KEYS]), 0, a.err, DEV_ERR_FULL_WAIT, HEED);
     tc_ring r;
     for (int it = 0; it < n_tiles && ok; ++it, r.step(2)) {
@@ -782,7 +783,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
       if (lane == 0) mbar_arrive(smem_u32(&bars[W_FREE + r.slot]));
     }
     if (half) s_total[quad * 32 + lane] = total;
-    bar_sync(1, 32 * PR_SOFT_WARPS);
+    bar_sync(1, 32 * PW_SOFT_WARPS);
     total += s_total[quad * 32 + lane];
     if (go && j < seen && !half) {
       if (a.segments > 1) a.part_w[((size_t)segment * units + unit) * a.t_pad + j] = total;
@@ -793,7 +794,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_weights_kernel(const __g
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == PR_SOFT_WARPS + 1) {
+  if (warp == PW_SOFT_WARPS + 1) {
     __syncwarp();
     tc_fence_after();
     tmem_free(tmem, TMEM_COLS);
@@ -871,14 +872,15 @@ int launch_prompt(const prompt_args& a, cudaStream_t stream) {
   using sh = prompt_shape<HD>;
   const cache4_attention_params& p = a.p;
   const int units = p.c.n_seqs * p.c.n_kv, key_blocks = a.t_pad / PR_KEYS, row_blocks = a.r_pad / PR_ROWS;
-  CUtensorMap map_q, map_k, map_v;
+  CUtensorMap map_q, map_k, map_v, map_k128;
   {
     const uint64_t rows_q[3] = {(uint64_t)HD, (uint64_t)a.r_pad, (uint64_t)units}, step_q[2] = {(uint64_t)HD * 2, (uint64_t)a.r_pad * HD * 2};
     const uint64_t rows_k[3] = {(uint64_t)HD, (uint64_t)a.t_pad, (uint64_t)units}, step_k[2] = {(uint64_t)HD * 2, (uint64_t)a.t_pad * HD * 2};
-    const uint32_t box[3] = {64, 128, 1}, box_v[3] = {64, 64, 1};
+    const uint32_t box[3] = {64, 128, 1}, box_step[3] = {64, PR_STEP, 1};
     int rc = tc_encode_map(&map_q, a.q_half, 3, rows_q, step_q, box);
-    if (!rc) rc = tc_encode_map(&map_k, a.k_half, 3, rows_k, step_k, box);
-    if (!rc) rc = tc_encode_map(&map_v, a.v_half, 3, rows_k, step_k, box_v);
+    if (!rc) rc = tc_encode_map(&map_k, a.k_half, 3, rows_k, step_k, box_step);
+    if (!rc) rc = tc_encode_map(&map_v, a.v_half, 3, rows_k, step_k, box_step);
+    if (!rc && p.weights) rc = tc_encode_map(&map_k128, a.k_half, 3, rows_k, step_k, box);
     if (rc) return rc;
   }
   prompt_expand_kernel<T, HD><<<(unsigned)units * (key_blocks + row_blocks) + (a.ctas ? 1 : 0), 256, 0, stream>>>(a, key_blocks, row_blocks);
@@ -892,7 +894,7 @@ int launch_prompt(const prompt_args& a, cudaStream_t stream) {
     constexpr uint32_t SMEM_W = 3 * sh::OPERAND + 4 * 128 * sizeof(float2) + 1024 + 256;
     rc = allow_smem(prompt_weights_kernel<HD>, SMEM_W, done_w);
     if (rc) return rc;
-    LCU_CUDA(launch_after(prompt_weights_kernel<HD>, dim3((unsigned)units * key_blocks * a.segments), dim3(PR_THREADS), SMEM_W, stream, map_q, map_k, a, key_blocks, units));
+    LCU_CUDA(launch_after(prompt_weights_kernel<HD>, dim3((unsigned)units * key_blocks * a.segments), dim3(PW_THREADS), SMEM_W, stream, map_q, map_k128, a, key_blocks, units));
     if (a.segments > 1) LCU_CUDA(launch_after(prompt_add_kernel, dim3((p.max_len + 255) / 256, (unsigned)units), dim3(256), 0, stream, a, units));
   }
   return LCU_OK;
