@@ -5,11 +5,15 @@
 // of the call - 4 bytes moved per value and product, against codes expanded again for each 128 x 128 tile at a cost close to the tile's own
 // exponentials.  bfloat16 queries become halves too, each row by a power of two, so that both types share everything behind.
 //
-// One CTA per (sequence, key/value head, 128 rows), two CTAs per SM: while one's scores are exponentiated, the other's products run.
-// Scores lie in tensor memory; a thread owns a row, reads 32 keys at a time and keeps the running maximum and the sum; probabilities
-// go back to tensor memory, over the scores, as halves: the A operand of the product with the values, whose accumulator stays in tensor
-// memory.  A maximum is raised only when a score passes it by 8 (powers of two), so that the exponentials of a tile are formed with
-// the old one while its own maximum is looked for; only where a row fails that test is its warp's tile done again and the output rescaled.
+// One CTA per (sequence, key/value head, 128 rows), two CTAs per SM, in steps of 64 keys.  Scores lie in two buffers of tensor memory: those of
+// the next step are formed under this step's exponentials (in one buffer, steps of 128 keys, score - exponential - product followed one
+// another: 2000 rows of 32 heads behind 6000 rows of 8, timed in turn, took 294 us instead of 255, 4000 rows 190 instead of 162).  Three accumulators' columns
+// for two CTAs are what tensor memory holds; narrower products of the scores read their queries from shared memory more often, 1.5 x the time.
+// A thread owns a row, reads 32 keys at a time and keeps the running maximum and the sum; probabilities go back to tensor memory, over the
+// scores, as halves: the A operand of the product with the values, whose accumulator stays in tensor memory.  A maximum is raised only
+// when a score passes it by 8 (powers of two), so that the exponentials of a step are formed with the old one while its own maximum is
+// looked for; only where a row fails that test is its warp's step done again and the output rescaled, once the product before is done.
+// Exponentials (16 a cycle and SM) and products are both busy 59 % of the time that a CTA is there.
 //
 // Weights: once maxima and sums are known, a second kernel forms the scores the other way round - a thread owns a cached row - and adds
 // e^(s - max) / sum over all rows in their order.
@@ -177,6 +181,28 @@ __device__ __forceinline__ float ex2(float y) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
   return r;
 }
+// two binary32 numbers as one operand: half as many instructions for the exponentials' arguments and sums
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float2 both_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -192,6 +218,14 @@ __device__ __forceinline__ void st_32x32(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
       "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -445,7 +479,9 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
       uint32_t pw[32];
       float top, part;
       auto step = [&]() {
-        float t0 = -INFINITY, t1 = -INFINITY, a0 = 0.f, a1 = 0.f;
+        float t0 = -INFINITY, t1 = -INFINITY;
+        uint64_t sums = 0;
+        const uint64_t factor = pair_of(f, f), minus = pair_of(less, less);
         uint32_t s[2][32];
         auto half = [&](uint32_t (&x)[32], int c) {
           if (ragged) {
@@ -455,12 +491,11 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
           }
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float s0 = __uint_as_float(x[e]), s1 = __uint_as_float(x[e + 1]);
-            t0 = fmaxf(t0, s0);
-            t1 = fmaxf(t1, s1);
-            const float e0 = ex2(fmaf(s0, f, less)), e1 = ex2(fmaf(s1, f, less));
-            a0 += e0;
-            a1 += e1;
+            t0 = fmaxf(t0, __uint_as_float(x[e]));
+            t1 = fmaxf(t1, __uint_as_float(x[e + 1]));
+            const float2 y = both_of(fma_pair(pair_of(x[e], x[e + 1]), factor, minus));
+            const float e0 = ex2(y.x), e1 = ex2(y.y);
+            sums = add_pair(sums, pair_of(e0, e1));
             pw[c * 16 + e / 2] = pack2<__half>(e0, e1);
           }
         };
@@ -471,7 +506,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         tc_wait_ld();
         half(s[1], 1);
         top = fmaxf(t0, t1);
-        part = a0 + a1;
+        part = both_of(sums).x + both_of(sums).y;
       };
       step();
       if (__any_sync(0xffffffffu, top > high)) {
@@ -754,18 +789,20 @@ __global__ void __launch_bounds__(PW_THREADS, 2) prompt_weights_kernel(const __g
       const float4* st = reinterpret_cast<const float4*>(smem + 3 * OPERAND + (size_t)(it & 3) * STATS) + half * 32;
       float part = 0.f;
       auto tile = [&](auto checked) {  // (checked: some of the keys, or of the rows, are none that count)
+        uint32_t both[2][16];
+        ld_32x16(s_at, both[0]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s[32];
-          tc_ld_32x32(s_at + (uint32_t)(c * 32), s);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t(&s)[16] = both[c & 1];
           tc_wait_ld();
+          if (c < 3) ld_32x16(s_at + (uint32_t)(c * 16 + 16), both[(c + 1) & 1]);  // (on its way under these exponentials)
           float a0 = 0.f, a1 = 0.f;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float4 fl = st[c * 16 + e / 2];
+          for (int e = 0; e < 16; e += 2) {
+            const float4 fl = st[c * 8 + e / 2];
             float e0 = ex2(fmaf(__uint_as_float(s[e]), fl.x, -fl.y)), e1 = ex2(fmaf(__uint_as_float(s[e + 1]), fl.z, -fl.w));
             if constexpr (decltype(checked)::value) {
-              const int row = q0 + half * 64 + c * 32 + e;
+              const int row = q0 + half * 64 + c * 16 + e;
               if (row < from || row >= rows) e0 = 0.f;
               if (row + 1 < from || row + 1 >= rows) e1 = 0.f;
             }
@@ -804,8 +841,8 @@ __global__ void __launch_bounds__(PW_THREADS, 2) prompt_weights_kernel(const __g
 // ------------------------------------------------------------------ host
 // How the work is shared, from the sizes as the host knows them.  A CTA per item leaves slots idle where items are few or their last wave is
 // half full; an equal share of all tiles per CTA costs each the start of another run, the partial sums of two and their join, about what
-// eight tiles take.  8 key heads x 4 queries each: 8 rows behind 30000 (16 tiles of 128 rows at once) 510 us per item, 82 shared; 2000 rows
-// behind 6000 (504 items of 47 to 63 tiles, 296 slots) 414 us per item, 464 shared.
+// eight tiles take.  8 key heads x 4 queries each: 50 rows behind 30000 481 us per item, 96 shared; 300 behind 4000 89 and 57; 500 behind
+// 2000 53 and 55; 2000 behind 6000 (504 items of 47 to 63 tiles, 296 slots) 244 and 292.
 struct prompt_plan {
   int ctas, segments;
   prompt_plan(int n_seqs, int m, int n_heads, int n_kv, int max_len) {
