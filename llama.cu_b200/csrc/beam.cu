@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
   __shared__ double s_sum[8];
   __shared__ uint64_t s_threshold;
   __shared__ int s_count;
+  pdl_launch_dependents();
   const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n_out = a.p.n_out, v0 = chunk * BEAM_CHUNK;
   const T* x = reinterpret_cast<const T*>(a.p.logits) + (size_t)row * a.p.ld;
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
   __shared__ int s_count;
   extern __shared__ scored cand_scored[];
   const int group = blockIdx.x, tid = threadIdx.x, n_out = a.p.n_out;
+  pdl_launch_dependents();  // (the reordering of the caches, where that comes next)
   pdl_wait();
   if (tid == 0) {
     s_count = 0;

@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
   __shared__ int2 s_warp[32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_left;
+  pdl_launch_dependents();  // (the kernels that move rows start, and wait for the list)
   const int sh = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = min(a.lengths[sh / a.n_kv], a.ctx);
   int* kept = a.kept + (size_t)sh * a.keep;
@@ -288,6 +289,7 @@ __device__ __forceinline__ size_t piece_bytes(const plane& p, int ctx) {
 constexpr size_t REORDER_CTA_BYTES = 16384;
 __global__ void __launch_bounds__(256) reorder_copy_kernel(const reorder_args a, int chunks) {
   const plane p = a.planes[blockIdx.y];
+  pdl_wait();
   const int chunk = blockIdx.x % chunks, sh = blockIdx.x / chunks, seq = sh / a.n_kv, head = sh % a.n_kv;
   const int parent = a.parents[seq];
   if (parent < 0 || parent >= a.beams) return;
@@ -340,6 +342,7 @@ __device__ __forceinline__ void permute_run(const reorder_args& a, const plane& 
 template <int B>
 __global__ void __launch_bounds__(256) reorder_permute_kernel(const reorder_args a, int chunks) {
   const plane p = a.planes[blockIdx.y];
+  pdl_wait();
   const int chunk = blockIdx.x % chunks, gh = blockIdx.x / chunks, group = gh / a.n_kv, head = gh % a.n_kv;
   const size_t head_bytes = (size_t)a.ctx * p.row_bytes, lo = (size_t)chunk * REORDER_CTA_BYTES / 4, hi = min(head_bytes, lo + REORDER_CTA_BYTES / 4);
   if (lo >= hi) return;
@@ -452,16 +455,14 @@ int launch_cache_reorder(const reorder_params& p, cudaStream_t stream) {
   if (n_away) {
     const size_t chunks = ceil_div(widest_away * p.ctx, REORDER_CTA_BYTES), ctas = chunks * heads * p.beams;
     LCU_REQUIRE(ctas < (1ull << 31), "cache_reorder: planes are too large");
-    reorder_copy_kernel<<<dim3((unsigned)ctas, n_away), 256, 0, stream>>>(away, (int)chunks);
+    LCU_CUDA(launch_after(reorder_copy_kernel, dim3((unsigned)ctas, n_away), dim3(256), 0, stream, away, (int)chunks));
   }
   if (n_here) {
     const size_t chunks = ceil_div(widest_here * p.ctx, REORDER_CTA_BYTES / 4), ctas = chunks * heads;
     LCU_REQUIRE(ctas < (1ull << 31), "cache_reorder: planes are too large");
     const dim3 grid((unsigned)ctas, n_here);
-    if (p.beams <= 4) reorder_permute_kernel<4><<<grid, 256, 0, stream>>>(here, (int)chunks);
-    else if (p.beams <= 8) reorder_permute_kernel<8><<<grid, 256, 0, stream>>>(here, (int)chunks);
-    else if (p.beams <= 16) reorder_permute_kernel<16><<<grid, 256, 0, stream>>>(here, (int)chunks);
-    else reorder_permute_kernel<32><<<grid, 256, 0, stream>>>(here, (int)chunks);
+    auto* kernel = p.beams <= 4 ? reorder_permute_kernel<4> : p.beams <= 8 ? reorder_permute_kernel<8> : p.beams <= 16 ? reorder_permute_kernel<16> : reorder_permute_kernel<32>;
+    LCU_CUDA(launch_after(kernel, grid, dim3(256), 0, stream, here, (int)chunks));
   }
   LCU_CUDA(cudaGetLastError());
   return LCU_OK;
