@@ -55,28 +55,39 @@ __device__ __forceinline__ int2 block_exclusive(int2 v, int2* s_warp) {
   return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
 }
 
-// One CTA per (sequence, head): the `want` largest of the weights before the latest rows, by digits from the top - a histogram of 2048
-// bins, the bin in which the want-th largest lies, the next digit among that bin's weights - then one pass in row order that writes
-// the rows above the threshold and as many of those at it as are left to take, lowest rows first.  A warp owns a run of rows; up to 16
-// weights of a thread (16384 of a CTA) stay in registers, so that they are read once: 32 heads of 16000 rows 28 -> 18 us with cold caches.
-template <int K>
+// int2 of the same place in shared memory of another CTA of the cluster
+__device__ __forceinline__ int2 remote_pair(const void* at, uint32_t rank) {
+  int2 v;
+  asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(mapa(smem_u32(at), rank)) : "memory");
+  return v;
+}
+
+// One cluster of CL CTAs per (sequence, head): the `want` largest of the weights before the latest rows, by digits from the top - a histogram of
+// 2048 bins, the bin in which the want-th largest lies, the next digit among that bin's weights - then one pass in row order that
+// writes the rows above the threshold and as many of those at it as are left to take, lowest rows first.  A warp owns a run of rows; up
+// to 16 weights of a thread stay in registers, so that they are read once.  Bound by the chain of three histograms and their sums over the
+// bins.  Four CTAs share a head where rows are many: every CTA adds up the four histograms for itself and finds the same bin, and a CTA's
+// places begin behind the counts of those before it.  One CTA / four, us with the rows' move: 8 heads x 16000 rows 17.7 / 13.9, 32 heads (to
+// 8001) 61.0 / 56.4, 64 heads 23.2 / 30.1; 32 heads x 5000 13.3 / 15.9; 8 heads x 60000 75.6 / 21.4, 64 heads 101 / 43.
+template <int K, int CL>
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_args a) {
-  __shared__ int hist[SEL_BINS];
+  __shared__ __align__(8) int hist_of[CL > 1 ? 2 : 1][SEL_BINS];  // (two in turn: others read the last one while the next is filled)
+  __shared__ int2 s_total;
   __shared__ int2 s_warp[32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_left;
   pdl_launch_dependents();  // (the kernels that move rows start, and wait for the list)
-  const int sh = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int sh = blockIdx.x / CL, rank = blockIdx.x % CL, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = min(a.lengths[sh / a.n_kv], a.ctx);
   int* kept = a.kept + (size_t)sh * a.keep;
   if (len <= a.keep) {
-    for (int i = tid; i < a.keep; i += SEL_THREADS) kept[i] = i < len ? i : -1;
-    return;
+    for (int i = rank * SEL_THREADS + tid; i < a.keep; i += CL * SEL_THREADS) kept[i] = i < len ? i : -1;
+    return;  // (the whole cluster)
   }
   const int old = len - a.recent, want = a.keep - a.recent;  // (len > keep: want < old)
   const float* w = a.weights + (size_t)sh * a.ctx;
   // the rows of a warp; a thread's are 32 apart
-  const int run = (old + SEL_THREADS - 1) / SEL_THREADS * 32, from = warp * run, to = min(old, from + run);
+  const int run = (old + CL * SEL_THREADS - 1) / (CL * SEL_THREADS) * 32, from = (rank * (SEL_THREADS / 32) + warp) * run, to = min(old, from + run);
   uint32_t held[K > 0 ? K : 1];
   if constexpr (K > 0) {
 #pragma unroll
@@ -94,10 +105,17 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
         f(from + k * 32 + lane, held[k], from + k * 32 + lane < to);
       }
     } else {
-      for (int i0 = from; i0 < to; i0 += 32) f(i0 + lane, i0 + lane < to ? weight_key(w[i0 + lane]) : 0u, i0 + lane < to);
+      for (int i0 = from; i0 < to; i0 += 4 * 32) {
+        float next[4];  // (requested together)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) next[k] = i0 + k * 32 + lane < to ? w[i0 + k * 32 + lane] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i0 + k * 32 < to) f(i0 + k * 32 + lane, weight_key(next[k]), i0 + k * 32 + lane < to);
+      }
     }
   };
-  for (int i = tid; i < a.recent; i += SEL_THREADS) kept[want + i] = old + i;
+  for (int i = rank * SEL_THREADS + tid; i < a.recent; i += CL * SEL_THREADS) kept[want + i] = old + i;
   if (want == 0) return;
   if (tid == 0) {
     s_prefix = 0;
@@ -106,6 +124,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    int* hist = hist_of[CL > 1 ? pass & 1 : 0];
     for (int b = tid; b < SEL_BINS; b += SEL_THREADS) hist[b] = 0;
     __syncthreads();
     const uint32_t prefix = s_prefix;
@@ -122,9 +141,22 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
         atomicAdd(&hist[digit], 1);
       }
     });
-    __syncthreads();
+    if constexpr (CL > 1) cluster_sync();
+    else __syncthreads();
     // bins from the top, two per thread
-    const int hi = SEL_BINS - 1 - 2 * tid, c0 = hist[hi], c1 = hist[hi - 1];
+    const int hi = SEL_BINS - 1 - 2 * tid;
+    int c0 = 0, c1 = 0;
+    if constexpr (CL > 1) {
+#pragma unroll
+      for (int r = 0; r < CL; ++r) {
+        const int2 c = remote_pair(&hist[hi - 1], r);
+        c0 += c.y;
+        c1 += c.x;
+      }
+    } else {
+      c0 = hist[hi];
+      c1 = hist[hi - 1];
+    }
     const int before = block_exclusive(make_int2(c0 + c1, 0), s_warp).x;
     if (before < left && left <= before + c0 + c1) {
       const bool first = left <= before + c0;
@@ -142,6 +174,19 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const select_
     equal += __popc(__ballot_sync(0xffffffffu, there && key == threshold));
   });
   int2 base = block_exclusive(lane == 0 ? make_int2(above, equal) : make_int2(0, 0), s_warp);
+  if constexpr (CL > 1) {
+    if (tid == SEL_THREADS - 1) s_total = base;  // (lane 31 adds nothing: the sums of all warps)
+    cluster_sync();
+#pragma unroll
+    for (int r = 0; r + 1 < CL; ++r) {
+      const int2 c = remote_pair(&s_total, r);
+      if (r < rank) {
+        base.x += c.x;
+        base.y += c.y;
+      }
+    }
+    cluster_sync();  // (nothing of this CTA's is read any more)
+  }
   base.x = __shfl_sync(0xffffffffu, base.x, 0);
   base.y = __shfl_sync(0xffffffffu, base.y, 0);
   each([&](int i, uint32_t key, bool there) {
@@ -402,9 +447,24 @@ int launch_cache_evict(const evict_params& p, cudaStream_t stream) {
   LCU_REQUIRE((long long)heads * chunks < (1ll << 31), "cache_evict: planes are too large");
   if (int rc_dev = need_device()) return rc_dev;
   const select_args sel{p.weights, p.kept, p.lengths, p.n_kv, p.ctx, p.keep, p.recent};
-  if (p.ctx <= 4 * SEL_THREADS) evict_select_kernel<4><<<heads, SEL_THREADS, 0, stream>>>(sel);
-  else if (p.ctx <= 16 * SEL_THREADS) evict_select_kernel<16><<<heads, SEL_THREADS, 0, stream>>>(sel);
-  else evict_select_kernel<0><<<heads, SEL_THREADS, 0, stream>>>(sel);
+  if (p.ctx <= 4 * SEL_THREADS) {
+    evict_select_kernel<4, 1><<<heads, SEL_THREADS, 0, stream>>>(sel);
+  } else if (p.ctx <= 8 * SEL_THREADS || (p.ctx <= 16 * SEL_THREADS && 4 * heads > 148)) {
+    evict_select_kernel<16, 1><<<heads, SEL_THREADS, 0, stream>>>(sel);
+  } else {
+    auto* kernel = p.ctx <= 16 * SEL_THREADS ? evict_select_kernel<4, 4> : p.ctx <= 64 * SEL_THREADS ? evict_select_kernel<16, 4> : evict_select_kernel<0, 4>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)heads * 4);
+    cfg.blockDim = dim3(SEL_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 4;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    LCU_CUDA(cudaLaunchKernelEx(&cfg, kernel, sel));
+  }
   if (n_away) {
     away.lengths_out = p.lengths_out;
     LCU_CUDA(launch_after(evict_gather_kernel, dim3((unsigned)(heads * chunks), n_away), dim3(256), 0, stream, away, rows, chunks));

@@ -470,7 +470,9 @@ def evict(lcu, dst, src, weights, lengths, ctx, dctx, keep, recent, lengths_out=
 @pytest.mark.parametrize("kind", ["ordinary", "equal", "steps", "odd"])
 @pytest.mark.parametrize("ctx,lengths,keep,recent", [
     (1, [1, 0], 1, 0), (2, [2, 1], 1, 1), (40, [40, 33, 7, -1], 16, 5), (300, [300, 299, 17], 16, 0), (300, [150, 300], 200, 200), (2048, [2048, 1500], 1024, 256),
-    (5000, [5000, 4097], 1, 0), (5000, [4999], 4998, 3), (70000, [70000], 33333, 100), (64, [64, 70], 64, 3)])
+    (5000, [5000, 4097], 1, 0), (5000, [4999], 4998, 3), (70000, [70000], 33333, 100), (64, [64, 70], 64, 3),
+    (4097, [4097, 1, 4000], 700, 699), (16384, [16384, 12000], 16383, 0), (16385, [16385, 3], 1, 1), (65536, [65536, 40000], 20000, 1), (5000, [5000, 4000, 100, -1] * 7, 1234, 99),
+    (17000, [17000, 16000] * 13, 16, 0)])
 def test_evict(lcu, kind, ctx, lengths, keep, recent):
     rng = np.random.default_rng(ctx + keep)
     seqs, kv = len(lengths), 3
