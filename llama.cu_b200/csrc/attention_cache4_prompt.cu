@@ -7,7 +7,7 @@
 //
 // One CTA per (sequence, key/value head, 128 rows), two CTAs per SM, in steps of 64 keys.  Scores lie in two buffers of tensor memory: those of
 // the next step are formed under this step's exponentials (in one buffer, steps of 128 keys, score - exponential - product followed one
-// another: 2000 rows of 32 heads behind 6000 rows of 8, timed in turn, took 294 us instead of 255, 4000 rows 190 instead of 162).  Three accumulators' columns
+// another: 2000 rows of 32 heads behind 6000 rows of 8, timed in turn, took 294 us instead of 264, 4000 rows 190 instead of 165).  Three accumulators' columns
 // for two CTAs are what tensor memory holds; narrower products of the scores read their queries from shared memory more often, 1.5 x the time.
 // A thread owns a row, reads 32 keys at a time and keeps the running maximum and the sum; probabilities go back to tensor memory, over the
 // scores, as halves: the A operand of the product with the values, whose accumulator stays in tensor memory.  A maximum is raised only
@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
     }
     __syncwarp();
   } else if (warp == PR_SOFT_WARPS + 1) {
-    // ---- products, in this order: S_0, S_1, O += P_0 V_0, S_2, O += P_1 V_1, ..: a step's scores are there when the step before is done, and
-    // only replace probabilities whose product comes before them
+    // ---- products, in this order: S_0, S_1, O += P_0 V_0, S_2, O += P_1 V_1, ..: a step's scores are formed under the exponentials of the step
+    // before, once the product of the probabilities that they replace is done
     tc_ring r;  // (keys and values in the loads' order: K_0, V_0, K_1, ..)
     run w;
     bool ok = true;
@@ -414,7 +414,10 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         r.step(RING);  // to this step's values
         tc_ring next = r;
         next.step(RING);
-        if (u + 1 < w.to) scores(next, (count + 1) & 1);
+        // (products of different shapes are not promised to run in the order of issue: what the next scores replace must have been read;
+        // left to that order, 2000 rows behind 6000 took 262 us instead of 271 in turn, others the same)
+        if (u > w.from) ok = ok && mbar_wait_warp(smem_u32(&bars[B_V]), (uint32_t)(count - 1) & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
+        if (ok && u + 1 < w.to) scores(next, (count + 1) & 1);
         ok = ok && mbar_wait_warp(smem_u32(&bars[B_P + (count & 1)]), (uint32_t)(count >> 1) & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
         ok = ok && mbar_wait_warp(smem_u32(&bars[B_FULL + r.slot]), r.phase, a.err, DEV_ERR_FULL_WAIT, HEED);
         if (!ok) break;
