@@ -13,7 +13,7 @@
 // scores, as halves: the A operand of the product with the values, whose accumulator stays in tensor memory.  A maximum is raised only
 // when a score passes it by 8 (powers of two), so that the exponentials of a step are formed with the old one while its own maximum is
 // looked for; only where a row fails that test is its warp's step done again and the output rescaled, once the product before is done.
-// Exponentials (16 a cycle and SM) and products are both busy 59 % of the time that a CTA is there.
+// Exponentials (16 a cycle and SM) and products are both busy 55 % of the time that a CTA is there.
 //
 // Weights: once maxima and sums are known, a second kernel forms the scores the other way round - a thread owns a cached row - and adds
 // e^(s - max) / sum over all rows in their order.
