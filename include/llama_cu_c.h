@@ -181,8 +181,10 @@ int lcu_cache_evict(void* const* dst_planes, const void* const* src_planes, cons
                     int keep, int recent, void* stream);
 /* Beam search, one step of n_groups groups of `beams` beams (1 to 32).  Row g * beams + b of logits (ld elements apart) belongs to beam b of
  * group g, whose score so far is scores[g][b].  The n_out (up to 64) best of scores[b] + log softmax(logits[b])[v] over beams and tokens,
- * best first: parents (b), tokens (v) and scores_out, [n_groups][n_out].  Compared in binary64; ties go to the lowest beam, then the larger
- * logit (where binary64 loses the difference), then the lowest token.  A NaN among logits counts as minus infinity; beams whose score is not finite, or whose logits have no finite maximum, offer all
+ * best first: parents (b), tokens (v) and scores_out, [n_groups][n_out].  Scores are formed and compared in binary64 from sums of
+ * exponentials that are good to 2^-18 of themselves (binary32 terms of logit - maximum, whatever the maximum): beams closer than that may change places.
+ * Ties go to the lowest beam, then the larger logit (where binary64 loses the difference), then the lowest token.  Finite logits of any size will do
+ * as masks.  A NaN among logits counts as minus infinity; beams whose score is not finite, or whose logits have no finite maximum, offer all
  * their tokens at minus infinity. */
 uint64_t lcu_beam_select_workspace(int n_groups, int beams, int n_vocab, int n_out);
 int lcu_beam_select(int32_t* parents_dev, int32_t* tokens_dev, float* scores_out_dev, const void* logits_dev, int ld, int dtype, const float* scores_dev,

@@ -98,10 +98,12 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_rows_kernel(const beam_args
   }
   double sum = 0.0;
   if (mx > -INFINITY) {
-    constexpr float LOG2E = 1.4426950408889634f;  // (2^-22 of a term, and 2^-24 of its distance from the maximum)
+    // The difference first: it is at most 0 and overflows to minus infinity at worst, the largest term is 1 whatever the maximum, and a term
+    // is off by 2^-22, and by 2.25 x 2^-24 of its distance from the maximum.
+    constexpr float LOG2E = 1.4426950408889634f;
     float part = 0.f;
 #pragma unroll
-    for (int i = 0; i < BEAM_ITEMS; ++i) part += ex2(fmaf(val[i], LOG2E, -mx * LOG2E));
+    for (int i = 0; i < BEAM_ITEMS; ++i) part += ex2((val[i] - mx) * LOG2E);
     sum = part;
   }
 #pragma unroll
@@ -144,10 +146,11 @@ __device__ __forceinline__ int beam_of(uint64_t place) { return (int)(place >> 5
 __device__ __forceinline__ int token_of(uint64_t place) { return (int)(place & 0xffffffu); }
 __device__ __forceinline__ bool better(const scored& a, const scored& b) { return a.order > b.order || (a.order == b.order && a.place < b.place); }
 
-// One CTA per group: log-sum-exp of every beam in 64 bits, then the n best of the chunks' candidates.  A thread owns chunks' lists, which are
+// One CTA per group: every beam's maximum and the logarithm of its sum (of the chunks' binary32 sums, in 64 bits), then the n best of the
+// chunks' candidates.  The two stay apart, so that a score is as good behind a maximum of 1e30 as behind one of 0.  A thread owns chunks' lists, which are
 // sorted: the heads of 64 groups of lists give a bound in the way of the first kernel, and lists are walked down to it.
 __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_args a, int most) {
-  __shared__ double lse[MAX_BEAMS], base[MAX_BEAMS];
+  __shared__ double top_logit[MAX_BEAMS], base[MAX_BEAMS];  // (base: score so far less the logarithm of the sum)
   __shared__ scored tops[BEAM_THREADS];  // (the largest of four threads' lists each; of every thread in the other way)
   __shared__ scored s_threshold;
   __shared__ int s_count;
@@ -173,8 +176,8 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
       const float s = a.p.scores[(size_t)group * a.p.beams + b];
       // a beam without a finite score, or whose logits have no finite maximum, offers its first tokens at minus infinity
       const bool fine = mx > -INFINITY && mx < INFINITY && s > -INFINITY && s < INFINITY;
-      lse[b] = (double)mx + log(sum);
-      base[b] = fine ? (double)s : -INFINITY;
+      top_logit[b] = mx;
+      base[b] = fine ? (double)s - log(sum) : -INFINITY;
     }
   }
   __syncthreads();
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_group_kernel(const beam_arg
     if (fine ? !k : list != b * a.chunks || e >= a.p.n_vocab) return scored{0, ~0ull};
     if (!fine) return scored{double_order(-INFINITY), (uint64_t)b << 56 | (uint32_t)e};
     const uint32_t logit = (uint32_t)(k >> 32);
-    return scored{double_order((double)order_float(logit) - lse[b] + base[b]), (uint64_t)b << 56 | (uint64_t)~logit << 24 | (uint32_t)~(uint32_t)k};
+    return scored{double_order(((double)order_float(logit) - top_logit[b]) + base[b]), (uint64_t)b << 56 | (uint64_t)~logit << 24 | (uint32_t)~(uint32_t)k};
   };
   scored top{0, ~0ull};
 #pragma unroll 4
