@@ -160,6 +160,8 @@ int lcu_cache4_read(void* k_out_dev, void* v_out_dev, const void* k_codes_dev, c
  * lcu_cache4_append): row i of sequence s sees rows 0 .. lengths[s] + i.  n_heads is a multiple of n_kv_heads; head h reads key/value head
  * h / (n_heads / n_kv_heads).  Scores are divided by sqrt(head_dim).  max_len: a bound on lengths[s] + m, at most ctx_len (rows beyond it are
  * not seen).  A row that sees nothing (a negative length) gives zeros.
+ * Scores, maxima, sums and accumulators are binary32.  Probabilities become halves for their product with the values: off by 2^-11 of themselves,
+ * or by 2^-32 of the row's largest where they are smaller than 2^-21 of it.
  * weights (NULL: not wanted), binary32 [n_seqs][n_kv_heads][ctx_len]: = beta * weights + the probabilities that the cached row received from
  * all m rows and the heads that read it, summed in a fixed order.  The call's own rows, from lengths[s] on, start from nothing, whatever
  * their entries held; with beta 0 all do.  Entries of rows that none sees stay as they are.  The workspace is lcu_attention_cache4_workspace bytes (0 where none is needed). */

@@ -45,7 +45,7 @@ struct prompt_args {
   int ctas;           // split: CTAs that share the tiles of all items (0: a CTA per item)
   int* prefix;        // split: [units * row blocks + 1] tiles of the items before each
   float* part_o;      // split: [ctas][2][128][hd] sums of runs of tiles that begin, or end, inside an item
-  float2* part_ml;    // split: [ctas][2][128] their rows' maxima (powers of two) and sums
+  float2* part_ml;    // split: [ctas][2][128] their rows' references (powers of two) and sums
   float* part_w;      // weights of runs of rows: [segments][units][t_pad]
   int segments;
   int* err;
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         if (v != 0x7fffffff) atomicMin(&s_bad[e % nb], v);
       }
     }
-    float less = 0.f, high = -INFINITY, sum = 0.f;  // minus the maximum (0 while there is none); 8 above it, as the products give scores
+    float less = 0.f, high = -INFINITY, sum = 0.f;  // minus the reference (0 while there is none); 8 above the maximum, as the products give scores
     for (int u = w.from; u < w.to; ++u, ++count) {
       const bool ok = mbar_wait(smem_u32(&bars[B_S + (count & 1)]), (uint32_t)(count >> 1) & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
       tc_fence_after();
@@ -513,13 +513,14 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
       };
       step();
       if (__any_sync(0xffffffffu, top > high)) {
-        const bool none = high == -INFINITY;
-        float now = top * f;
-        if (!none) now = fmaxf(now, -less);
-        const float k = none ? 0.f : ex2(-less - now);
-        less = now == -INFINITY ? 0.f : -now;
-        high = (now + 8.f) / f;
-        sum *= k;
+        float k = 1.f;
+        if (top > high) {
+          const float now = top * f, reference = reference_of(now);
+          k = high == -INFINITY ? 0.f : ex2(-less - reference);
+          less = -reference;
+          high = (now + 8.f) / f;
+          sum *= k;
+        }
         if (u > w.from) {
           // the output as the product before left it (this step's waits for this warp's probabilities)
           const bool done = mbar_wait(smem_u32(&bars[B_V]), (uint32_t)(count - 1) & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
@@ -579,7 +580,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
           }
         }
       }
-      if (p.weights && r < rows) a.row_stats[(size_t)w.unit * a.r_pad + r].y = limit ? log2f(sum) - less : INFINITY;
+      if (p.weights && r < rows) a.row_stats[(size_t)w.unit * a.r_pad + r].y = limit ? log2f(sum * (1.f / LIFT_FACTOR)) - (less - LIFT) : INFINITY;
     } else {
       const size_t place = ((size_t)blockIdx.x * 2 + (w.first == 0)) * PR_ROWS + in_tile;
       float* to = a.part_o + place * HD;
@@ -646,7 +647,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const prompt_args a, i
 #pragma unroll 4
   for (int b = first; b <= last; ++b) {
     const float2 ml = a.part_ml[place(b)];
-    const float k = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // (a maximum of nothing: sums of 0, or of NaN)
+    const float k = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // (a reference of nothing: sums of 0, or of NaN)
     l += ml.y * k;
     const float* from = a.part_o + place(b) * HD + lane * EACH;
     if constexpr (EACH == 4) {
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const prompt_args a, i
   const float rl = s_bad[lane * EACH / p.c.bs] < limit ? __int_as_float(0x7fffffff) : 1.f / l;
 #pragma unroll
   for (int e = 0; e < EACH; e += 2) reinterpret_cast<uint32_t*>(out)[(lane * EACH + e) / 2] = pack2<T>(x[e] * rl, x[e + 1] * rl);
-  if (p.weights && lane == 0) a.row_stats[(size_t)unit * a.r_pad + r].y = log2f(l) + top;
+  if (p.weights && lane == 0) a.row_stats[(size_t)unit * a.r_pad + r].y = log2f(l * (1.f / LIFT_FACTOR)) + (top + LIFT);
 }
 
 // ------------------------------------------------------------------ weights

@@ -12,7 +12,7 @@
 // The order of the codes in a row (cache4.cuh) is such that a lane's words of 32 dimensions belong to one block of scales: scores are
 // scaled in binary32 per block after the product, exactly; values take their scale as halves, exactly too (7-bit scales).
 // Scores, sums and outputs are binary32; probabilities are rounded to half (2^-11) as operands.  The running maximum of a column is raised
-// only when a score passes it by 8 (powers of two): e^(s - max) up to 256 fits a half.
+// only when a score passes it by 8 (powers of two), and exponentials are formed against a reference 7 below it (cache4_attention.cuh).
 //
 // Work is dealt in chunks of 32 cached rows: those of all (sequence, key/value head, up to 16 columns) in a row, an equal run of them per
 // CTA, whatever the lengths (which only the device knows).  A warp's chunks come through a ring of its own in shared memory, one
@@ -37,9 +37,9 @@ struct step_args {
   int per_unit;          // CTAs of a unit, for a single sequence (0: chunks are dealt evenly, whatever the units)
   bool alone;            // short caches: a CTA per unit and nothing to join
   float* parts;          // [ctas][2][cols][hd] sums of runs that begin, or end, inside a unit
-  float2* part_ml;       // [ctas][2][cols] their maxima (powers of two) and sums
+  float2* part_ml;       // [ctas][2][cols] their references (powers of two) and sums
   int* part_bad;         // [ctas][2][4] first row whose values of a block are no numbers
-  float2* unit_ml;       // [units][cols] maximum and sum of units that one CTA did (weights only)
+  float2* unit_ml;       // [units][cols] reference and sum of units that one CTA did (weights only)
   float* scores;         // [n_seqs * m][n_heads][max_len], powers of two (weights only)
 };
 
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
       }
     }
 
-    // less: minus the maximum (0 while there is none); high: 8 above it, as the products give scores (minus infinity while there is none)
+    // less: minus the reference (0 while there is none); high: 8 above the maximum, as the products give scores (minus infinity while there is none)
     float o[NT][VW * 4][4], less[NT][2], high[NT][2], sum[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -474,15 +474,17 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
             float k[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(s[n][e], s[n][e + 2]) * f[n][e];
+              float top = fmaxf(s[n][e], s[n][e + 2]);
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-              const bool none = high[n][e] == -INFINITY;
-              if (!none) top = fmaxf(top, -less[n][e]);
-              k[e] = none ? 0.f : ex2(-less[n][e] - top);
-              less[n][e] = top == -INFINITY ? 0.f : -top;
-              high[n][e] = (top + 8.f) / f[n][e];
+              k[e] = 1.f;
+              if (top > high[n][e]) {
+                const float now = top * f[n][e], reference = reference_of(now);
+                k[e] = high[n][e] == -INFINITY ? 0.f : ex2(-less[n][e] - reference);
+                less[n][e] = -reference;
+                high[n][e] = (now + 8.f) / f[n][e];
+              }
               sum[n][e] *= k[e];
             }
 #pragma unroll
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
 #pragma unroll
       for (int w = 0; w < ST_WARPS; ++w) {
         const float2 ml = s_ml[w][c];
-        const float k = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // (a maximum of nothing: sums of 0, or of NaN)
+        const float k = ml.x == -INFINITY ? 1.f : ex2(ml.x - top);  // (a reference of nothing: sums of 0, or of NaN)
         const float2 v = s_o[w * (NT * VW * 256) + e];
         l += ml.y * k;
         x += v.x * k;
@@ -602,8 +604,8 @@ __global__ void __launch_bounds__(ST_THREADS, NT == 1 ? 2 : 1) attention_step_ke
             for (int w = 0; w < ST_WARPS; ++w) top = fmaxf(top, s_ml[w][c].x);
 #pragma unroll
             for (int w = 0; w < ST_WARPS; ++w) l += s_ml[w][c].y * (s_ml[w][c].x == -INFINITY ? 1.f : ex2(s_ml[w][c].x - top));
-            fin[n][e] = top;
-            rl[n][e] = 1.f / l;
+            fin[n][e] = top + LIFT;
+            rl[n][e] = LIFT_FACTOR / l;
           }
         for (int u = 2 * (lo + warp); u < 2 * hi; u += u & 1 ? 2 * ST_WARPS - 1 : 1) {
           float add[2] = {0.f, 0.f};
@@ -680,7 +682,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step
     if (lane == 0) s_warp[tid >> 5] = top;
     __syncthreads();
     top = fmaxf(fmaxf(s_warp[0], s_warp[1]), fmaxf(s_warp[2], s_warp[3]));
-    for (int b = ctas.x + tid; b <= ctas.y; b += JOIN_THREADS) s_k[b - ctas.x] = s_k[b - ctas.x] == -INFINITY ? 1.f : ex2(s_k[b - ctas.x] - top);  // (a maximum of nothing: sums of 0, or of NaN)
+    for (int b = ctas.x + tid; b <= ctas.y; b += JOIN_THREADS) s_k[b - ctas.x] = s_k[b - ctas.x] == -INFINITY ? 1.f : ex2(s_k[b - ctas.x] - top);  // (a reference of nothing: sums of 0, or of NaN)
     __syncthreads();
     const int pair = tid % LANES, of = tid / LANES;
     float x = 0.f, y = 0.f;
@@ -740,7 +742,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step
         }
         all.y = warp_sum(all.y);
       }
-      if (lane == 0) s_fin[c - c64] = make_float2(all.x, 1.f / all.y);
+      if (lane == 0) s_fin[c - c64] = make_float2(all.x + LIFT, LIFT_FACTOR / all.y);  // (maximum, and the sum's inverse against it)
     }
     __syncthreads();
     for (int c = c64; c < min(n_cols, c64 + 64); ++c) {
