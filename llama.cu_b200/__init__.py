@@ -331,6 +331,12 @@ def _need(ok, words):
         raise LcuError(words)
 
 
+def _int32(who, a):
+    """Whole numbers of a host array as the library takes them."""
+    _need(a.dtype.kind in "iu" and (a.size == 0 or (a.min() >= -2 ** 31 and a.max() < 2 ** 31)), f"{who}: {a.dtype} numbers that 32-bit ones do not hold")
+    return a.astype(np.int32, copy=False)
+
+
 def _pointers(buffers):
     return (vp * len(buffers))(*[b.ptr for b in buffers])
 
@@ -370,15 +376,16 @@ class Cache4:
 
     def _per_seq(self, a):
         a = np.ascontiguousarray(a)
-        _need(a.shape == (self.n_seqs,) and a.dtype.kind in "iu", f"Cache4: {a.shape} numbers of {a.dtype} for {self.n_seqs} sequences")
-        return a.astype(np.int32)
+        _need(a.shape == (self.n_seqs,), f"Cache4: {a.shape} numbers for {self.n_seqs} sequences")
+        return _int32("Cache4", a)
 
     def _rows(self, a, width):
         """Rows of the call, [seqs, m, heads * hd]; width None: any number of heads."""
-        a = np.ascontiguousarray(a, np.uint16)
+        a = np.ascontiguousarray(a)
+        _need(a.dtype.kind in "iu", f"Cache4: rows of {a.dtype}, not 16-bit patterns")  # (numbers would be cut to whole ones)
         _need(a.ndim == 3 and a.size > 0 and a.shape[0] == self.n_seqs and a.shape[2] % self.hd == 0 and width in (None, a.shape[2]),
               f"Cache4: rows {a.shape} for {self.n_seqs} sequences and heads of {self.hd}")
-        return a
+        return a.astype(np.uint16, copy=False)
 
     def append(self, q, k, v, theta=10000.0):
         """Rows q [seqs, m, heads * hd], k, v [seqs, m, kv * hd] at the sequences' ends; returns the rotated queries.  `advance` counts them."""
@@ -423,7 +430,7 @@ class Cache4:
 
     def reorder(self, parents):
         """Sequences as beams of groups, parents [groups, beams]: beam b goes on from beam parents[g, b]."""
-        parents = np.ascontiguousarray(parents, np.int32)
+        parents = _int32("Cache4", np.ascontiguousarray(parents))
         _need(parents.ndim == 2 and parents.size == self.n_seqs, f"Cache4: parents {parents.shape} for {self.n_seqs} sequences")
         groups, beams = parents.shape
         lengths = self._per_seq(self.lengths)

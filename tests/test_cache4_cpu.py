@@ -226,3 +226,22 @@ def test_cache_of_senseless_sizes(change):
 def test_beam_selection_refuses_arrays_of_other_shapes(logits, scores, n_out, dtype):
     with pytest.raises(lcu.LcuError, match="beam_select"):
         lcu.beam_select(logits, scores, n_out, dtype)
+
+
+@pytest.mark.parametrize("call", [
+    lambda c: c.append(rows(4, 1, 256).view(np.float16), rows(4, 1, 128), rows(4, 1, 128)),  # numbers, which would be cut to whole ones
+    lambda c: c.append(rows(4, 1, 256), rows(4, 1, 128).astype(np.float32), rows(4, 1, 128)),
+    lambda c: c.append(rows(4, 1, 256), rows(4, 1, 128), rows(4, 1, 128).astype(np.float64)),
+    lambda c: c.attend(np.full((4, 1, 256), 0.7, np.float16)),
+    lambda c: c.reorder(np.full((1, 4), 0.9)),
+    lambda c: c.reorder(np.full((1, 4), 2 ** 32)),                                           # would be beam 0
+    lambda c: c.read(1, first=np.full(4, 2 ** 32 + 1))])
+def test_cache_refuses_numbers_that_are_no_bit_patterns_or_whole_ones(call):
+    with pytest.raises(lcu.LcuError, match="Cache4: .*(patterns|do not hold)"):
+        call(cache_without_planes())
+
+
+@pytest.mark.parametrize("change", [dict(lengths=np.full(4, 2 ** 32)), dict(positions=np.full(4, -2 ** 31 - 1))])
+def test_cache_refuses_lengths_beyond_32_bits(change):
+    with pytest.raises(lcu.LcuError, match="Cache4: .*do not hold"):
+        cache_without_planes(**change).append(rows(4, 1, 256), rows(4, 1, 128), rows(4, 1, 128))
