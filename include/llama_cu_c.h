@@ -175,8 +175,8 @@ int lcu_attention_cache4(void* out_dev, int ld_out, void* weights_dev, float bet
  * their order: kept [n_seqs][n_kv_heads][keep] lists them, -1 behind the last (sequences of up to keep rows keep all).  Row kept[i] of every
  * plane moves to row i.  A plane is [n_seqs][n_kv_heads][ctx_len] rows of row_bytes[i] bytes (even, up to 65536; codes, scales, halves, the
  * weights themselves); up to 8 of them (0: only the list is wanted); host arrays of device pointers.  Each destination,
- * [n_seqs][n_kv_heads][dst_ctx_len], is its source (dst_ctx_len = ctx_len then) or does not overlap any source; its rows behind the last kept
- * one stay as they are.  lengths_out (NULL: not wanted; may be lengths) = min(lengths, keep).  Keys stay rotated as they are: new rows go on
+ * [n_seqs][n_kv_heads][dst_ctx_len], is its source (dst_ctx_len = ctx_len then) or does not overlap any source, and overlaps no other destination
+ * (others are refused); its rows behind the last kept one stay as they are.  lengths_out (NULL: not wanted; may be lengths) = min(lengths, keep).  Keys stay rotated as they are: new rows go on
  * at the position that the sequence had, which lcu_cache4_append takes beside the length.  All heads of a sequence keep as many rows. */
 int lcu_cache_evict(void* const* dst_planes, const void* const* src_planes, const int* row_bytes, int n_planes, const void* weights_dev,
                     int32_t* kept_dev, int32_t* lengths_out_dev, const int32_t* lengths_dev, int n_seqs, int n_kv_heads, int ctx_len, int dst_ctx_len,
@@ -193,7 +193,7 @@ int lcu_beam_select(int32_t* parents_dev, int32_t* tokens_dev, float* scores_out
                     int n_groups, int beams, int n_vocab, int n_out, void* workspace_dev, uint64_t workspace_bytes, void* stream);
 /* The caches follow: rows 0 .. lengths[parent] of sequence g * beams + parents[g][b] go to sequence g * beams + b, in planes as above
  * ([n_groups * beams][n_kv_heads][ctx_len] rows); other rows stay as they are.  lengths [n_groups * beams] are those before the step.  A plane whose
- * destination is its source is permuted in place, any other destination must not overlap a source.  A parent outside 0 .. beams - 1
+ * destination is its source is permuted in place, any other destination must not overlap a source, nor any two each other (refused).  A parent outside 0 .. beams - 1
  * leaves the destination's sequence as it is. */
 int lcu_cache_reorder(void* const* dst_planes, const void* const* src_planes, const int* row_bytes, int n_planes, const int32_t* parents_dev,
                       const int32_t* lengths_dev, int n_groups, int beams, int n_kv_heads, int ctx_len, void* stream);

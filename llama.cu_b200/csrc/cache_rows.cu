@@ -397,6 +397,22 @@ __global__ void __launch_bounds__(256) reorder_permute_kernel(const reorder_args
   else permute_run<uint16_t, B>(a, p, group, head, lo, hi);
 }
 
+// `src_rows`, `dst_rows`: of a whole plane.  Planes are moved by separate CTAs in any order: a destination that another plane reads or writes would be a
+// race.  (Only where a plane goes to others and is moved in place too, the copies come first.)
+int check_overlaps(const char* who, void* const* dst, const void* const* src, const int* row_bytes, int n, unsigned long long dst_rows, unsigned long long src_rows) {
+  auto apart = [](const void* a, unsigned __int128 na, const void* b, unsigned __int128 nb) {  // (2^51 rows of 2^16 bytes at most)
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y ? y - x >= na : x - y >= nb;
+  };
+  for (int i = 0; i < n; ++i)
+    for (int j = 0; j < n; ++j) {
+      const unsigned __int128 to = (unsigned __int128)dst_rows * row_bytes[i];
+      LCU_REQUIRE(i <= j || apart(dst[i], to, dst[j], (unsigned __int128)dst_rows * row_bytes[j]), "%s: the destinations of planes %d and %d overlap", who, j, i);
+      LCU_REQUIRE(dst[i] == src[i] || apart(dst[i], to, src[j], (unsigned __int128)src_rows * row_bytes[j]), "%s: the destination of plane %d overlaps the source of plane %d", who, i, j);
+    }
+  return LCU_OK;
+}
+
 int check_planes(const char* who, void* const* dst, const void* const* src, const int* row_bytes, int n) {
   LCU_REQUIRE(n >= 1 && n <= MAX_CACHE_PLANES && dst && src && row_bytes, "%s: %d planes (1 to %d)", who, n, MAX_CACHE_PLANES);
   for (int i = 0; i < n; ++i) {
@@ -421,6 +437,7 @@ int launch_cache_evict(const evict_params& p, cudaStream_t stream) {
   LCU_REQUIRE(p.keep >= 1 && p.keep <= p.dst_ctx && p.keep <= p.ctx && p.recent >= 0 && p.recent <= p.keep,
               "cache_evict: keep %d rows (%d of them the latest) of %d into %d", p.keep, p.recent, p.ctx, p.dst_ctx);
   const int heads = p.n_seqs * p.n_kv;
+  if (int rc = check_overlaps("cache_evict", p.dst, p.src, p.row_bytes, p.n_planes, (unsigned long long)heads * p.dst_ctx, (unsigned long long)heads * p.ctx)) return rc;
   gather_args away{}, here{};
   int n_away = 0, n_here = 0, widest_away = 0, widest_here = 0;
   for (int i = 0; i < p.n_planes; ++i) {
@@ -489,6 +506,9 @@ int launch_cache_reorder(const reorder_params& p, cudaStream_t stream) {
   LCU_REQUIRE(p.n_groups >= 1 && p.beams >= 1 && p.beams <= MAX_BEAMS, "cache_reorder: %d groups of %d beams (1 to %d)", p.n_groups, p.beams, MAX_BEAMS);
   LCU_REQUIRE(p.n_kv >= 1 && p.ctx >= 1 && p.ctx < (1 << 26) && (long long)p.n_groups * p.beams * p.n_kv < (1 << 20), "cache_reorder: %d groups of %d beams, %d heads of %d rows",
               p.n_groups, p.beams, p.n_kv, p.ctx);
+  const unsigned long long all_rows = (unsigned long long)p.n_groups * p.beams * p.n_kv * p.ctx;
+  rc = check_overlaps("cache_reorder", p.dst, p.src, p.row_bytes, p.n_planes, all_rows, all_rows);
+  if (rc) return rc;
   reorder_args away{}, here{};
   int n_away = 0, n_here = 0;
   size_t widest_away = 0, widest_here = 0;

@@ -245,3 +245,33 @@ def test_cache_refuses_numbers_that_are_no_bit_patterns_or_whole_ones(call):
 def test_cache_refuses_lengths_beyond_32_bits(change):
     with pytest.raises(lcu.LcuError, match="Cache4: .*do not hold"):
         cache_without_planes(**change).append(rows(4, 1, 256), rows(4, 1, 128), rows(4, 1, 128))
+
+
+HEAD = 64 * 64  # bytes of a head's 64 rows of 64
+
+
+@pytest.mark.parametrize("dst,src,rb,dctx,words", [
+    ([0, 0], [0, 0], [64, 64], 64, "destinations of planes 0 and 1"),                            # the same plane twice
+    ([8 * HEAD, 8 * HEAD], [0, 2 * HEAD], [64, 64], 64, "destinations of planes 0 and 1"),
+    ([8 * HEAD, 9 * HEAD - 64], [0, 2 * HEAD], [32, 64], 64, "destinations of planes 0 and 1"),  # the last row of one
+    ([HEAD], [0], [64], 64, "plane 0 overlaps the source of plane 0"),                           # moved on by a head
+    ([2 * HEAD - 64], [0], [64], 16, "plane 0 overlaps the source of plane 0"),
+    ([8 * HEAD, 2 * HEAD], [0, 2 * HEAD + 64], [64, 64], 64, "plane 1 overlaps the source of plane 1"),
+    ([2 * HEAD, 8 * HEAD], [0, 2 * HEAD], [64, 64], 64, "plane 0 overlaps the source of plane 1"),
+    ([2 * HEAD, 2 * HEAD], [0, 2 * HEAD], [64, 64], 64, "plane 0 overlaps the source of plane 1")])  # which is moved in place
+def test_planes_that_overlap_are_refused(dst, src, rb, dctx, words):
+    d, s = planes(*[A + x for x in dst]), planes(*[A + x for x in src])
+    n = len(dst)
+    refused(lcu.lib.lcu_cache_evict(d, s, (C.c_int * n)(*rb), n, A, A, None, A, 1, 2, 64, dctx, 10, 2, None), words)
+    if dctx == 64:
+        refused(lcu.lib.lcu_cache_reorder(d, s, (C.c_int * n)(*rb), n, A, A, 1, 2, 1, 64, None), words)
+
+
+def test_planes_side_by_side_are_taken():
+    """Neighbours that touch, and a plane that goes to another place and is moved in place as well."""
+    if lcu.lib.lcu_device_count() > 0:
+        pytest.skip("a GPU is present: these addresses are none")
+    d, s, rb = planes(A, A + 2 * HEAD, A + 4 * HEAD), planes(A, A + 6 * HEAD, A), (C.c_int * 3)(64, 64, 64)
+    assert lcu.lib.lcu_cache_evict(d, s, rb, 3, A, A, None, A, 1, 2, 64, 64, 10, 2, None) == 1 and b"no CUDA device" in lcu.lib.lcu_last_error()
+    assert lcu.lib.lcu_cache_reorder(d, s, rb, 3, A, A, 1, 2, 1, 64, None) == 1 and b"no CUDA device" in lcu.lib.lcu_last_error()
+    assert lcu.lib.lcu_cache_evict(d, s, rb, 2, A, A, None, A, 1 << 10, 1 << 9, 1 << 25, 1 << 25, 10, 2, None) == 2  # (planes of 2^50 bytes do overlap)
