@@ -10,7 +10,17 @@ namespace lcu {
 // however many heads share a key.
 static bool few_rows(int m, int group) { return (long long)m * group <= 64 || m == 1; }
 
+static bool sizes_fit(int n_seqs, int m, int n_heads, int n_kv, int hd) {
+  return (long long)n_seqs * n_kv < 65536 && (long long)n_heads * hd < (1 << 24) && (long long)n_seqs * m * n_heads < (1ll << 31);
+}
+// sizes that a call is not refused for (positive ones, of whole heads)
+static bool sizes_taken(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len) {
+  return (hd == 64 || hd == 128) && n_heads % n_kv == 0 && m < (1 << 26) && max_len < (1 << 26) && sizes_fit(n_seqs, m, n_heads, n_kv, hd) &&
+         (few_rows(m, n_heads / n_kv) ? attention_cache4_step_takes : attention_cache4_prompt_takes)(n_seqs, m, n_heads, n_kv, max_len);
+}
+
 size_t cache4_attention_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
+  if (!sizes_taken(n_seqs, m, n_heads, n_kv, hd, max_len)) return 0;
   if (few_rows(m, n_heads / n_kv)) return attention_cache4_step_workspace(n_seqs, m, n_heads, n_kv, hd, max_len, weights);
   return attention_cache4_prompt_workspace(n_seqs, m, n_heads, n_kv, hd, max_len, weights);
 }
@@ -23,8 +33,9 @@ int launch_attention_cache4(const cache4_attention_params& p, int dtype, void* w
   LCU_REQUIRE(p.m >= 1 && p.n_heads >= 1 && p.n_heads % p.c.n_kv == 0, "attention_cache4: %d rows, %d heads over %d key/value heads", p.m, p.n_heads, p.c.n_kv);
   LCU_REQUIRE(p.m < (1 << 26) && p.c.ctx < (1 << 26), "attention_cache4: %d rows, %d in the cache", p.m, p.c.ctx);
   LCU_REQUIRE(p.max_len >= 1 && p.max_len <= p.c.ctx, "attention_cache4: %d rows exceed the cache's %d", p.max_len, p.c.ctx);
-  LCU_REQUIRE((long long)p.n_heads * p.c.hd < (1 << 24) && (long long)p.c.n_seqs * p.m * p.n_heads < (1ll << 31) && (long long)p.c.n_seqs * p.c.n_kv < 65536,
-              "attention_cache4: %d sequences of %d rows of %d heads are too many", p.c.n_seqs, p.m, p.n_heads);
+  LCU_REQUIRE(sizes_fit(p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.c.hd), "attention_cache4: %d sequences of %d rows of %d heads are too many", p.c.n_seqs, p.m, p.n_heads);
+  LCU_REQUIRE(sizes_taken(p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.c.hd, p.max_len), "attention_cache4: %d sequences of %d rows of %d heads over %d rows are too many", p.c.n_seqs,
+              p.m, p.n_heads, p.max_len);
   LCU_REQUIRE(p.ld_q % 8 == 0 && p.ld_out % 8 == 0 && p.ld_q >= p.n_heads * p.c.hd && p.ld_out >= p.n_heads * p.c.hd,
               "attention_cache4: row strides must be multiples of 8 that hold a row");
   LCU_REQUIRE((((uintptr_t)p.q | (uintptr_t)p.out) & 15) == 0, "attention_cache4: rows must be 16-byte aligned");

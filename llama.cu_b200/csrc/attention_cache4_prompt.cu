@@ -943,14 +943,16 @@ int launch_prompt(const prompt_args& a, cudaStream_t stream) {
 
 }  // namespace
 
+bool attention_cache4_prompt_takes(int n_seqs, int m, int n_heads, int n_kv, int max_len) {
+  const long long units = (long long)n_seqs * n_kv, rows = (long long)m * (n_heads / n_kv);
+  return rows < (1ll << 30) && units * ((max_len + rows) / 128 + 2) * 16 < (1ll << 31) && units * (rows / 128 + 1) * (max_len / 128 + 1) < (1ll << 31);
+}
+
 size_t attention_cache4_prompt_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
   return prompt_layout(nullptr, nullptr, n_seqs, m, n_heads, n_kv, hd, max_len, weights);
 }
 
 int launch_attention_cache4_prompt(const cache4_attention_params& p, int dtype, void* workspace, cudaStream_t stream) {
-  const long long units = (long long)p.c.n_seqs * p.c.n_kv, rows = (long long)p.m * (p.n_heads / p.c.n_kv);
-  LCU_REQUIRE(rows < (1ll << 30) && units * ((p.max_len + rows) / 128 + 2) * 16 < (1ll << 31) && units * (rows / 128 + 1) * (p.max_len / 128 + 1) < (1ll << 31), "attention_cache4: %d sequences of %d rows of %d heads over %d rows are too many", p.c.n_seqs,
-              p.m, p.n_heads, p.max_len);
   prompt_args a{};
   a.p = p;
   a.err = device_scratch_words();

@@ -865,13 +865,15 @@ size_t step_layout(step_args* a, void* workspace, const step_shape& w, int n_seq
 
 }  // namespace
 
+bool attention_cache4_step_takes(int n_seqs, int m, int n_heads, int n_kv, int max_len) {
+  return (long long)n_seqs * n_kv * ((m * (n_heads / n_kv) + 7) / 8) * ((max_len + ST_CHUNK - 1) / ST_CHUNK) < (1ll << 31);
+}
+
 size_t attention_cache4_step_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights) {
   return step_layout(nullptr, nullptr, step_shape(n_seqs, m, n_heads, n_kv, max_len, weights), n_seqs, m, n_heads, hd, max_len, weights);
 }
 
 int launch_attention_cache4_step(const cache4_attention_params& p, int dtype, void* workspace, cudaStream_t stream) {
-  const long long chunks = (long long)p.c.n_seqs * p.c.n_kv * ((p.m * (p.n_heads / p.c.n_kv) + 7) / 8) * ((p.max_len + ST_CHUNK - 1) / ST_CHUNK);
-  LCU_REQUIRE(chunks < (1ll << 31), "attention_cache4: %d sequences of %d heads over %d rows are too many", p.c.n_seqs, p.n_heads, p.max_len);
   const step_shape w(p.c.n_seqs, p.m, p.n_heads, p.c.n_kv, p.max_len, p.weights != nullptr);
   step_args a{p, w.ctas, w.col_blocks, w.per_unit, w.alone};
   step_layout(&a, workspace, w, p.c.n_seqs, p.m, p.n_heads, p.c.hd, p.max_len, p.weights != nullptr);

@@ -275,6 +275,7 @@ int beam_chunks(int n_vocab) { return (int)ceil_div((size_t)n_vocab, BEAM_CHUNK)
 }  // namespace
 
 size_t beam_select_workspace(int n_groups, int beams, int n_vocab, int n_out) {
+  if (beams > MAX_BEAMS || n_vocab > (1 << 24) || n_out > BEAM_MAX_OUT) return 0;  // (such a call is refused)
   return (size_t)n_groups * beams * beam_chunks(n_vocab) * (sizeof(float2) + (size_t)n_out * sizeof(uint64_t));
 }
 

@@ -14,11 +14,13 @@ constexpr float LIFT = 7.f, LIFT_FACTOR = 128.f;
 __device__ __forceinline__ float reference_of(float top) { return fabsf(top) < 1048576.f ? top - LIFT : top; }
 #endif
 
-// few rows (attention_cache4_step.cu)
+// few rows (attention_cache4_step.cu); takes: whether the kernels' numbers hold the work (of sizes that fit otherwise)
+bool attention_cache4_step_takes(int n_seqs, int m, int n_heads, int n_kv, int max_len);
 size_t attention_cache4_step_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights);
 int launch_attention_cache4_step(const cache4_attention_params& p, int dtype, void* workspace, cudaStream_t stream);
 
 // prompts (attention_cache4_prompt.cu)
+bool attention_cache4_prompt_takes(int n_seqs, int m, int n_heads, int n_kv, int max_len);
 size_t attention_cache4_prompt_workspace(int n_seqs, int m, int n_heads, int n_kv, int hd, int max_len, bool weights);
 int launch_attention_cache4_prompt(const cache4_attention_params& p, int dtype, void* workspace, cudaStream_t stream);
 

@@ -275,3 +275,21 @@ def test_planes_side_by_side_are_taken():
     assert lcu.lib.lcu_cache_evict(d, s, rb, 3, A, A, None, A, 1, 2, 64, 64, 10, 2, None) == 1 and b"no CUDA device" in lcu.lib.lcu_last_error()
     assert lcu.lib.lcu_cache_reorder(d, s, rb, 3, A, A, 1, 2, 1, 64, None) == 1 and b"no CUDA device" in lcu.lib.lcu_last_error()
     assert lcu.lib.lcu_cache_evict(d, s, rb, 2, A, A, None, A, 1 << 10, 1 << 9, 1 << 25, 1 << 25, 10, 2, None) == 2  # (planes of 2^50 bytes do overlap)
+
+
+@pytest.mark.parametrize("change", [dict(heads=5), dict(hd=96), dict(most=2 ** 31 - 1), dict(most=1 << 26), dict(m=2 ** 31 - 1), dict(m=1 << 26), dict(seqs=2 ** 31 - 1),
+                                    dict(seqs=1 << 15), dict(seqs=1 << 30, m=1 << 25, heads=1 << 9), dict(heads=1 << 18), dict(m=1 << 25, heads=64),
+                                    dict(seqs=16384, m=32, most=(1 << 26) - 1), dict(seqs=16384, m=2000, heads=2, most=(1 << 26) - 1)])
+def test_workspaces_of_sizes_that_are_refused(change):
+    """0, whatever the numbers' products, and the call says so."""
+    a = {**dict(seqs=1, m=500, heads=4, kv=2, hd=128, most=100), **change}
+    for weights in (0, 1):
+        assert lcu.lib.lcu_attention_cache4_workspace(a["seqs"], a["m"], a["heads"], a["kv"], a["hd"], a["most"], weights) == 0
+    a = {**a, "ctx": a["most"], "ldq": 1 << 26, "ldo": 1 << 26}
+    assert attend(**a) == 2 and b"attention_cache4" in lcu.lib.lcu_last_error()
+
+
+def test_beam_workspaces_of_sizes_that_are_refused():
+    b = lcu.lib.lcu_beam_select_workspace
+    assert b(1, 33, 100, 4) == 0 and b(1, 4, (1 << 24) + 1, 4) == 0 and b(1, 4, 100, 65) == 0 and b(2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1) == 0
+    assert b(1, 32, 1 << 24, 64) > 0
