@@ -2,6 +2,7 @@
 // (TMA) PTX wrappers with bounded waits, programmatic-dependent-launch controls, cluster helpers.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <cuda_fp16.h>
@@ -43,11 +44,11 @@ const char* last_error();
 
 // for entry points that check their arguments before they look for a device
 inline int need_device() {
-  static bool seen = false;  // (devices do not go away)
-  if (seen) return LCU_OK;
+  static std::atomic<bool> seen{false};  // (devices do not go away; calls may come from any thread)
+  if (seen.load(std::memory_order_relaxed)) return LCU_OK;
   int n = 0;
   if (cudaGetDeviceCount(&n) == cudaSuccess && n > 0) {
-    seen = true;
+    seen.store(true, std::memory_order_relaxed);
     return LCU_OK;
   }
   cudaGetLastError();

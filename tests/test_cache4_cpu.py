@@ -293,3 +293,19 @@ def test_beam_workspaces_of_sizes_that_are_refused():
     b = lcu.lib.lcu_beam_select_workspace
     assert b(1, 33, 100, 4) == 0 and b(1, 4, (1 << 24) + 1, 4) == 0 and b(1, 4, 100, 65) == 0 and b(2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1) == 0
     assert b(1, 32, 1 << 24, 64) > 0
+
+
+def test_calls_from_several_threads_look_for_a_device():
+    """Each thread gets its own status and message."""
+    if lcu.lib.lcu_device_count() > 0:
+        pytest.skip("a GPU is present: these addresses are none")
+    from concurrent.futures import ThreadPoolExecutor
+
+    def one(i):
+        if i % 2:
+            return attend(m=0), lcu.lib.lcu_last_error()
+        return append(), lcu.lib.lcu_last_error()
+
+    with ThreadPoolExecutor(8) as pool:
+        for i, (rc, words) in enumerate(pool.map(one, range(400))):
+            assert (rc == 2 and b"0 rows" in words) if i % 2 else (rc == 1 and b"no CUDA device" in words)
