@@ -651,6 +651,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const step
   const bool join = (int)blockIdx.x < joins;
   const int sh = join ? 0 : ((int)blockIdx.x - joins) / key_blocks;
   const int seq = join ? (int)blockIdx.x / (per_seq * COLS) : sh / p.c.n_kv;
+  // Lengths are read ahead of the wait (0.4 to 0.8 us: 8 rows behind 8000 18.0 us, 18.6 behind it).  That rests on the kernel in front, which does not
+  // write them and is launched without the attribute (launch_step): whatever wrote them is done.  Nothing else is touched before the wait.
   const int held = p.lengths[seq], chunks = step_plan::chunks(p, held);
   if (!join && held < 0) return;
   unsigned before, sum_chunks;
@@ -810,7 +812,7 @@ int launch_step(const step_args& a, cudaStream_t stream) {
     LCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
     if (dev < 16) attr_done[dev] = true;
   }
-  kernel<<<a.ctas, ST_THREADS, SMEM, stream>>>(a);
+  kernel<<<a.ctas, ST_THREADS, SMEM, stream>>>(a);  // (behind everything: attention_join_kernel reads lengths without waiting for it)
   if (a.alone && (!WEIGHTS || a.col_blocks == 1)) {
     LCU_CUDA(cudaGetLastError());
     return LCU_OK;

@@ -75,7 +75,8 @@ __device__ __forceinline__ float silu_of_half(float a) { return __fdividef(a, 1.
 // Programmatic dependent launch for the kernels of a prompt pass: with the attribute a kernel's CTAs may start - set up
 // barriers, allocate tensor memory, fetch descriptors - while the kernel before it in the stream drains.  Every kernel
 // launched this way executes griddepcontrol.wait (pdl_wait) before it touches global memory, so its body still runs
-// after the previous kernel has completed and flushed.  prompt_pdl() = 0 turns the attribute off.
+// after the previous kernel has completed and flushed.  (A kernel that reads something earlier says what makes that safe.)
+// prompt_pdl() = 0 turns the attribute off.
 int& prompt_pdl();
 template <typename... KP, typename... Args>
 cudaError_t launch_after(void (*kernel)(KP...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
