@@ -132,15 +132,17 @@ int lcu_logits_head(void* probs_dev, const void* logits_dev, int n_vocab, float 
 /* ---- long contexts: a cache in 4 bits, eviction, beams ---------------------------------------- */
 /* No counterpart in the reference, whose caches are halves and whose client runs one sequence.  dtype of these operators: 0 half,
  * 1 bfloat16, 2 binary32 (logits only).  Lengths and positions are read on the device (a captured step replays with new ones) and
- * are the caller's to advance.  No call waits or keeps anything, and none allocates but the first attention of more than 64 (row, query head) pairs per key/value
- * head on a device, which takes 256 bytes for the operators' error word (make one outside stream capture; kernels are loaded then, too).
+ * are the caller's to advance.  No call waits, allocates or keeps anything but the first attention of more than 64 (row, query head) pairs per key/value
+ * head on a device, which takes 256 bytes for the operators' error word and waits for the default stream (make one outside stream capture; kernels are loaded then, too).
+ * Pointers and streams are the current device's.
  * Workspaces belong to the caller, 16-byte aligned, with any contents, and calls that may overlap on the GPU need one each.  Arguments are
  * checked before anything is launched.
  *
  * A 4-bit cache of one layer is four planes, 16-byte aligned: codes, u8 [n_seqs][n_kv_heads][ctx_len][head_dim / 2], and scales, half
  * [n_seqs][n_kv_heads][ctx_len][head_dim / bs], for keys and for values.  head_dim 64 or 128; bs 32, 64 or 128, at most head_dim.
  * With a the largest magnitude of a block of bs neighbouring dimensions the scale s is a / 7.5 rounded to 7 significant bits, at most
- * 8704; x becomes floor(x / s + 8) within 0 .. 15 (8 where s is 0) and stands for (code - 7.5) * s, which a half holds exactly.  A block
+ * 8704; x becomes floor(x / s + 8) within 0 .. 15 (8 where s is 0) and stands for (code - 7.5) * s, which a half holds exactly from s = 2^-17 on
+ * (attention takes smaller values off by up to 2^-24).  A block
  * with an infinity or a NaN gets the scale NaN: rows that see it come out as NaN, others do not.  The codes of dimensions
  * 32 g + 8 o .. + 7 are the nibbles, lowest first, of the row's little-endian 32-bit word o * (head_dim / 32) + g. */
 /* The counterpart of lcu_rope_scatter: m new rows for each of n_seqs sequences.  Row i of sequence s (row s * m + i of q, k_new and v_new,
@@ -162,6 +164,8 @@ int lcu_cache4_read(void* k_out_dev, void* v_out_dev, const void* k_codes_dev, c
  * not seen).  A row that sees nothing (a negative length) gives zeros.
  * Scores, maxima, sums and accumulators are binary32.  Probabilities become halves for their product with the values: off by 2^-11 of themselves,
  * or by 2^-32 of the row's largest where they are smaller than 2^-21 of it.
+ * Queries become halves times a power of two of their row, off by at most 2^-25 of its largest element (bfloat16 only), which may be
+ * up to 2^103.  Scores times log2 e are in range up to 2^27 either way; rows with larger ones may come out as NaN.
  * weights (NULL: not wanted), binary32 [n_seqs][n_kv_heads][ctx_len]: = beta * weights + the probabilities that the cached row received from
  * all m rows and the heads that read it, summed in a fixed order.  The call's own rows, from lengths[s] on, start from nothing, whatever
  * their entries held; with beta 0 all do.  Entries of rows that none sees stay as they are.  The workspace is lcu_attention_cache4_workspace bytes (0 where none is needed). */

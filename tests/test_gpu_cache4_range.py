@@ -87,6 +87,32 @@ def test_scores_of_tens_of_thousands(lcu, dtype, hd, bs, seqs, m, lengths, heads
                 assert (np.abs(w[:, :rows] - want) <= (0.00272 + 2.0 ** -19) * want + 1e-28).all() and (w[:, rows:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m,held,heads,kv", [(1, 200, 4, 2), (3, 900, 8, 2), (140, 60, 4, 2)])
+def test_values_below_the_normal_halves(lcu, dtype, m, held, heads, kv):
+    """Scales from 2^-24 to 2^-17 under queries of thousands.  A value is off by 2^-24 at most, an output below the normal halves by 2^-25 more; keys as
+    halves (prompts) are off by 2^-25, scores by the queries' sum of that, 8e-4, and the outputs by twice that of values of 1e-5, below 2^-25."""
+    rng = np.random.default_rng(held)
+    cache = Cache(lcu, 1, kv, 128, held + m, 32, dtype)
+    cache.fill(rng, held + m)
+    for which in range(2):
+        steps = torch.from_numpy(rng.integers(1, 128, tuple(cache.scales[0].shape)).astype(np.float32)).cuda()
+        cache.scales[which][:] = steps * 2.0 ** -24
+    assert ((cache.scales[0] > 0) & (cache.scales[0] < 2.0 ** -17)).all()
+    qb = P.float_to_bits(rng.standard_normal((m, heads * 128)) * 3000, dtype)
+    w = torch.zeros(1, kv, held + m, device="cuda")
+    q = P.bits_to_float(qb, dtype).reshape(m, heads, 128)
+    o, p, spread, big = P.attention(q, cache.values(0)[0], cache.values(1)[0], held, heads // kv)
+    assert np.abs(q).sum(-1).max() * 2.0 ** -25 / np.sqrt(128) < 1e-3 and np.abs(cache.values(1)).max() < 6e-5
+    ds = (2 * 128 * 2.0 ** -24 * big + 8 * 2.0 ** -24 * (1 + big))[..., None]
+    for weights in (None, w):
+        out = P.bits_to_float(bits(cache.attend(tensor(qb, dtype), i32([held]), m, heads, weights=weights)), dtype).reshape(o.shape)
+        tol = P.step_of(dtype) * np.abs(o) + (2.0 ** -11 + 2 * ds + 2.0 ** -20 + (2e-3 if m * heads // kv > 64 else 0)) * spread * 1.01 + 2.0 ** -24 + 2.0 ** -25
+        assert (np.abs(out - o) <= tol).all(), float((np.abs(out - o) / tol).max())
+    want = p.reshape(kv, -1, held + m).sum(1)
+    assert (np.abs(w[0].double().cpu().numpy() - want) <= (2 * ds.max() + 2.0 ** -19 + 2e-3) * want + 2.0 ** -40).all()
+
+
 def test_a_cache_is_evicted_twice(lcu):
     """A cache that fills up two times: positions run further ahead of lengths each time, kept rows and their weights follow the lists."""
     seqs, kv, heads, hd, bs, ctx, keep, recent, dtype = 2, 2, 4, 64, 32, 40, 17, 5, "float16"
