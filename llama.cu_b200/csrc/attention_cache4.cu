@@ -5,8 +5,8 @@
 namespace lcu {
 
 // Up to 64 (row, query head) pairs per key/value head go to the kernel that walks the codes, 16 of them a time.  One sequence, 8 key heads x 4
-// queries each: 8 rows behind 8000 / 30000 17 / 32 us against 42 / 79 on tcgen05, 16 rows 26 / 54 against 42 / 80; 32 heads with a key each:
-// 64 rows behind 500 / 8000 / 30000 11 / 59 / 169 against 21 / 79 / 224, 96 rows 21 / 87 / 256 against 22 / 79 / 224.  A single row always does,
+// queries each: 8 rows behind 8000 / 30000 18 / 35 us against 43 / 81 on tcgen05, 16 rows 28 / 58 against 44 / 84; 32 heads with a key each:
+// 64 rows behind 500 / 8000 / 30000 12 / 63 / 180 against 21 / 81 / 230, 96 rows 22 / 93 / 268 against 23 / 80 / 230.  A single row always does,
 // however many heads share a key.
 static bool few_rows(int m, int group) { return (long long)m * group <= 64 || m == 1; }
 

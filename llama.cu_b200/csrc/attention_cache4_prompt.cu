@@ -7,12 +7,13 @@
 //
 // One CTA per (sequence, key/value head, 128 rows), two CTAs per SM, in steps of 64 keys.  Scores lie in two buffers of tensor memory: those of
 // the next step are formed under this step's exponentials (in one buffer, steps of 128 keys, score - exponential - product followed one
-// another: 2000 rows of 32 heads behind 6000 rows of 8, timed in turn, took 294 us instead of 264, 4000 rows 190 instead of 165).  Three accumulators' columns
+// another: timed in turn, 2000 rows of 32 heads behind 6000 rows of 8 took a ninth longer, 4000 rows a seventh).  Three accumulators' columns
 // for two CTAs are what tensor memory holds; narrower products of the scores read their queries from shared memory more often, 1.5 x the time.
 // A thread owns a row, reads 32 keys at a time and keeps the running maximum and the sum; probabilities go back to tensor memory, over the
 // scores, as halves: the A operand of the product with the values, whose accumulator stays in tensor memory.  A maximum is raised only
-// when a score passes it by 8 (powers of two), so that the exponentials of a step are formed with the old one while its own maximum is
-// looked for; only where a row fails that test is its warp's step done again and the output rescaled, once the product before is done.
+// when a score passes it by 8 (powers of two; the reference of the exponentials is 7 below it, cache4_attention.cuh), so that a step's
+// exponentials are formed with the old one while its own maximum is looked for; only where a row fails that test is its warp's step done again and
+// the output rescaled, once the product before is done.
 // Exponentials (16 a cycle and SM) and products are both busy 55 % of the time that a CTA is there.
 //
 // Weights: once maxima and sums are known, a second kernel forms the scores the other way round - a thread owns a cached row - and adds
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(PR_THREADS, 2) prompt_attention_kernel(const _
         tc_ring next = r;
         next.step(RING);
         // (products of different shapes are not promised to run in the order of issue: what the next scores replace must have been read;
-        // left to that order, 2000 rows behind 6000 took 262 us instead of 271 in turn, others the same)
+        // left to that order, 2000 rows behind 6000 took 3 % less in turn, others the same)
         if (u > w.from) ok = ok && mbar_wait_warp(smem_u32(&bars[B_V]), (uint32_t)(count - 1) & 1u, a.err, DEV_ERR_TMEM_WAIT, HEED);
         if (ok && u + 1 < w.to) scores(next, (count + 1) & 1);
         ok = ok && mbar_wait_warp(smem_u32(&bars[B_P + (count & 1)]), (uint32_t)(count >> 1) & 1u, a.err, DEV_ERR_FULL_WAIT, HEED);
@@ -845,8 +846,8 @@ __global__ void __launch_bounds__(PW_THREADS, 2) prompt_weights_kernel(const __g
 // ------------------------------------------------------------------ host
 // How the work is shared, from the sizes as the host knows them.  A CTA per item leaves slots idle where items are few or their last wave is
 // half full; an equal share of all tiles per CTA costs each the start of another run, the partial sums of two and their join, about what
-// eight tiles take.  8 key heads x 4 queries each: 50 rows behind 30000 481 us per item, 96 shared; 300 behind 4000 89 and 57; 500 behind
-// 2000 53 and 55; 2000 behind 6000 (504 items of 47 to 63 tiles, 296 slots) 244 and 292.
+// eight tiles take.  8 key heads x 4 queries each, in turn: 50 rows behind 30000 507 us per item, 98 shared; 300 behind 4000 89 and 57; 500 behind
+// 2000 54 and 55; 2000 behind 6000 (504 items of 47 to 63 tiles, 296 slots) 259 and 280.
 struct prompt_plan {
   int ctas, segments;
   prompt_plan(int n_seqs, int m, int n_heads, int n_kv, int max_len) {

@@ -7,7 +7,7 @@
 // made in registers:
 //   keys: a masked nibble is a half already, the subnormal code * 2^-24 (or * 2^-20, four bits further up; those dimensions' queries
 //     are a sixteenth).  The 7.5 is a product with the column's sum of queries, where the accumulator starts.  Where weights are wanted,
-//     code - 7.5 is formed instead: the products' sums then cancel less, and weights are 1.4e-7 off (2-norm) instead of 8e-7, for 1 us of 58.
+//     code - 7.5 is formed instead: the products' sums then cancel less, and weights are 1.2e-7 off (2-norm) instead of 8e-7, for 1 us of 58.
 //   values: bits or'ed below an exponent are 1024 + code (or 64 + code); less the constant, times the scale, less 7.5 scales: exact.
 // The order of the codes in a row (cache4.cuh) is such that a lane's words of 32 dimensions belong to one block of scales: scores are
 // scaled in binary32 per block after the product, exactly; values take their scale as halves, exactly too (7-bit scales).
@@ -789,9 +789,9 @@ struct step_shape {
     per_unit = n_seqs == 1 && (each >= 6 || (each && each * ST_WARPS * units >= chunks)) ? (int)each : 0;
     if (per_unit) ctas = (int)(per_unit * units);
     // Short caches: a CTA per unit, one launch.  Its rounds of eight chunks (1.5 us each) against the even deal's other overheads, which grow
-    // with the units; the weights' second look at the scores costs as much again.  Alone / shared, us: 32 units x 500 rows 7.5 / 8.5,
-    // 700 8.9 / 8.9, 1000 10.7 / 9.6; 64 x 1400 13.3 / 15.3, 2000 16.3 / 16.7; 512 x 3000 52 / 63; with weights 32 x 250 8.3 / 9.2, 500
-    // 11.6 / 9.4; 64 x 500 13.8 / 15.2; 512 x 1000 42 / 45.
+    // with the units; the weights' second look at the scores costs as much again.  Alone / shared, us: 32 units x 400 rows 7.9 / 9.0,
+    // 600 8.9 / 9.4, 650 to 720 a tie at 9.5 (one launch less for the host), 770 10.6 / 9.6, 1000 11.3 / 9.7; 64 x 1000 11.3 / 15.2, 1300 13.6 / 14.9,
+    // 2000 16.3 / 16.7; 512 x 3000 52 / 63; with weights 32 x 250 8.9 / 9.6, 300 11.1 / 9.8; 64 x 500 12.1 / 14.0; 512 x 1000 42 / 45.
     alone = chunks / units <= (weights ? 8 * std::min(4ll, std::max(1ll, units / 32)) : 22 * std::min(8ll, std::max(1ll, units / 32)));
     if (alone) {
       per_unit = 0;

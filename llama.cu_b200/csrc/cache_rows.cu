@@ -279,7 +279,9 @@ __global__ void __launch_bounds__(256) evict_gather_kernel(const gather_args a, 
 
 // Rows to the front of the same plane.  Kept rows only move down and stay in order, so row i may be written once every row up to the
 // i-th kept one has been read: a CTA walks a column of a head's rows in steps, reads a step, waits, writes it.  A step's targets lie
-// below every later step's sources.  Columns of 32 bytes (a sector) are independent: they are what runs side by side.
+// below every later step's sources.  Columns of 32 bytes (a sector) are independent: they are what runs side by side.  Bound by the chain of
+// steps of a column where heads are few: the five planes of a 4-bit cache (rows of 64, 8, 64, 8 and 4 bytes) of 4 x 8 heads, 16000 to 8001 rows, take 73 us,
+// 12 of them the selection, for 12 us of bytes; 16 x 8 heads 136 for 48; 32 heads, 2048 to 1024 12.0 for 1.5.
 constexpr int MOVE_UNROLL = 8;
 template <typename V>
 __device__ __forceinline__ void move_rows(const gather_args& a, const plane& p, int sh, int col, int col_units) {
@@ -364,7 +366,8 @@ __global__ void __launch_bounds__(256) reorder_copy_kernel(const reorder_args a,
   for (size_t b = done + 2 * threadIdx.x; b < hi; b += 512) *reinterpret_cast<uint16_t*>(dst + b) = *reinterpret_cast<const uint16_t*>(src + b);
 }
 
-// In place: a thread owns one place in all beams of a group, reads what every beam takes there and then writes.
+// In place: a thread owns one place in all beams of a group, reads what every beam takes there and then writes.  The five planes of a 4-bit
+// cache: 8 x 4 beams, 8 heads x 1000 rows 15.8 us for 8.7 of bytes, 4 x 16 beams, 4 x 500 13.8 for 5.5, 4 beams, 32 heads x 16000 92 for 62.
 template <typename V, int B>
 __device__ __forceinline__ void permute_run(const reorder_args& a, const plane& p, int group, int head, size_t lo, size_t hi) {
   const size_t head_units = (size_t)a.ctx * p.row_bytes / sizeof(V), seq_units = head_units * a.n_kv;
