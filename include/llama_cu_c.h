@@ -165,7 +165,8 @@ int lcu_cache4_read(void* k_out_dev, void* v_out_dev, const void* k_codes_dev, c
  * Scores, maxima, sums and accumulators are binary32.  Probabilities become halves for their product with the values: off by 2^-11 of themselves,
  * or by 2^-32 of the row's largest where they are smaller than 2^-21 of it.
  * Queries become halves times a power of two of their row, off by at most 2^-25 of its largest element (bfloat16 only), which may be
- * up to 2^103.  Scores times log2 e are in range up to 2^27 either way; rows with larger ones may come out as NaN.
+ * up to 2^103.  Scores times log2 e are in range up to 2^26 either way (as binary32 numbers, 2^-24 of themselves off);
+ * rows with larger ones may come out as NaN.
  * weights (NULL: not wanted), binary32 [n_seqs][n_kv_heads][ctx_len]: = beta * weights + the probabilities that the cached row received from
  * all m rows and the heads that read it, summed in a fixed order.  The call's own rows, from lengths[s] on, start from nothing, whatever
  * their entries held; with beta 0 all do.  Entries of rows that none sees stay as they are.  The workspace is lcu_attention_cache4_workspace bytes (0 where none is needed). */

@@ -88,6 +88,30 @@ def test_scores_of_tens_of_thousands(lcu, dtype, hd, bs, seqs, m, lengths, heads
 
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m,held,heads,kv", [(1, 200, 6, 2), (4, 3000, 8, 2), (130, 0, 4, 2), (40, 2500, 8, 4), (300, 40, 16, 16)])
+def test_scores_up_to_the_end_of_their_range(lcu, dtype, m, held, heads, kv):
+    """Scores (powers of two) up to 2^26, of queries that are 8192 times a key's steps, exact as above; the rows that see one key alone have it with the
+    other sign.  Outputs are the key's values: a probability rounded to a half, sums 2^-20, one rounding."""
+    rng = np.random.default_rng(m)
+    cache = Cache(lcu, 1, kv, 128, held + m, 32, dtype)
+    cache.scales[0][:], cache.scales[1][:] = 16.0, 0.5
+    k, v = cache.values(0)[0], cache.values(1)[0]
+    q, want = np.zeros((m, heads, 128)), np.zeros((m, heads, 128))
+    for i in range(m):
+        for h in range(heads):
+            d = rng.integers(0, held + i + 1)
+            q[i, h] = k[h // (heads // kv), d] * (512 if held + i else -512)
+            want[i, h] = v[h // (heads // kv), d]
+            score = k[h // (heads // kv), :held + i + 1] @ q[i, h] * (1.4426950408889634 / np.sqrt(128))
+            assert 2 ** 24 < abs(score[d]) < 2 ** 26 and (np.delete(score, d) < score[d] - 2 ** 20).all()
+    qb = P.float_to_bits(q.reshape(m, heads * 128), dtype)
+    assert np.array_equal(P.bits_to_float(qb, dtype).reshape(q.shape), q)
+    for weights in (None, torch.zeros(1, kv, held + m, device="cuda")):
+        out = P.bits_to_float(bits(cache.attend(tensor(qb, dtype), i32([held]), m, heads, weights=weights)), dtype).reshape(q.shape)
+        assert (np.abs(out - want) <= (P.step_of(dtype) + (2.0 ** -11 + 2.0 ** -20) * 1.01) * np.abs(want)).all(), float(np.abs(out - want).max())
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("m,held,heads,kv", [(1, 200, 4, 2), (3, 900, 8, 2), (140, 60, 4, 2)])
 def test_values_below_the_normal_halves(lcu, dtype, m, held, heads, kv):
     """Scales from 2^-24 to 2^-17 under queries of thousands.  A value is off by 2^-24 at most, an output below the normal halves by 2^-25 more; keys as
